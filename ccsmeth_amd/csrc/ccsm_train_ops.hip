@@ -1,0 +1,332 @@
+// libccsm_train: the training operators' C-ABI (include/ccsm_train_ops.h).  Checks, workspace layout and launches; the kernels are in
+// ccsm_train_ops_linear.hip, ccsm_train_ops_embed.hip and ccsm_train_ops_act8.hip.
+#include <string>
+
+#include "../../include/ccsm_train_ops.h"
+#include "ccsm_train_ops_act8.hip"
+#include "ccsm_train_ops_embed.hip"
+#include "ccsm_train_ops_linear.hip"
+
+namespace {
+
+using namespace ccsm_ops;
+
+thread_local std::string g_err;
+ccsm_status fail(ccsm_status s, const char* what) {
+    try { g_err = what; } catch (...) {}
+    return s;
+}
+ccsm_status hip_fail(hipError_t e, const char* what) {
+    try { g_err = std::string(what) + ": " + hipGetErrorString(e); } catch (...) {}
+    return CCSM_ERR_HIP;
+}
+#define REFUSE(cond, text) do { if (cond) return fail(CCSM_ERR_INVALID_ARG, text); } while (0)
+#define LAUNCHED(what) do { hipError_t e_ = hipGetLastError(); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
+
+// makes `device` current for the call, and the caller's own again behind it
+struct OnDevice {
+    int before = -1;
+    hipError_t err;
+    explicit OnDevice(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device); else if (err == hipSuccess) before = -1;
+    }
+    ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+#define ON_DEVICE(device)                      \
+    OnDevice on_device_(device);               \
+    if (on_device_.err != hipSuccess) return hip_fail(on_device_.err, "hipSetDevice")
+
+constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
+
+size_t size_of(int type) { return type == CCSM_TYPE_F32 ? 4 : 2; }
+bool good_type(int t) { return t == CCSM_TYPE_F32 || t == CCSM_TYPE_F16 || t == CCSM_TYPE_BF16; }
+bool off_by(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+size_t up(size_t n, size_t a) { return (n + a - 1) / a * a; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+unsigned grid_of(int64_t n, int64_t most = 1 << 20) { return (unsigned)(n < 1 ? 1 : n > most ? most : n); }
+
+// scratch of a call, handed out piece by piece; without a base it only counts
+struct Scratch {
+    char* base = nullptr;
+    size_t used = 0;
+    template <typename T> T* take(size_t n) {
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += up(n * sizeof(T), 256);
+        return p;
+    }
+};
+#define TYPED(type, ...)                                                       \
+    do {                                                                       \
+        if ((type) == CCSM_TYPE_F32) { typedef float T; __VA_ARGS__; }         \
+        else if ((type) == CCSM_TYPE_F16) { typedef f16 T; __VA_ARGS__; }      \
+        else { typedef b16 T; __VA_ARGS__; }                                   \
+    } while (0)
+
+ccsm_status check_saved(const ccsm_saved& s, int type, int64_t width, const char* what) {
+    REFUSE(!s.data, what);
+    if (s.code == CCSM_CODE_NONE) {
+        REFUSE(s.ld < width, "a kept matrix: ld is less than its width");
+        REFUSE(off_by(s.data, size_of(type)), "a kept matrix is not aligned to its elements");
+        return CCSM_OK;
+    }
+    REFUSE(s.code != CCSM_CODE_INT8 && s.code != CCSM_CODE_E4M3, "unknown code of a kept matrix");
+    REFUSE(!s.scales, "a kept matrix in 8 bits needs its scales");
+    REFUSE(s.ld % 32 != 0 || s.ld < (int64_t)up(width, 32) || s.lds < cdiv(width, 32), "a kept matrix in 8 bits: ld is a multiple of 32 and covers whole blocks, lds the blocks");
+    REFUSE(off_by(s.data, 16), "a kept matrix in 8 bits is 16-byte aligned");
+    return CCSM_OK;
+}
+Saved saved_of(const ccsm_saved& s) { return Saved{s.data, s.ld, s.code, s.scales, s.lds}; }
+Saved plain(const void* p, int64_t ld) { return Saved{p, ld, kCodeNone, nullptr, 0}; }
+
+template <typename T>
+void product(hipStream_t st, Operand a, Operand b, int64_t M, int64_t N, int64_t K, const Epilogue& ep) {
+    product_fma_kernel<T><<<dim3((unsigned)cdiv(N, 64), (unsigned)cdiv(M, 64)), 256, 0, st>>>(a, b, M, N, K, ep);
+}
+
+ccsm_status check_linear(const ccsm_linear* p) {
+    REFUSE(!p, "linear: NULL argument");
+    REFUSE(!good_type(p->type), "linear: unknown type");
+    REFUSE(p->activation < CCSM_ACT_NONE || p->activation > CCSM_ACT_SILU, "linear: unknown activation");
+    REFUSE(p->rows < 0 || p->rows > kMostRows || p->inner <= 0 || p->inner > kMostCols || p->outer <= 0 || p->outer > kMostCols, "linear: sizes out of range");
+    REFUSE(!p->w || (p->rows && (!p->x || !p->y)), "linear: x, w and y must be non-NULL");
+    REFUSE(p->ldx < p->inner || p->ldw < p->inner || p->ldy < p->outer || (p->residual && p->ldr < p->outer) || (p->preact && p->ldp < p->outer), "linear: a row stride is less than the row's width");
+    const size_t s = size_of(p->type);
+    REFUSE(off_by(p->x, s) || off_by(p->w, s) || off_by(p->y, s) || off_by(p->bias, s) || off_by(p->residual, s) || off_by(p->preact, s), "linear: a pointer is not aligned to its elements");
+    return CCSM_OK;
+}
+template <typename T>
+ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bool count) {
+    if (count) return CCSM_OK;
+    Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
+    product<T>(st, Operand{plain(p->x, p->ldx), 0}, Operand{plain(p->w, p->ldw), 0}, p->rows, p->outer, p->inner, ep);
+    LAUNCHED("linear_forward");
+    return CCSM_OK;
+}
+
+ccsm_status check_grad(const ccsm_linear_grad* p) {
+    REFUSE(!p, "linear_backward: NULL argument");
+    REFUSE(!good_type(p->type), "linear_backward: unknown type");
+    REFUSE(p->activation < CCSM_ACT_NONE || p->activation > CCSM_ACT_SILU, "linear_backward: unknown activation");
+    REFUSE(p->rows < 0 || p->rows > kMostRows || p->inner <= 0 || p->inner > kMostCols || p->outer <= 0 || p->outer > kMostCols, "linear_backward: sizes out of range");
+    const size_t s = size_of(p->type);
+    REFUSE(off_by(p->dy, s) || off_by(p->w, s) || off_by(p->dx, s) || off_by(p->dw, s) || off_by(p->dbias, s), "linear_backward: a pointer is not aligned to its elements");
+    if (p->rows) {
+        REFUSE(!p->dy, "linear_backward: dy must be non-NULL");
+        REFUSE(p->lddy < p->outer, "linear_backward: a row stride is less than the row's width");
+        if (p->activation != CCSM_ACT_NONE) {
+            ccsm_status e = check_saved(p->preact, p->type, p->outer, "linear_backward: an activation's slope needs the pre-activation");
+            if (e != CCSM_OK) return e;
+        }
+        if (p->dx) REFUSE(!p->w || p->ldw < p->inner || p->lddx < p->inner, "linear_backward: dx needs w, and strides of at least inner");
+        if (p->dw) {
+            ccsm_status e = check_saved(p->x, p->type, p->inner, "linear_backward: dw needs x");
+            if (e != CCSM_OK) return e;
+        }
+    }
+    REFUSE(p->dw && p->lddw < p->inner, "linear_backward: a row stride is less than the row's width");
+    return CCSM_OK;
+}
+template <typename T>
+ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t st, bool count) {
+    const int64_t M = p->rows;
+    const int K = p->inner, N = p->outer;
+    if (M == 0) {
+        if (count) return CCSM_OK;
+        if (p->dw) fill_zero_kernel<T><<<grid_of(cdiv((int64_t)N * K, 256), 4096), 256, 0, st>>>((T*)p->dw, p->lddw, N, K);
+        if (p->dbias) fill_zero_kernel<T><<<grid_of(cdiv(N, 256)), 256, 0, st>>>((T*)p->dbias, N, 1, N);
+        LAUNCHED("linear_backward");
+        return CCSM_OK;
+    }
+    const bool products = p->dx || p->dw, slope = p->activation != CCSM_ACT_NONE && products;
+    const int64_t parts = cdiv(M, 32);
+    T* d = slope ? ws.take<T>((size_t)M * N) : nullptr;
+    float* part = p->dbias ? ws.take<float>((size_t)parts * N) : nullptr;
+    if (count) return CCSM_OK;
+    if (slope || p->dbias) {
+        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 256)), 256, 0, st>>>((const T*)p->dy, p->lddy, saved_of(p->preact), p->activation, M, N, d, N, part);
+        if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 32), 256, 0, st>>>(part, parts, N, (T*)p->dbias);
+    }
+    const Saved dm = slope ? plain(d, N) : plain(p->dy, p->lddy);
+    if (p->dx) product<T>(st, Operand{dm, 0}, Operand{plain(p->w, p->ldw), 1}, M, K, N, Epilogue{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone});
+    if (p->dw) product<T>(st, Operand{dm, 1}, Operand{saved_of(p->x), 1}, N, K, M, Epilogue{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone});
+    LAUNCHED("linear_backward");
+    return CCSM_OK;
+}
+
+struct SortPlan { int bits, passes, digit; int64_t blocks, pieces; };
+SortPlan sort_plan(int64_t tokens, int64_t rows) {
+    SortPlan s;
+    s.bits = 1;
+    while (((int64_t)1 << s.bits) < rows + 1) ++s.bits;          // ids 0 .. rows (rows = no token)
+    s.passes = (s.bits + 7) / 8;
+    s.digit = (s.bits + s.passes - 1) / s.passes;
+    s.blocks = cdiv(tokens, kSortItems);
+    s.pieces = cdiv(tokens, kPiece);
+    return s;
+}
+struct EmbedScratch { unsigned *keys[2], *at[2], *counts; float* part; };
+EmbedScratch embed_scratch(Scratch& ws, const SortPlan& s, int64_t tokens, int width) {
+    EmbedScratch e;
+    for (int k = 0; k < 2; ++k) {
+        e.keys[k] = ws.take<unsigned>(tokens);
+        e.at[k] = ws.take<unsigned>(tokens);
+    }
+    e.counts = ws.take<unsigned>((size_t)s.blocks << s.digit);
+    e.part = ws.take<float>((size_t)2 * s.pieces * width);
+    return e;
+}
+ccsm_status check_embedding(int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int width) {
+    REFUSE(!good_type(type), "embedding: unknown type");
+    REFUSE(id_type < CCSM_ID_U8 || id_type > CCSM_ID_I64, "embedding: unknown type of ids");
+    REFUSE(tokens < 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols, "embedding: sizes out of range");
+    REFUSE(tokens && !ids, "embedding: ids must be non-NULL");
+    REFUSE(off_by(ids, id_type == CCSM_ID_U8 ? 1 : id_type == CCSM_ID_I32 ? 4 : 8), "embedding: ids are not aligned to their elements");
+    return CCSM_OK;
+}
+// 16-byte pieces where every row of both matrices consists of whole, aligned ones
+bool whole_pieces(int type, int width, const void* a, int64_t lda, const void* b, int64_t ldb) {
+    const int n = 16 / (int)size_of(type);
+    return width % n == 0 && lda % n == 0 && ldb % n == 0 && !off_by(a, 16) && !off_by(b, 16);
+}
+template <typename T, int N>
+void embedding_sums(hipStream_t st, const SortPlan& s, const EmbedScratch& e, int64_t tokens, int64_t rows, int width, const void* dy, int64_t lddy, float scale, void* dt, int64_t ldt, int k) {
+    const int lanes = width / N;
+    piece_sum_kernel<T, N><<<(unsigned)cdiv(s.pieces * lanes, 256), 256, 0, st>>>(e.keys[k], e.at[k], tokens, rows, lanes, width, (const T*)dy, lddy, scale, (T*)dt, ldt, e.part);
+    join_kernel<T><<<(unsigned)(s.pieces + grid_of(rows, 4096)), 256, 0, st>>>(e.keys[k], tokens, rows, width, scale, (T*)dt, ldt, e.part, s.pieces);
+}
+
+ccsm_status check_room(size_t need, const void* workspace, size_t have) {
+    if (need && (!workspace || have < need)) return fail(CCSM_ERR_CAPACITY, "the workspace is too small");
+    REFUSE(need && off_by(workspace, 256), "the workspace is not 256-byte aligned");
+    return CCSM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* ccsm_train_ops_last_error(void) { return g_err.c_str(); }
+
+size_t ccsm_train_linear_workspace(const ccsm_linear* p) {
+    if (check_linear(p) != CCSM_OK) return 0;
+    Scratch ws;
+    TYPED(p->type, (void)linear_forward<T>(p, ws, nullptr, true));
+    return ws.used;
+}
+ccsm_status ccsm_train_linear_forward(int device, const ccsm_linear* p, void* workspace, size_t workspace_bytes, void* stream) {
+    ccsm_status e = check_linear(p);
+    if (e != CCSM_OK || p->rows == 0) return e;
+    if ((e = check_room(ccsm_train_linear_workspace(p), workspace, workspace_bytes)) != CCSM_OK) return e;
+    ON_DEVICE(device);
+    Scratch ws;
+    ws.base = (char*)workspace;
+    TYPED(p->type, return linear_forward<T>(p, ws, (hipStream_t)stream, false));
+}
+
+size_t ccsm_train_linear_backward_workspace(const ccsm_linear_grad* p) {
+    if (check_grad(p) != CCSM_OK) return 0;
+    Scratch ws;
+    TYPED(p->type, (void)linear_backward<T>(p, ws, nullptr, true));
+    return ws.used;
+}
+ccsm_status ccsm_train_linear_backward(int device, const ccsm_linear_grad* p, void* workspace, size_t workspace_bytes, void* stream) {
+    ccsm_status e = check_grad(p);
+    if (e != CCSM_OK) return e;
+    if ((e = check_room(ccsm_train_linear_backward_workspace(p), workspace, workspace_bytes)) != CCSM_OK) return e;
+    ON_DEVICE(device);
+    Scratch ws;
+    ws.base = (char*)workspace;
+    TYPED(p->type, return linear_backward<T>(p, ws, (hipStream_t)stream, false));
+}
+
+ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
+                                         const void* table, int64_t ldt, float scale, void* y, int64_t ldy, void* stream) {
+    ccsm_status e = check_embedding(type, id_type, tokens, ids, rows, width);
+    if (e != CCSM_OK || tokens == 0) return e;
+    REFUSE(!table || !y || ldt < width || ldy < width, "embedding: table and y must be non-NULL, their strides at least the width");
+    REFUSE(off_by(table, size_of(type)) || off_by(y, size_of(type)), "embedding: a pointer is not aligned to its elements");
+    ON_DEVICE(device);
+    hipStream_t st = (hipStream_t)stream;
+    const bool whole = whole_pieces(type, width, table, ldt, y, ldy);
+    TYPED(type, constexpr int P = 16 / sizeof(T);
+          if (whole) lookup_kernel<T, P><<<grid_of(cdiv(tokens * (width / P), 256)), 256, 0, st>>>(ids, id_type, tokens, rows, width / P, (const T*)table, ldt, scale, (T*)y, ldy);
+          else lookup_kernel<T, 1><<<grid_of(cdiv(tokens * width, 256)), 256, 0, st>>>(ids, id_type, tokens, rows, width, (const T*)table, ldt, scale, (T*)y, ldy));
+    LAUNCHED("embedding_forward");
+    return CCSM_OK;
+}
+
+size_t ccsm_train_embedding_backward_workspace(int64_t tokens, int64_t rows, int32_t width) {
+    if (tokens <= 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols) return 0;
+    Scratch ws;
+    (void)embed_scratch(ws, sort_plan(tokens, rows), tokens, width);
+    return ws.used;
+}
+ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
+                                          const void* dy, int64_t lddy, float scale, void* dtable, int64_t ldt, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+    ccsm_status e = check_embedding(type, id_type, tokens, ids, rows, width);
+    if (e != CCSM_OK) return e;
+    REFUSE(!dtable || ldt < width || (tokens && (!dy || lddy < width)), "embedding: dy and dtable must be non-NULL, their strides at least the width");
+    REFUSE(off_by(dtable, size_of(type)) || off_by(dy, size_of(type)), "embedding: a pointer is not aligned to its elements");
+    if ((e = check_room(ccsm_train_embedding_backward_workspace(tokens, rows, width), workspace, workspace_bytes)) != CCSM_OK) return e;
+    ON_DEVICE(device);
+    hipStream_t st = (hipStream_t)stream;
+    if (tokens == 0) {
+        TYPED(type, fill_zero_kernel<T><<<grid_of(cdiv(rows * width, 256), 4096), 256, 0, st>>>((T*)dtable, ldt, rows, width));
+        LAUNCHED("embedding_backward");
+        return CCSM_OK;
+    }
+    Scratch ws;
+    ws.base = (char*)workspace;
+    const SortPlan s = sort_plan(tokens, rows);
+    const EmbedScratch b = embed_scratch(ws, s, tokens, width);
+    const int bins = 1 << s.digit;
+    int k = 0;
+    for (int pass = 0; pass < s.passes; ++pass) {
+        const unsigned *keys = pass ? b.keys[k] : nullptr, *at = pass ? b.at[k] : nullptr;
+        sort_count_kernel<<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, tokens, rows, pass * s.digit, bins, b.counts);
+        sort_scan_kernel<<<1, 1024, 0, st>>>(b.counts, s.blocks << s.digit);
+        sort_scatter_kernel<<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, at, tokens, rows, pass * s.digit, bins, b.counts, b.keys[k ^ 1], b.at[k ^ 1]);
+        k ^= 1;
+    }
+    const bool whole = whole_pieces(type, width, dy, lddy, dtable, ldt);
+    TYPED(type, constexpr int P = 16 / sizeof(T);
+          if (whole) embedding_sums<T, P>(st, s, b, tokens, rows, width, dy, lddy, scale, dtable, ldt, k);
+          else embedding_sums<T, 1>(st, s, b, tokens, rows, width, dy, lddy, scale, dtable, ldt, k));
+    LAUNCHED("embedding_backward");
+    return CCSM_OK;
+}
+
+ccsm_status ccsm_train_act8_pack(int device, int type, int code, int64_t rows, int32_t width, const void* x, int64_t ldx, void* codes,
+                                 int64_t ldc, uint8_t* scales, int64_t lds, void* stream) {
+    REFUSE(!good_type(type), "act8_pack: unknown type");
+    REFUSE(code != CCSM_CODE_INT8 && code != CCSM_CODE_E4M3, "act8_pack: unknown code");
+    REFUSE(rows < 0 || rows > kMostRows || width <= 0 || width > kMostCols, "act8_pack: sizes out of range");
+    if (rows == 0) return CCSM_OK;
+    REFUSE(!x || ldx < width || off_by(x, size_of(type)), "act8_pack: x must be non-NULL and aligned to its elements, its stride at least the width");
+    ccsm_status e = check_saved(ccsm_saved{codes, ldc, code, scales, lds}, type, width, "act8_pack: codes must be non-NULL");
+    if (e != CCSM_OK) return e;
+    ON_DEVICE(device);
+    const unsigned grid = grid_of(cdiv(rows * cdiv(width, 32), 8));
+    TYPED(type, if (code == CCSM_CODE_INT8) act8_pack_kernel<T, kCodeInt8><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)x, ldx, rows, width, (uint8_t*)codes, ldc, scales, lds);
+                else act8_pack_kernel<T, kCodeE4m3><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)x, ldx, rows, width, (uint8_t*)codes, ldc, scales, lds));
+    LAUNCHED("act8_pack");
+    return CCSM_OK;
+}
+ccsm_status ccsm_train_act8_unpack(int device, int type, int64_t rows, int32_t width, const ccsm_saved* s, void* y, int64_t ldy, void* stream) {
+    REFUSE(!s, "act8_unpack: NULL argument");
+    REFUSE(!good_type(type), "act8_unpack: unknown type");
+    REFUSE(s->code != CCSM_CODE_INT8 && s->code != CCSM_CODE_E4M3, "act8_unpack: unknown code");
+    REFUSE(rows < 0 || rows > kMostRows || width <= 0 || width > kMostCols, "act8_unpack: sizes out of range");
+    if (rows == 0) return CCSM_OK;
+    ccsm_status e = check_saved(*s, type, width, "act8_unpack: codes must be non-NULL");
+    if (e != CCSM_OK) return e;
+    REFUSE(!y || ldy < width || off_by(y, size_of(type)), "act8_unpack: y must be non-NULL and aligned to its elements, its stride at least the width");
+    ON_DEVICE(device);
+    TYPED(type, act8_unpack_kernel<T><<<grid_of(cdiv(rows * width, 256)), 256, 0, (hipStream_t)stream>>>(saved_of(*s), rows, width, (T*)y, ldy));
+    LAUNCHED("act8_unpack");
+    return CCSM_OK;
+}
+
+}  // extern "C"

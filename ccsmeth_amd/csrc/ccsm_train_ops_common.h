@@ -1,0 +1,154 @@
+// Shared by the training operators' kernels (ccsm_train_ops*.hip): element types, activations and their slopes, 8-bit codes.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ccsm_ops {
+
+typedef _Float16 f16;
+typedef __bf16 b16;
+
+template <typename T> struct TypeOf;                       // the ccsm_type of an element type
+template <> struct TypeOf<float> { static constexpr int v = 0; };
+template <> struct TypeOf<f16> { static constexpr int v = 1; };
+template <> struct TypeOf<b16> { static constexpr int v = 2; };
+
+// N elements that are loaded and stored as one piece of up to 16 bytes
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+
+enum { kActNone = 0, kActRelu, kActTanh, kActSigmoid, kActGelu, kActSilu };
+
+// FAST (16-bit tensors, whose results keep 11 bits at most): hardware exp2 and reciprocal (1 ulp each), and for gelu the rational form of erfc
+// by Abramowitz and Stegun (7.1.26; |error| <= 1.5e-7): 14 instructions where the library's erff has more than 40, which was a sixth of
+// a wide layer's time in the epilogue.  fp32 tensors take the accurate library functions.
+template <bool FAST>
+__device__ __forceinline__ float exp_(float x) { return FAST ? __expf(x) : expf(x); }
+template <bool FAST>
+__device__ __forceinline__ float rcp_(float x) { return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x; }
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_(float z) { return rcp_<FAST>(1.f + exp_<FAST>(-z)); }
+template <bool FAST>
+__device__ __forceinline__ float tanh_(float z) {
+    if (!FAST) return tanhf(z);
+    // 1 - 2 / (1 + e^2|z|); below 2^-4 that loses bits, and z - z^3 / 3 + 2 z^5 / 15 is within 2^-20 z
+    const float a = fabsf(z), t = 1.f - 2.f * rcp_<true>(1.f + exp_<true>(2.f * a)), q = z * z;
+    return a < 0.0625f ? z * (1.f + q * (-0.33333333f + q * 0.13333333f)) : copysignf(t, z);
+}
+// the normal distribution's Phi(z), and e^(-z^2 / 2) (the library's erfc keeps its relative accuracy in the lower tail)
+template <bool FAST>
+__device__ __forceinline__ float phi_(float z, float* e) {
+    const float x = fabsf(z) * 0.70710678f;
+    *e = exp_<FAST>(-0.5f * z * z);
+    if (!FAST) return 0.5f * erfcf(-z * 0.70710678118654752f);
+    const float t = rcp_<true>(1.f + 0.3275911f * x);
+    const float q = 0.5f * *e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return z >= 0.f ? 1.f - q : q;
+}
+template <bool FAST>
+__device__ __forceinline__ float act_(float z, int act) {
+    float e;
+    switch (act) {
+        case kActRelu: return z < 0.f ? 0.f : z;            // (a NaN stays one)
+        case kActTanh: return tanh_<FAST>(z);
+        case kActSigmoid: return sigmoid_<FAST>(z);
+        case kActGelu: return z * phi_<FAST>(z, &e);
+        case kActSilu: return z * sigmoid_<FAST>(z);
+        default: return z;
+    }
+}
+template <bool FAST>
+__device__ __forceinline__ float slope_(float z, int act) {
+    float e, a;
+    switch (act) {
+        case kActRelu: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
+        case kActTanh: {                                     // 1 - tanh^2 = 4 e / (1 + e)^2 with e = e^-2|z|: no cancellation for large |z|
+            e = exp_<FAST>(-2.f * fabsf(z));
+            a = rcp_<FAST>(1.f + e);
+            return 4.f * e * a * a;
+        }
+        case kActSigmoid: {
+            e = exp_<FAST>(-fabsf(z));
+            a = rcp_<FAST>(1.f + e);
+            return e * a * a;
+        }
+        case kActGelu: {
+            a = phi_<FAST>(z, &e);
+            return a + z * e * 0.3989422804f;
+        }
+        case kActSilu: a = sigmoid_<FAST>(z); return a * (1.f + z * (1.f - a));
+        default: return 1.f;
+    }
+}
+
+// ---- 8-bit codes (ccsm_code8) ---------------------------------------------------------------------------------------
+enum { kCodeNone = 0, kCodeInt8 = 1, kCodeE4m3 = 2 };
+
+__device__ __forceinline__ float pow2_of_byte(unsigned b) { return __uint_as_float(b << 23); }      // 2^(b - 127), b in [1, 254]
+// the scale byte of a block whose largest finite magnitude is `most`: the least e with most <= 127 2^e (448 2^e), read off most's exponent
+// and fraction (127 = 1.984375 2^6, 448 = 1.75 2^8)
+template <int CODE>
+__device__ __forceinline__ unsigned scale_byte(float most) {
+    const unsigned u = __float_as_uint(most), frac = u & 0x7fffffu;
+    const int b = (int)(u >> 23) - (CODE == kCodeInt8 ? 6 : 8) + (frac > (CODE == kCodeInt8 ? 0x7e0000u : 0x600000u) ? 1 : 0);
+    return b < 1 ? 1u : (unsigned)b;
+}
+// the largest code of a block: one that rounds up past the packed type's range has to stay below it (the topmost scale byte only)
+template <int CODE, int TYPE>
+__device__ __forceinline__ float largest_code(unsigned b) {
+    const unsigned top = (TYPE == 1 ? 142u : 254u) + (CODE == kCodeInt8 ? -5 : -7);
+    return b >= top ? (CODE == kCodeInt8 ? 63.f : 240.f) : (CODE == kCodeInt8 ? 127.f : 448.f);
+}
+// four values, already divided by 2^e, as four codes
+template <int CODE>
+__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float top) {
+    if (CODE == kCodeE4m3) {
+        auto lim = [top](float v) { return fminf(fmaxf(v, -top), top); };
+        auto fin = [](float v) { return fabsf(v) < INFINITY; };
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32(lim(a), lim(b), 0, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(lim(c), lim(d), r, true);
+        unsigned u = (unsigned)r;
+        if (!fin(a)) u = (u & 0xffffff00u) | 0x7fu;
+        if (!fin(b)) u = (u & 0xffff00ffu) | 0x7f00u;
+        if (!fin(c)) u = (u & 0xff00ffffu) | 0x7f0000u;
+        if (!fin(d)) u = (u & 0x00ffffffu) | 0x7f000000u;
+        return u;
+    }
+    auto one = [top](float v) -> unsigned {
+        const float q = fminf(fmaxf(__builtin_rintf(v), -top), top);
+        return fabsf(v) < INFINITY ? (unsigned)(int)q & 0xffu : 0x80u;
+    };
+    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+}
+// four codes as the values they stand for
+template <int CODE>
+__device__ __forceinline__ void decode4(unsigned u, float scale, float (&v)[4]) {
+    if (CODE == kCodeE4m3) {
+        v[0] = __builtin_amdgcn_cvt_f32_fp8((int)u, 0) * scale;
+        v[1] = __builtin_amdgcn_cvt_f32_fp8((int)u, 1) * scale;
+        v[2] = __builtin_amdgcn_cvt_f32_fp8((int)u, 2) * scale;
+        v[3] = __builtin_amdgcn_cvt_f32_fp8((int)u, 3) * scale;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int q = (int)(signed char)(u >> (8 * j));
+        v[j] = q == -128 ? __builtin_nanf("") : (float)q * scale;
+    }
+}
+__device__ __forceinline__ float decode1(int code, unsigned byte, float scale) {
+    if (code == kCodeE4m3) return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0) * scale;
+    const int q = (int)(signed char)byte;
+    return q == -128 ? __builtin_nanf("") : (float)q * scale;
+}
+
+// element (row, col) of a kept matrix in type T, or of its codes
+struct Saved {
+    const void* data; long long ld; int code; const uint8_t* scales; long long lds;
+};
+template <typename T>
+__device__ __forceinline__ float saved_at(const Saved& s, long long row, long long col) {
+    if (s.code == kCodeNone) return (float)((const T*)s.data)[row * s.ld + col];
+    return decode1(s.code, ((const uint8_t*)s.data)[row * s.ld + col], pow2_of_byte(s.scales[row * s.lds + (col >> 5)]));
+}
+
+}  // namespace ccsm_ops

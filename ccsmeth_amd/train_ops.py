@@ -1,0 +1,390 @@
+"""The operators of a training step on torch tensors (include/ccsm_train_ops.h, in libccsm_train): products with bias, activation and residual,
+embedding lookup, and activations kept in 8 bits, each with the gradients that a training step needs.
+
+    y, z = linear(x, w, b, residual, activation="gelu", keep_preact=True)
+    dx, dw, db = linear_backward(dy, x, w, z, activation="gelu")          # x and z may be checkpoint8(x, ...) and checkpoint8(z, ...)
+    y = embedding(ids, table, scale=2.0);   dtable = embedding_backward(dy, ids, len(table), scale=2.0)
+    c = checkpoint8(x, "int8");             x_hat = c.values()
+
+What torch.nn does for the reference here: nn.Embedding (ccsmeth/models.py:35, 91), nn.Linear and the activation behind it
+(ccsmeth/utils/attention.py:34-36, 69), autograd's saved tensors (ccsmeth/train_multigpu.py:283-312).
+
+Tensors are float32, float16 or bfloat16 on one GPU, one type per call.  Work is enqueued on `stream` (a torch.cuda.Stream; default: torch's
+current stream of the tensors' device) and nothing waits for the GPU; calls can be captured into a graph.  Row-strided views are taken as
+they are, other layouts are copied.  There is no autograd: gradients are calls, as in Trainer.forward_backward, and inputs that require a
+gradient are refused while grad mode is on.  There is no CPU path.
+"""
+import contextlib
+import ctypes as C
+
+from . import _lib
+from . import train as _train
+
+EXPORTS = ("ccsm_train_ops_last_error", "ccsm_train_linear_workspace", "ccsm_train_linear_forward", "ccsm_train_linear_backward_workspace",
+           "ccsm_train_linear_backward", "ccsm_train_embedding_forward", "ccsm_train_embedding_backward_workspace",
+           "ccsm_train_embedding_backward", "ccsm_train_act8_pack", "ccsm_train_act8_unpack")
+ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "gelu": 4, "silu": 5}
+CODES = {"int8": 1, "e4m3": 2}
+
+
+class Saved(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("ld", C.c_int64), ("code", C.c_int32), ("scales", C.c_void_p), ("lds", C.c_int64)]
+
+
+class Linear(C.Structure):
+    _fields_ = [("type", C.c_int32), ("activation", C.c_int32), ("rows", C.c_int64), ("inner", C.c_int32), ("outer", C.c_int32),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64), ("bias", C.c_void_p),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64), ("preact", C.c_void_p), ("ldp", C.c_int64)]
+
+
+class LinearGrad(C.Structure):
+    _fields_ = [("type", C.c_int32), ("activation", C.c_int32), ("rows", C.c_int64), ("inner", C.c_int32), ("outer", C.c_int32),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("x", Saved), ("w", C.c_void_p), ("ldw", C.c_int64), ("preact", Saved),
+                ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64), ("dbias", C.c_void_p)]
+
+
+_ops = None
+
+
+def load():
+    global _ops
+    if _ops is not None:
+        return _ops
+    lib = _train.load()
+    vp, ci, cl, cf, cs = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
+    lib.ccsm_train_ops_last_error.restype = C.c_char_p
+    lib.ccsm_train_linear_workspace.argtypes = [C.POINTER(Linear)]
+    lib.ccsm_train_linear_workspace.restype = cs
+    lib.ccsm_train_linear_forward.argtypes = [ci, C.POINTER(Linear), vp, cs, vp]
+    lib.ccsm_train_linear_backward_workspace.argtypes = [C.POINTER(LinearGrad)]
+    lib.ccsm_train_linear_backward_workspace.restype = cs
+    lib.ccsm_train_linear_backward.argtypes = [ci, C.POINTER(LinearGrad), vp, cs, vp]
+    lib.ccsm_train_embedding_forward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp]
+    lib.ccsm_train_embedding_backward_workspace.argtypes = [cl, cl, C.c_int32]
+    lib.ccsm_train_embedding_backward_workspace.restype = cs
+    lib.ccsm_train_embedding_backward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp, cs, vp]
+    lib.ccsm_train_act8_pack.argtypes = [ci, ci, ci, cl, C.c_int32, vp, cl, vp, cl, vp, cl, vp]
+    lib.ccsm_train_act8_unpack.argtypes = [ci, ci, cl, C.c_int32, C.POINTER(Saved), vp, cl, vp]
+    _ops = lib
+    return lib
+
+
+def _check(status):
+    if status != _lib.OK:
+        raise _lib.CcsmError(status, load().ccsm_train_ops_last_error().decode())
+
+
+def _types():
+    import torch
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}, {torch.uint8: 0, torch.int32: 1, torch.int64: 2}
+
+
+_TYPE = _ID = _torch = None
+
+
+def _init():
+    global _TYPE, _ID, _torch
+    if _torch is None:
+        import torch
+        _TYPE, _ID = _types()
+        _torch = torch
+    return _torch
+
+
+def _tensor(t, name, dtype=None, device=None):
+    torch = _torch
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor" % name)
+    if t.dtype not in _TYPE:
+        raise ValueError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
+    if dtype is not None and t.dtype is not dtype:
+        raise ValueError("%s is %s, the call's type is %s" % (name, t.dtype, dtype))
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient: these calls are not seen by autograd (use torch.no_grad() and the *_backward calls)" % name)
+    return t
+
+
+def _on_gpu(t, name):
+    if not t.is_cuda:
+        raise ValueError("%s must be on a GPU: there is no CPU path" % name)
+
+
+def _rows(t):
+    """(2-D view or copy with contiguous rows, its row stride)"""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.dim() else t.reshape(1, 1)
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
+
+
+class _Run:
+    """The call's stream: what it allocates belongs to that stream, and what it was given is kept for it until its work is done."""
+
+    __slots__ = ("device", "stream", "_with", "_other")
+
+    def __init__(self, device, stream):
+        torch = _torch
+        now = torch.cuda.current_stream(device)
+        if stream is None:
+            stream = now
+        elif not isinstance(stream, torch.cuda.Stream):
+            raise TypeError("stream must be a torch.cuda.Stream")
+        elif stream.device != device:
+            raise ValueError("stream belongs to %s, the tensors to %s" % (stream.device, device))
+        self.device, self.stream = device, stream
+        self._other = stream.cuda_stream != now.cuda_stream
+
+    def __enter__(self):
+        self._with = _torch.cuda.stream(self.stream) if self._other else contextlib.nullcontext()
+        self._with.__enter__()
+        return self
+
+    def __exit__(self, *a):
+        return self._with.__exit__(*a)
+
+    def keep(self, *tensors):
+        if self._other:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(self.stream)
+
+    def empty(self, shape, dtype):
+        return _torch.empty(shape, dtype=dtype, device=self.device)
+
+    def scratch(self, n):
+        return _torch.empty(n, dtype=_torch.uint8, device=self.device) if n else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError("activation must be one of %s, not %r" % (", ".join(ACTIVATIONS), name))
+    return ACTIVATIONS[name]
+
+
+def _out(out, shape, dtype, device, name):
+    if out.shape != shape or out.dtype is not dtype or out.device != device:
+        raise ValueError("%s must be a %s tensor of shape %s on %s" % (name, dtype, tuple(shape), device))
+    if out.dim() > 1 and not out.is_contiguous() and (out.dim() != 2 or out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]) or \
+            out.dim() == 1 and out.numel() > 1 and out.stride(0) != 1:
+        raise ValueError("%s must have contiguous rows" % name)
+    return out
+
+
+class Checkpoint8:
+    """An activation in 8 bits (layout: include/ccsm_train_ops.h): `codes` (rows, width rounded up to 32) and `scales` (rows, width / 32 rounded up),
+    uint8; `shape` and `dtype` of the tensor it was made of; `code` "int8" or "e4m3"."""
+
+    def __init__(self, codes, scales, shape, dtype, code):
+        torch = _init()
+        shape = tuple(int(n) for n in shape)
+        if code not in CODES:
+            raise ValueError("code must be one of %s, not %r" % (", ".join(CODES), code))
+        if dtype not in _TYPE:
+            raise ValueError("dtype must be float32, float16 or bfloat16, not %s" % dtype)
+        if not shape or shape[-1] < 1:
+            raise ValueError("a checkpoint has at least one column")
+        rows = 1
+        for n in shape[:-1]:
+            rows *= n
+        blocks = -(-shape[-1] // 32)
+        for t, cols, name in ((codes, 32 * blocks, "codes"), (scales, blocks, "scales")):
+            if t.dtype is not torch.uint8 or tuple(t.shape) != (rows, cols) or not t.is_contiguous():
+                raise ValueError("%s must be a contiguous uint8 tensor of shape %s" % (name, (rows, cols)))
+        if codes.device != scales.device:
+            raise ValueError("codes and scales are on different devices")
+        self.codes, self.scales, self.shape, self.dtype, self.code = codes, scales, torch.Size(shape), dtype, code
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def _saved(self):
+        return Saved(self.codes.data_ptr(), self.codes.shape[1], CODES[self.code], self.scales.data_ptr(), self.scales.shape[1])
+
+    def values(self, dtype=None, *, out=None, stream=None):
+        """The values that the codes stand for, as a tensor of `dtype` (default: the type it was made of, which holds them exactly)."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _TYPE:
+            raise ValueError("dtype must be float32, float16 or bfloat16, not %s" % dtype)
+        lib = load()
+        _on_gpu(self.codes, "the checkpoint")
+        with _Run(self.device, stream) as run:
+            y = run.empty(self.shape, dtype) if out is None else _out(out, self.shape, dtype, self.device, "out")
+            run.keep(self.codes, self.scales, out)
+            y2, ldy = _rows(y)
+            s = self._saved()
+            _check(lib.ccsm_train_act8_unpack(run.device.index, _TYPE[dtype], y2.shape[0], y2.shape[1], C.byref(s), y2.data_ptr(), ldy, run.stream.cuda_stream))
+        return y
+
+
+def checkpoint8(x, code="int8", *, stream=None):
+    """x (..., width) -> Checkpoint8: blocks of 32 values of a row share a power of two; "int8" keeps 127 even steps either side of zero (bounded
+    activations, normalised inputs), "e4m3" three bits behind the leading one (long-tailed ones)."""
+    torch = _init()
+    lib = load()
+    if code not in CODES:
+        raise ValueError("code must be one of %s, not %r" % (", ".join(CODES), code))
+    _tensor(x, "x")
+    _on_gpu(x, "x")
+    if x.dim() == 0 or x.shape[-1] < 1:
+        raise ValueError("x must have at least one column")
+    with _Run(x.device, stream) as run:
+        x2, ldx = _rows(x)
+        rows, width = x2.shape
+        blocks = -(-width // 32)
+        codes = run.empty((rows, 32 * blocks), torch.uint8)
+        scales = run.empty((rows, blocks), torch.uint8)
+        run.keep(x)
+        _check(lib.ccsm_train_act8_pack(run.device.index, _TYPE[x.dtype], CODES[code], rows, width, x2.data_ptr(), ldx, codes.data_ptr(), 32 * blocks,
+                                        scales.data_ptr(), blocks, run.stream.cuda_stream))
+    return Checkpoint8(codes, scales, x.shape, x.dtype, code)
+
+
+def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=False, *, out=None, stream=None):
+    """y = act(x weight^T + bias) + residual; x (..., inner), weight (outer, inner), bias (outer), residual and y (..., outer).
+    keep_preact: -> (y, z) with z = x weight^T + bias as linear_backward takes it.  out: where y goes (it may be the residual)."""
+    _init()
+    lib = load()
+    act = _activation(activation)
+    t, dev = _tensor(x, "x").dtype, x.device
+    _on_gpu(x, "x")
+    _tensor(weight, "weight", t, dev)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("x must be (..., inner) and weight (outer, inner): got %s and %s" % (tuple(x.shape), tuple(weight.shape)))
+    outer, inner = weight.shape
+    if inner < 1 or outer < 1:
+        raise ValueError("weight has no rows or no columns")
+    shape = x.shape[:-1] + (outer,)
+    if bias is not None and tuple(_tensor(bias, "bias", t, dev).shape) != (outer,):
+        raise ValueError("bias must be (%d,)" % outer)
+    if residual is not None and _tensor(residual, "residual", t, dev).shape != shape:
+        raise ValueError("residual must be %s" % (tuple(shape),))
+    with _Run(dev, stream) as run:
+        y = run.empty(shape, t) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
+        z = run.empty(shape, t) if keep_preact else None
+        run.keep(x, weight, bias, residual, out)
+        x2, ldx = _rows(x)
+        w2, ldw = _rows(weight)
+        b1 = None if bias is None else bias.contiguous()
+        y2, ldy = _rows(y)
+        r2, ldr = (None, 0) if residual is None else _rows(residual)
+        p = Linear(_TYPE[t], act, x2.shape[0], inner, outer, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b1), _ptr(r2), ldr, y2.data_ptr(), ldy, _ptr(z), outer)
+        need = lib.ccsm_train_linear_workspace(C.byref(p))
+        ws = run.scratch(need)
+        _check(lib.ccsm_train_linear_forward(dev.index, C.byref(p), _ptr(ws), need, run.stream.cuda_stream))
+    return (y, z) if keep_preact else y
+
+
+def linear_backward(dy, x, weight, preact=None, activation="none", *, need_dx=True, need_dw=True, need_db=True, stream=None):
+    """The gradients of y = act(x weight^T + bias) (+ residual, whose gradient is dy itself): (dx, dw, db), None for what is not needed.
+    dy (..., outer); x (..., inner) and preact (..., outer) are tensors or Checkpoint8s; preact only where there is an activation."""
+    _init()
+    lib = load()
+    act = _activation(activation)
+    t, dev = _tensor(dy, "dy").dtype, dy.device
+    _on_gpu(dy, "dy")
+    _tensor(weight, "weight", t, dev)
+    if weight.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != weight.shape[0]:
+        raise ValueError("dy must be (..., outer) and weight (outer, inner): got %s and %s" % (tuple(dy.shape), tuple(weight.shape)))
+    outer, inner = weight.shape
+    if inner < 1 or outer < 1:
+        raise ValueError("weight has no rows or no columns")
+    if act and preact is None:
+        raise ValueError("preact is needed for the slope of %s" % activation)
+
+    def saved(v, cols, name):
+        if v is None:
+            return Saved(), ()
+        if tuple(v.shape) != tuple(dy.shape[:-1]) + (cols,):
+            raise ValueError("%s must be %s, not %s" % (name, tuple(dy.shape[:-1]) + (cols,), tuple(v.shape)))
+        if isinstance(v, Checkpoint8):
+            if v.device != dev:
+                raise ValueError("%s is on %s, not on %s" % (name, v.device, dev))
+            if v.dtype is not t:
+                raise ValueError("%s was made of %s, the call's type is %s" % (name, v.dtype, t))
+            return v._saved(), (v.codes, v.scales)
+        v2, ld = _rows(_tensor(v, name, t, dev))
+        return Saved(v2.data_ptr(), ld, 0, None, 0), (v, v2)
+
+    if need_dw and x is None:
+        raise ValueError("x is needed for dw")
+    with _Run(dev, stream) as run:
+        xs, keep_x = saved(x if need_dw else None, inner, "x")
+        zs, keep_z = saved(preact if act else None, outer, "preact")
+        dx = run.empty(dy.shape[:-1] + (inner,), t) if need_dx else None
+        dw = run.empty((outer, inner), t) if need_dw else None
+        db = run.empty((outer,), t) if need_db else None
+        run.keep(dy, weight, *keep_x, *keep_z)
+        d2, ldd = _rows(dy)
+        w2, ldw = _rows(weight)
+        p = LinearGrad(_TYPE[t], act, d2.shape[0], inner, outer, d2.data_ptr(), ldd, xs, w2.data_ptr(), ldw, zs, _ptr(dx), inner, _ptr(dw), inner, _ptr(db))
+        need = lib.ccsm_train_linear_backward_workspace(C.byref(p))
+        ws = run.scratch(need)
+        _check(lib.ccsm_train_linear_backward(dev.index, C.byref(p), _ptr(ws), need, run.stream.cuda_stream))
+    return dx, dw, db
+
+
+def _ids(ids, device):
+    torch = _torch
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in _ID:
+        raise ValueError("ids must be a uint8, int32 or int64 tensor")
+    if ids.device != device:
+        raise ValueError("ids are on %s, not on %s" % (ids.device, device))
+    return ids.contiguous()
+
+
+def embedding(ids, table, scale=1.0, *, out=None, stream=None):
+    """y (*ids.shape, width) = scale * table[ids].  Ids outside [0, len(table)), padding of -1 for instance, give a row of zeros."""
+    _init()
+    lib = load()
+    t, dev = _tensor(table, "table").dtype, table.device
+    _on_gpu(table, "table")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError("table must be (rows, width)")
+    with _Run(dev, stream) as run:
+        i = _ids(ids, dev)
+        shape = ids.shape + (table.shape[1],)
+        y = run.empty(shape, t) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
+        run.keep(ids, table, out)
+        t2, ldt = _rows(table)
+        y2, ldy = _rows(y)
+        _check(lib.ccsm_train_embedding_forward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), t2.shape[0], t2.shape[1], t2.data_ptr(), ldt, float(scale),
+                                                y2.data_ptr(), ldy, run.stream.cuda_stream))
+    return y
+
+
+def embedding_backward(dy, ids, rows, scale=1.0, *, out=None, stream=None):
+    """The gradient of embedding()'s table, (rows, width) in dy's type: row v = scale * the sum of dy's rows whose id is v, zero where there is none.
+    A row's sum has one order, that of its tokens: the same inputs give the same bits."""
+    _init()
+    lib = load()
+    t, dev = _tensor(dy, "dy").dtype, dy.device
+    _on_gpu(dy, "dy")
+    rows = int(rows)
+    if rows < 1:
+        raise ValueError("rows must be at least 1")
+    if dy.dim() < 1 or dy.shape[-1] < 1 or not hasattr(ids, "shape") or dy.shape[:-1] != ids.shape:
+        raise ValueError("dy must be (*ids.shape, width)")
+    width = dy.shape[-1]
+    with _Run(dev, stream) as run:
+        i = _ids(ids, dev)
+        dt = run.empty((rows, width), t) if out is None else _out(_tensor(out, "out"), _torch.Size((rows, width)), t, dev, "out")
+        run.keep(dy, ids, out)
+        d2, ldd = _rows(dy)
+        t2, ldt = _rows(dt)
+        need = lib.ccsm_train_embedding_backward_workspace(i.numel(), rows, width)
+        ws = run.scratch(need)
+        _check(lib.ccsm_train_embedding_backward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), rows, width, d2.data_ptr(), ldd, float(scale),
+                                                 t2.data_ptr(), ldt, _ptr(ws), need, run.stream.cuda_stream))
+    return dt

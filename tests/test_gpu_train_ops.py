@@ -1,0 +1,493 @@
+"""The training operators on the GPU (include/ccsm_train_ops.h) against plain implementations in 64 bits.
+
+Tolerances.  h = half a step of the type (fp32 2^-24, fp16 2^-11, bf16 2^-8), relative.
+  product    a sum of K products kept in fp32: the k-th addition rounds a partial sum of about sqrt(k) s, s = rms of the products, by 2^-24 at most; the
+             roundings add up like a random walk to 2^-24 s K / sqrt(6) = 2^-24 q sqrt(K) / 2.4, q = sqrt(sum (x w)^2).  Eight times that for the largest
+             of many, and sqrt(6) for fp32 operands taken as six products of three pieces each: 2^-24 (8 sqrt(K) + 8) q.
+  activation slopes are at most 1.13 in magnitude (gelu), the functions within 2^-20 absolute in 16-bit calls and 2^-22 in fp32 ones (times max(1, |z|)).
+  rounding   h |y| for what is written, and in a 16-bit backward pass h |d| for each d before its products: errors that are independent of each
+             other and of d's sign, so their sum is within 5 h sqrt(sum (d w)^2) (9 standard deviations of a uniform error)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from ccsmeth_amd import train_ops as ops  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F32, F16, BF16]
+H = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+TINY = {F32: 2.0 ** -149, F16: 2.0 ** -24, BF16: 2.0 ** -133}
+ACTS = ["none", "relu", "tanh", "sigmoid", "gelu", "silu"]
+DEV = "cuda:0"
+
+
+def normal(seed, *shape, t=F32, by=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * by).to(t).to(DEV)
+
+
+def act64(z, act):
+    return {"none": lambda: z, "relu": lambda: z.clamp_min(0), "tanh": lambda: z.tanh(), "sigmoid": lambda: torch.sigmoid(z),
+            "gelu": lambda: z * torch.special.ndtr(z), "silu": lambda: z * torch.sigmoid(z)}[act]()
+
+
+def slope64(z, act):
+    s = torch.sigmoid(z)
+    return {"none": lambda: torch.ones_like(z), "relu": lambda: (z > 0).double(), "tanh": lambda: 1 - z.tanh() ** 2, "sigmoid": lambda: s * (1 - s),
+            "gelu": lambda: torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), "silu": lambda: s * (1 + z * (1 - s))}[act]()
+
+
+def mm(a, b):
+    return torch.mm(a, b)
+
+
+def sum_tol(n):
+    return 2.0 ** -24 * (8 * math.sqrt(n) + 8)
+
+
+def within(got, ref, tol, t):
+    """|got - ref| <= tol + h |ref| (+ the smallest step of the type), everywhere"""
+    assert got.dtype is t and got.shape == ref.shape
+    d = (got.double().cpu() - ref.cpu()).abs()
+    lim = tol.cpu() + H[t] * (ref.cpu().abs() + tol.cpu()) + TINY[t]
+    assert torch.isfinite(got.double()).all()
+    over = d / lim
+    assert float(over.max() if over.numel() else 0) <= 1, (float(over.max()), int(over.argmax()))
+
+
+def act_tol(z, tz, t):
+    return 1.13 * tz + (2.0 ** -22 if t is F32 else 2.0 ** -20) * z.abs().clamp_min(1)
+
+
+def check_linear(x, w, b, r, act, t, y, z=None):
+    x6, w6 = x.double().reshape(-1, x.shape[-1]), w.double()
+    ref = mm(x6, w6.t())
+    tz = sum_tol(x.shape[-1]) * mm(x6 ** 2, (w6 ** 2).t()).sqrt()
+    if b is not None:
+        ref = ref + b.double()
+        tz = tz + 2.0 ** -23 * (ref.abs() + b.double().abs())
+    if z is not None:
+        within(z.reshape(ref.shape), ref, tz, t)
+    out = act64(ref, act)
+    ty = act_tol(ref, tz, t) if act != "none" else tz
+    if r is not None:
+        r6 = r.double().reshape(ref.shape)
+        out, ty = out + r6, ty + 2.0 ** -24 * (out + r6).abs()
+    within(y.reshape(ref.shape), out, ty, t)
+
+
+SIZES = [(1, 1, 1), (1, 512, 768), (2, 11, 9), (3, 64, 5), (7, 129, 33), (16, 768, 256), (17, 40, 520), (33, 8, 130), (64, 256, 64), (65, 72, 128), (127, 31, 257),
+         (128, 128, 128), (130, 200, 96), (255, 264, 136), (256, 64, 256), (257, 520, 264), (513, 96, 768), (1000, 11, 768), (1500, 512, 256)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_linear_sizes(t, m, k, n):
+    act = ACTS[(m + k + n) % 6]
+    x, w, b, r = normal(m, m, k, t=t), normal(k + 1, n, k, t=t, by=k ** -0.5), normal(n + 2, n, t=t, by=0.3), normal(3, m, n, t=t)
+    y, z = ops.linear(x, w, b, r, activation=act, keep_preact=True)
+    check_linear(x, w, b, r, act, t, y, z)
+    check_linear(x, w, None, None, "none", t, ops.linear(x, w))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [1, 5, 96, 300])
+def test_linear_activations(t, act, m):
+    """pre-activations from -9 to 9: the tails of every activation"""
+    k, n = 24, 80
+    x, w, b = normal(5, m, k, t=t), normal(6, n, k, t=t, by=0.1), torch.linspace(-9, 9, n).to(t).to(DEV)
+    for r in (None, normal(8, m, n, t=t)):
+        y, z = ops.linear(x, w, b, r, activation=act, keep_preact=True)
+        check_linear(x, w, b, r, act, t, y, z)
+
+
+def check_backward(dy, x, w, z, act, t, got):
+    """x, z: the values that the call reads (of a checkpoint: the ones it stands for), in 64 bits"""
+    dx, dw, db = got
+    dy6, w6 = dy.double().reshape(-1, dy.shape[-1]), w.double()
+    x6 = x.double().reshape(-1, x.shape[-1])
+    d = dy6 * (slope64(z.double().reshape(dy6.shape), act) if act != "none" else 1.0)
+    off = 0.0 if act == "none" else 2.0 ** -20 if t is not F32 else 2.0 ** -21      # the slope's own error, relative to dy
+    hd = 0.0 if t is F32 or act == "none" else 5 * H[t]
+    M, N = d.shape
+    for out, a, b, ay, n in ((dx, d, w6, dy6, N), (dw, d.t(), x6, dy6.t(), M)):
+        if out is None:
+            continue
+        q = mm(a ** 2, b ** 2).sqrt()
+        qy = mm(ay ** 2, b ** 2).sqrt()
+        sub = TINY[t] * b.abs().sum(0) if hd else 0.0            # d below the type's normal range
+        within(out.reshape(q.shape), mm(a, b), (sum_tol(n) + hd) * q + 5 * off * qy + sub, t)
+    if db is not None:
+        within(db, d.sum(0), sum_tol(M) * (d ** 2).sum(0).sqrt() + 5 * off * (dy6 ** 2).sum(0).sqrt(), t)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_backward_sizes(t, m, k, n):
+    act = ACTS[(m + k + 2 * n) % 6]
+    dy, x, w, z = normal(1, m, n, t=t, by=0.05), normal(2, m, k, t=t), normal(3, n, k, t=t, by=k ** -0.5), normal(4, m, n, t=t)
+    check_backward(dy, x, w, z, act, t, ops.linear_backward(dy, x, w, z if act != "none" else None, activation=act))
+    check_backward(dy, x, w, z, "none", t, ops.linear_backward(dy, x, w))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_backward_activations(t, act):
+    m, k, n = 70, 24, 80
+    dy, x, w = normal(1, m, n, t=t), normal(2, m, k, t=t), normal(3, n, k, t=t, by=0.2)
+    z = torch.linspace(-9, 9, m * n).reshape(n, m).t().to(t).to(DEV)
+    z[0, :3] = 0.0
+    check_backward(dy, x, w, z, act, t, ops.linear_backward(dy, x, w, z, activation=act))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("xc,zc", [("int8", None), ("e4m3", None), (None, "int8"), (None, "e4m3"), ("int8", "e4m3"), ("e4m3", "int8")])
+@pytest.mark.parametrize("m,k,n", [(1, 8, 8), (5, 33, 31), (64, 64, 96), (130, 40, 264), (257, 520, 72), (1031, 256, 136)])
+def test_backward_from_checkpoints(t, xc, zc, m, k, n):
+    dy, x, w, z = normal(1, m, n, t=t, by=0.05), normal(2, m, k, t=t), normal(3, n, k, t=t, by=k ** -0.5), normal(4, m, n, t=t, by=2.0)
+    cx, cz = ops.checkpoint8(x, xc) if xc else x, ops.checkpoint8(z, zc) if zc else z
+    got = ops.linear_backward(dy, cx, w, cz, activation="silu")
+    check_backward(dy, in8(x, xc) if xc else x, w, in8(z, zc) if zc else z, "silu", t, got)
+
+
+def test_backward_only_what_is_asked_for():
+    dy, x, w, z = normal(1, 40, 24), normal(2, 40, 16), normal(3, 24, 16), normal(4, 40, 24)
+    full = ops.linear_backward(dy, x, w, z, activation="tanh")
+    for k in range(8):
+        want = [bool(k & 1), bool(k & 2), bool(k & 4)]
+        got = ops.linear_backward(dy, x if want[1] else None, w, z, activation="tanh", need_dx=want[0], need_dw=want[1], need_db=want[2])
+        for g, f, on in zip(got, full, want):
+            assert (g is None) == (not on) and (g is None or torch.equal(g, f))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_no_rows(t):
+    w = normal(1, 12, 8, t=t)
+    assert ops.linear(normal(2, 0, 8, t=t), w).shape == (0, 12)
+    dx, dw, db = ops.linear_backward(normal(2, 0, 12, t=t), normal(2, 0, 8, t=t), w, normal(2, 0, 12, t=t), activation="gelu")
+    assert dx.shape == (0, 8) and not dw.any() and not db.any() and dw.shape == (12, 8)
+    assert ops.embedding(torch.zeros(0, dtype=torch.int64, device=DEV), w).shape == (0, 8)
+    assert not ops.embedding_backward(normal(2, 0, 8, t=t), torch.zeros(0, dtype=torch.int64, device=DEV), 7).any()
+    c = ops.checkpoint8(normal(2, 0, 8, t=t))
+    assert c.values().shape == (0, 8)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", [(3, 24, 40), (50, 24, 40), (300, 136, 264)])
+def test_strides_and_alignment(t, m, k, n):
+    """views into wider matrices, at odd offsets; what lies around the output stays as it was"""
+    for off, pad in ((0, 8), (1, 3), (3, 0), (8, 16)):
+        big = normal(9, m, k + off + pad, t=t)
+        x = big[:, off:off + k]
+        w = normal(10, n, k + off + pad, t=t, by=0.2)[:, off:off + k]
+        r = normal(11, m, n + off + pad, t=t)[:, off:off + n]
+        b = normal(12, n + off, t=t)[off:]
+        hold = torch.full((m + 2, n + off + pad), 7.0, dtype=t, device=DEV)
+        y = hold[1:m + 1, off:off + n]
+        assert ops.linear(x, w, b, r, activation="tanh", out=y) is y
+        check_linear(x, w, b, r, "tanh", t, y.clone())
+        hold[1:m + 1, off:off + n] = 7.0
+        assert (hold == 7).all()
+        dy, z = normal(13, m, n + off + pad, t=t)[:, off:off + n], normal(14, m, n + off + pad, t=t)[:, off:off + n]
+        check_backward(dy, x, w, z, "gelu", t, ops.linear_backward(dy, x, w, z, activation="gelu"))
+        c = ops.checkpoint8(x, "e4m3")
+        assert torch.equal(c.values().double(), in8(x, "e4m3"))
+    x3 = normal(15, 4, 5, k, t=t)                                    # leading dimensions, and a layout that has to be copied
+    w = normal(16, n, k, t=t, by=0.2)
+    y3 = ops.linear(x3, w)
+    assert y3.shape == (4, 5, n) and torch.equal(y3.reshape(20, n), ops.linear(x3.reshape(20, k), w))
+    assert torch.equal(ops.linear(x3.transpose(0, 1), w), ops.linear(x3.transpose(0, 1).contiguous(), w))
+    assert torch.equal(ops.linear(x3[0], w.t().contiguous().t()), ops.linear(x3[0], w))
+    e = normal(17, 1, n, t=t).expand(20, n)                          # one row for all: a broadcast gradient
+    g = ops.linear_backward(e, x3.reshape(20, k), w)
+    for a, c in zip(g, ops.linear_backward(e.contiguous(), x3.reshape(20, k), w)):
+        assert torch.equal(a, c)
+
+
+def test_residual_may_be_the_output():
+    for t in TYPES:
+        for m in (2, 200):
+            x, w, r = normal(1, m, 64, t=t), normal(2, 72, 64, t=t, by=0.1), normal(3, m, 72, t=t)
+            want = ops.linear(x, w, None, r, activation="relu")
+            got = ops.linear(x, w, None, r, activation="relu", out=r)
+            assert got is r and torch.equal(want, r)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_magnitudes_far_apart(t):
+    """rows that differ by 2^40 (fp16: 2^12) each keep their own precision; nothing is scaled by another row's size"""
+    k = 96
+    x, w = normal(1, 160, k, t=F32), normal(2, 130, k, t=F32, by=k ** -0.5)
+    s = torch.exp2(torch.arange(160, device=DEV).float() % (12 if t is F16 else 40) - (6 if t is F16 else 20))
+    x = (x * s[:, None]).to(t)
+    w = (w * torch.exp2(-(torch.arange(130, device=DEV).float() % (4 if t is F16 else 30)))[:, None]).to(t)
+    check_linear(x, w, None, None, "none", t, ops.linear(x, w))
+    g = ops.linear_backward(x @ torch.zeros(k, 130, dtype=t, device=DEV) + normal(3, 160, 130, t=t) * s[:, None].to(t), x, w)
+    assert all(torch.isfinite(v).all() for v in g)
+    if t is F32:
+        big = x.clone()
+        big[0, 0], big[1, 1] = 3.4e38, -3.4e38                       # finite values at the end of the range
+        w0 = torch.zeros_like(w)
+        w0[:, 2:] = w[:, 2:]
+        assert torch.isfinite(ops.linear(big, w0)).all()
+
+
+def test_nan_stays_in_its_row():
+    for t in TYPES:
+        for m in (4, 200):
+            x, w = normal(1, m, 64, t=t), normal(2, 48, 64, t=t, by=0.1)
+            x[1, 3] = float("nan")
+            y = ops.linear(x, w, activation="relu")
+            assert y[1].isnan().all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
+
+
+# ---- 8-bit checkpoints ----------------------------------------------------------------------------------------------
+def in8(x, code):
+    """what the header says, in 64 bits: blocks of 32, the least power of two, nearest code with ties to even, the type's range kept"""
+    t = x.dtype
+    v = x.detach().double().cpu().reshape(-1, x.shape[-1])                           # on the host, whose pow is exact for whole exponents
+    m, n = v.shape
+    full = torch.zeros(m, -(-n // 32) * 32, dtype=torch.float64)
+    full[:, :n] = v
+    full = full.reshape(m, -1, 32)
+    fin = torch.isfinite(full)
+    most = torch.where(fin, full.abs(), 0.0).amax(2, keepdim=True)
+    top = 127.0 if code == "int8" else 448.0
+    e = torch.frexp(most).exponent - (7 if code == "int8" else 9)
+    p = torch.pow(torch.full_like(most, 2.0), e.clamp_min(-200))
+    p = torch.where(most > top * p, 2 * p, p).clamp_min(2.0 ** -126)
+    u = full / p
+    if code == "int8":
+        q = torch.round(u)
+    else:
+        step = torch.pow(torch.full_like(u, 2.0), torch.frexp(torch.where(fin, u, 0.0)).exponent.clamp_min(-5) - 4)
+        q = torch.round(torch.where(fin, u, 0.0) / step) * step
+    most_t = float(torch.finfo(t).max)
+    below = 63.0 if code == "int8" else 240.0
+    q = torch.where((q * p).abs() > most_t, torch.sign(q) * below, q)
+    return torch.where(fin, q * p, float("nan")).reshape(m, -1)[:, :n].reshape(x.shape).to(x.device)
+
+
+def same(a, b):
+    a, b = a.double().cpu(), b.double().cpu()
+    assert torch.equal(a.isnan(), b.isnan())
+    assert torch.equal(torch.nan_to_num(a, 0.0), torch.nan_to_num(b, 0.0))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 31), (2, 32), (3, 33), (5, 64), (7, 500), (65, 512), (130, 96), (1000, 40)])
+def test_checkpoint_values(t, code, m, n):
+    x = normal(m + n, m, n, t=F32)
+    x = (x * torch.exp2(normal(2, m, n) * 3)).to(t)
+    c = ops.checkpoint8(x, code)
+    assert c.codes.shape == (m, -(-n // 32) * 32) and c.nbytes == c.codes.numel() + c.scales.numel()
+    want = in8(x, code)
+    same(c.values(), want)
+    assert c.values().dtype is t and torch.equal(c.values().double(), want)          # the type holds them exactly
+    for o in TYPES:
+        same(c.values(o), want.to(o) if o is not F16 else want.float().to(o))
+    assert not c.codes[:, n:].any()
+    again = ops.checkpoint8(c.values(), code)                                        # a checkpoint of its own values is the same again
+    same(again.values(), want)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_checkpoint_special_values(t, code):
+    inf, nan, mx, tiny = float("inf"), float("nan"), torch.finfo(t).max, torch.finfo(t).tiny
+    rows = [[0.0] * 40, [inf] + [1.0] * 39, [nan, -inf, 0.5, -0.25] + [3.0] * 36, [mx, -mx] + [mx / 3] * 38, [tiny] * 40, [tiny / 4, -tiny / 8] + [0.0] * 38,
+            [127.0, 63.5, 0.5, 1.5, 2.5, -0.5, -1.5] + [1.0] * 33, [448.0, 17.0, 19.0, 0.001953125, 0.0009765625] + [2.0] * 35, [float(i) for i in range(40)],
+            [nan] * 40, [inf, -inf] * 20, [-127.5] + [0.3] * 39, [449.0, 447.0] + [1.0] * 38, [1e-3 * i for i in range(40)]]
+    x = torch.tensor(rows, dtype=torch.float64).to(t).to(DEV)
+    same(ops.checkpoint8(x, code).values(), in8(x, code))
+    x = x[:, :32].contiguous().repeat(1, 2)                                          # whole blocks
+    same(ops.checkpoint8(x, code).values(), in8(x, code))
+
+
+# ---- embedding ------------------------------------------------------------------------------------------------------
+IDS = [torch.uint8, torch.int32, torch.int64]
+
+
+def check_embedding(ids, table, dy, scale, y, dt, t):
+    v = table.shape[0]
+    i = ids.long().reshape(-1)
+    ok = (i >= 0) & (i < v)
+    ref = torch.zeros(len(i), table.shape[1], dtype=torch.float64, device=DEV)
+    ref[ok] = table.double()[i[ok]] * scale
+    within(y.reshape(ref.shape), ref, 2.0 ** -24 * ref.abs(), t)
+    d = dy.double().reshape(len(i), -1)[ok].cpu()
+    at = i[ok].cpu()
+    g = torch.zeros(v, table.shape[1], dtype=torch.float64).index_add_(0, at, d) * scale
+    sq = torch.zeros(v, table.shape[1], dtype=torch.float64).index_add_(0, at, d ** 2).sqrt() * abs(scale)
+    n = torch.bincount(at, minlength=v).double().sqrt()[:, None]
+    within(dt, g, 2.0 ** -24 * (8 * n + 8) * sq, t)
+    assert not dt.cpu()[n[:, 0] == 0].any()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens,rows,width", [(1, 1, 1), (1, 300, 8), (2, 5, 8), (31, 5, 8), (33, 4, 12), (64, 70, 9), (1000, 5, 8), (1024, 256, 40), (3000, 200, 264), (4097, 4097, 72),
+                                               (5000, 70000, 16), (20000, 33, 3), (9000, 17, 520), (300, 1000, 2056)])
+def test_embedding(t, tokens, rows, width):
+    for k, it in enumerate(IDS):
+        if it is torch.uint8 and rows > 256:
+            continue
+        g = torch.Generator().manual_seed(tokens + k)
+        ids = (torch.rand(tokens, generator=g) ** 3 * rows).long().clamp_max(rows - 1)
+        if it is not torch.uint8:
+            ids[5::17], ids[6::19] = -1, rows + 3                     # no tokens
+        ids = ids.to(it).to(DEV)
+        table, dy, scale = normal(1, rows, width, t=t), normal(2, tokens, width, t=t, by=0.1), (1.0, 0.125, width ** 0.5)[k]
+        check_embedding(ids, table, dy, scale, ops.embedding(ids, table, scale), ops.embedding_backward(dy, ids, rows, scale), t)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_embedding_extremes(t):
+    """every token the same; every token another one; none; the last row only; ids beyond 32 bits; rows that no token names"""
+    tokens, width = 9000, 24
+    table, dy = normal(1, 9000, width, t=t), normal(2, tokens, width, t=t, by=0.1)
+    for ids in (torch.zeros(tokens), torch.full((tokens,), 8999), torch.arange(tokens), torch.arange(tokens).flip(0), torch.full((tokens,), -1),
+                torch.arange(tokens) // 32, torch.arange(tokens) // 33 * 7, torch.arange(tokens) * (1 << 33), torch.arange(tokens) - (1 << 40)):
+        ids = ids.long().to(DEV)
+        check_embedding(ids, table, dy, 2.0, ops.embedding(ids, table, 2.0), ops.embedding_backward(dy, ids, 9000, 2.0), t)
+    ids = (torch.arange(tokens) % 7).to(torch.uint8).to(DEV)
+    out = torch.full((11, width + 5), 3.0, dtype=t, device=DEV)
+    ops.embedding_backward(dy, ids, 9, 1.0, out=out[1:10, 2:2 + width])
+    check_embedding(ids, table[:9], dy, 1.0, ops.embedding(ids, table[:9]), out[1:10, 2:2 + width], t)
+    out[1:10, 2:2 + width] = 3.0
+    assert (out == 3).all()
+    i2 = ids.reshape(9, 1000)
+    y = ops.embedding(i2, table[:9])
+    assert y.shape == (9, 1000, width) and torch.equal(ops.embedding_backward(dy.reshape(9, 1000, width), i2, 9), ops.embedding_backward(dy, ids, 9))
+    wide = normal(5, 9, 2 * width + 1, t=t)
+    view = wide[:, 1:1 + width]
+    assert torch.equal(ops.embedding(ids, view), ops.embedding(ids, view.contiguous()))
+
+
+# ---- how the calls are used -----------------------------------------------------------------------------------------
+def _step(s, stream=None):
+    """tokens -> embedding -> two layers with a residual -> gradients from 8-bit checkpoints -> the table's gradient"""
+    h = ops.embedding(s["ids"], s["table"], 4.0, stream=stream)
+    a, z = ops.linear(h, s["w1"], s["b1"], activation="gelu", keep_preact=True, stream=stream)
+    ch, cz, ca = ops.checkpoint8(h, "e4m3", stream=stream), ops.checkpoint8(z, "e4m3", stream=stream), ops.checkpoint8(a, "int8", stream=stream)
+    y = ops.linear(a, s["w2"], s["b2"], h, stream=stream)
+    da, dw2, db2 = ops.linear_backward(s["dy"], ca, s["w2"], stream=stream)
+    dh, dw1, db1 = ops.linear_backward(da, ch, s["w1"], cz, activation="gelu", stream=stream)
+    dh = dh + s["dy"] if stream is None else _add(dh, s["dy"], stream)               # the residual's gradient
+    return y, dw2, db2, dw1, db1, ops.embedding_backward(dh, s["ids"], len(s["table"]), 4.0, stream=stream)
+
+
+def _add(a, b, stream):
+    with torch.cuda.stream(stream):
+        return a + b
+
+
+def _state(seed, m=300, v=50, k=64, n=136, t=BF16):
+    g = torch.Generator().manual_seed(seed)
+    return {"ids": torch.randint(-1, v, (m,), generator=g).to(DEV), "table": normal(seed + 1, v, k, t=t, by=0.25), "w1": normal(seed + 2, n, k, t=t, by=k ** -0.5),
+            "b1": normal(seed + 3, n, t=t, by=0.1), "w2": normal(seed + 4, k, n, t=t, by=n ** -0.5), "b2": normal(seed + 5, k, t=t, by=0.1), "dy": normal(seed + 6, m, k, t=t, by=0.1)}
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_a_step_of_them_together(t):
+    """against autograd in 64 bits on the plain formulas: bounded by what 8-bit checkpoints and the types' roundings may do (relative 2-norm: e4m3 keeps a
+    factor within 2^-4, on average 2^-5.3; int8 of a block within 2^-7 of its largest; each gradient has two such factors at most)"""
+    s = _state(1, t=t)
+    got = _step(s)
+    p = {k: s[k].double().cpu().requires_grad_() for k in ("table", "w1", "b1", "w2", "b2")}
+    ids = s["ids"].cpu()
+    h = torch.where((ids >= 0)[:, None], p["table"][ids.clamp_min(0)] * 4.0, 0.0)
+    z = h @ p["w1"].t() + p["b1"]
+    y = (z * torch.special.ndtr(z)) @ p["w2"].t() + p["b2"] + h
+    (y * s["dy"].double().cpu()).sum().backward()
+    refs = (y.detach(), p["w2"].grad, p["b2"].grad, p["w1"].grad, p["b1"].grad, p["table"].grad)
+    lim = (8 * H[t], 2.0 ** -6 + 8 * H[t], 8 * H[t] + 2.0 ** -22, 2.0 ** -4, 2.0 ** -4, 2.0 ** -4)
+    for a, b, m in zip(got, refs, lim):
+        assert float((a.double().cpu() - b).norm() / b.norm()) <= m
+
+
+def test_the_same_bits_every_time_and_on_any_stream():
+    s = _state(2, m=5000)
+    first = _step(s)
+    side = torch.cuda.Stream()
+    for k in range(3):
+        for a, b in zip(first, _step(s)):
+            assert torch.equal(a, b)
+    torch.cuda.synchronize()
+    got = _step(s, stream=side)
+    junk = [torch.full((5000, 136), 9.0, device=DEV, dtype=BF16) for _ in range(8)]      # what the call's scratch was must not be handed out again under it
+    side.synchronize()
+    for a, b in zip(first, got):
+        assert torch.equal(a, b)
+    del junk
+    with pytest.raises(TypeError):
+        ops.linear(s["dy"], s["w1"], stream=7)
+
+
+def test_captured_and_replayed():
+    """two graphs of a step, replayed in turn with eager work between them, on inputs that change in place"""
+    sa, sb = _state(3), _state(40, m=777, v=5000, k=72, n=40)
+    graphs = []
+    for s in (sa, sb):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _step(s)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _step(s)
+        graphs.append((g, s, out))
+    for k in range(4):
+        for j, (g, s, out) in enumerate(graphs):
+            new = _state(100 * k + j, m=s["dy"].shape[0], v=s["table"].shape[0], k=s["table"].shape[1], n=s["w1"].shape[0])
+            for name in s:
+                s[name].copy_(new[name])
+            want = [v.clone() for v in _step(s)]
+            for v in out:
+                v.zero_()
+            g.replay()
+            if k % 2:
+                torch.cuda.synchronize()
+            for a, b in zip(want, out):
+                assert torch.equal(a, b)
+
+
+def test_gradient_against_differences():
+    """fp32: (L(p + h v) - L(p - h v)) / 2h = <grad, v> for L = sum(y g): the central difference is off by h^2 / 6 times the third derivative
+    (|act'''| < 2 over arguments that move by h |v.x| < 4h here: below 2^-12 of the norm at h = 2^-6) and by L's own rounding, 2^-22 |L|-sums / h"""
+    m, k, n, h = 96, 48, 80, 2.0 ** -6
+    x, w, b, g = normal(1, m, k), normal(2, n, k, by=k ** -0.5), normal(3, n, by=0.2), normal(4, m, n)
+    for act in ("tanh", "sigmoid", "gelu", "silu"):
+        y, z = ops.linear(x, w, b, activation=act, keep_preact=True)
+        grads = ops.linear_backward(g, x, w, z, activation=act)
+        for which, grad in enumerate(grads):
+            p = (x, w, b)[which]
+            v = torch.sign(grad)                                     # along the gradient, so that <grad, v> is not a small difference
+            v = v / (8 if which == 1 else 4 if which == 0 else 1)
+
+            def loss(s):
+                q = [x, w, b]
+                q[which] = p + s * h * v
+                return (ops.linear(*q, activation=act).double() * g.double()).sum()
+            num = float((loss(1) - loss(-1)) / (2 * h))
+            ana = float((grad.double() * v.double()).sum())
+            assert abs(num - ana) <= 0.01 * abs(ana), (act, which, num, ana)
+
+
+def test_refusals_on_the_gpu():
+    x, w = normal(1, 4, 8), normal(2, 6, 8)
+    for call in (lambda: ops.linear(x, w.half()), lambda: ops.linear(x[:, :7], w), lambda: ops.linear(x, w.cpu()), lambda: ops.linear(x, w, x[0]),
+                 lambda: ops.linear(x, w, residual=x), lambda: ops.linear(x, w, out=torch.empty(4, 7, device=DEV)), lambda: ops.linear(x, w, out=torch.empty(6, 4, device=DEV).t()),
+                 lambda: ops.linear_backward(x, x, w), lambda: ops.linear_backward(normal(1, 4, 6), x, w, activation="tanh"),
+                 lambda: ops.linear_backward(normal(1, 4, 6), ops.checkpoint8(x.half()), w), lambda: ops.linear_backward(normal(1, 4, 6), None, w),
+                 lambda: ops.embedding(torch.zeros(3, device=DEV), w), lambda: ops.embedding(torch.zeros(3, dtype=torch.int64), w),
+                 lambda: ops.embedding_backward(x, torch.zeros(5, dtype=torch.int64, device=DEV), 3), lambda: ops.embedding_backward(x, torch.zeros(4, dtype=torch.int64, device=DEV), 0),
+                 lambda: ops.checkpoint8(x.double()), lambda: ops.checkpoint8(x).values(torch.float64)):
+        with pytest.raises(ValueError):
+            call()

@@ -1,0 +1,142 @@
+"""The training operators' interface without a GPU: symbols, refusals before anything is launched, workspace sizes (include/ccsm_train_ops.h)."""
+import ctypes as C
+import os
+import re
+
+import pytest
+
+from conftest import ROOT
+from ccsmeth_amd import _lib, train_ops as ops
+
+torch = pytest.importorskip("torch")
+INVALID, CAPACITY = _lib.ERR_INVALID_ARG, _lib.ERR_CAPACITY
+A = 1 << 20                      # an aligned address that nothing follows
+
+
+def test_exports_match_header():
+    header = open(os.path.join(ROOT, "include", "ccsm_train_ops.h")).read()
+    declared = set(re.findall(r"\b(ccsm_train_[a-z0-9_]+)\s*\(", header))
+    assert declared == set(ops.EXPORTS)
+    lib = ops.load()
+    for name in declared:
+        assert hasattr(lib, name), name
+
+
+def _linear(**kw):
+    d = dict(type=2, activation=4, rows=64, inner=32, outer=48, x=A, ldx=32, w=A, ldw=32, bias=A, residual=A, ldr=48, y=A, ldy=48, preact=A, ldp=48)
+    d.update(kw)
+    return ops.Linear(**d)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(type=3), dict(type=-1), dict(activation=6), dict(activation=-1), dict(rows=-1), dict(rows=1 << 40), dict(inner=0), dict(outer=0), dict(inner=-8),
+    dict(x=None), dict(w=None), dict(y=None), dict(ldx=31), dict(ldw=0), dict(ldy=47), dict(ldr=40), dict(ldp=-48), dict(x=A + 1), dict(w=A + 1), dict(y=A + 1),
+    dict(bias=A + 1), dict(residual=A + 1), dict(preact=A + 1), dict(type=0, x=A + 2),
+])
+def test_linear_refuses(kw):
+    lib = ops.load()
+    p = _linear(**kw)
+    assert lib.ccsm_train_linear_forward(0, C.byref(p), A, 1 << 40, None) == INVALID
+    assert lib.ccsm_train_ops_last_error()
+    assert lib.ccsm_train_linear_workspace(C.byref(p)) == 0
+
+
+def test_linear_null_and_empty():
+    lib = ops.load()
+    assert lib.ccsm_train_linear_forward(0, None, None, 0, None) == INVALID
+    assert lib.ccsm_train_linear_forward(0, C.byref(_linear(rows=0, x=None, y=None)), None, 0, None) == 0       # nothing to do: nothing is launched
+
+
+def _grad(**kw):
+    s = dict(x=ops.Saved(A, 32, 0, None, 0), preact=ops.Saved(A, 48, 0, None, 0))
+    d = dict(type=2, activation=4, rows=64, inner=32, outer=48, dy=A, lddy=48, w=A, ldw=32, dx=A, lddx=32, dw=A, lddw=32, dbias=A, **s)
+    d.update(kw)
+    return ops.LinearGrad(**d)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(type=7), dict(activation=9), dict(rows=-1), dict(inner=0), dict(outer=0), dict(dy=None), dict(lddy=47), dict(w=None), dict(ldw=31), dict(lddx=31), dict(lddw=31),
+    dict(dy=A + 1), dict(dx=A + 1), dict(dw=A + 1), dict(dbias=A + 1),
+    dict(x=ops.Saved(None, 32, 0, None, 0)), dict(x=ops.Saved(A, 31, 0, None, 0)), dict(x=ops.Saved(A + 1, 32, 0, None, 0)), dict(preact=ops.Saved(None, 48, 0, None, 0)),
+    dict(x=ops.Saved(A, 32, 3, A, 1)), dict(x=ops.Saved(A, 32, 1, None, 1)), dict(x=ops.Saved(A, 33, 1, A, 1)), dict(x=ops.Saved(A, 0, 1, A, 1)),
+    dict(x=ops.Saved(A, 32, 2, A, 0)), dict(x=ops.Saved(A + 4, 32, 2, A, 1)), dict(preact=ops.Saved(A, 32, 2, A, 2)), dict(preact=ops.Saved(A, 64, 2, A, 1)),
+])
+def test_linear_backward_refuses(kw):
+    lib = ops.load()
+    p = _grad(**kw)
+    assert lib.ccsm_train_linear_backward(0, C.byref(p), A, 1 << 40, None) == INVALID
+    assert lib.ccsm_train_linear_backward_workspace(C.byref(p)) == 0
+
+
+def test_too_small_a_workspace_is_refused():
+    lib = ops.load()
+    p = _grad()
+    need = lib.ccsm_train_linear_backward_workspace(C.byref(p))
+    assert need > 0
+    assert lib.ccsm_train_linear_backward(0, C.byref(p), None, need, None) == CAPACITY
+    assert lib.ccsm_train_linear_backward(0, C.byref(p), A, need - 1, None) == CAPACITY
+    assert lib.ccsm_train_linear_backward(0, C.byref(p), A + 8, need, None) == INVALID
+    need = lib.ccsm_train_embedding_backward_workspace(1000, 5, 8)
+    assert need > 0
+    args = (0, 0, 1, 1000, A, 5, 8, A, 8, 1.0, A, 8)
+    assert lib.ccsm_train_embedding_backward(*args, None, 0, None) == CAPACITY
+    assert lib.ccsm_train_embedding_backward(*args, A, need - 1, None) == CAPACITY
+
+
+def test_embedding_and_act8_refuse():
+    lib = ops.load()
+    fwd = dict(type=0, id_type=2, tokens=10, ids=A, rows=5, width=8, table=A, ldt=8, scale=1.0, y=A, ldy=8)
+    for kw in (dict(type=3), dict(id_type=3), dict(tokens=-1), dict(ids=None), dict(ids=A + 4), dict(rows=0), dict(width=0), dict(table=None), dict(y=None), dict(ldt=7),
+               dict(ldy=7), dict(table=A + 2), dict(y=A + 2), dict(rows=1 << 40)):
+        d = dict(fwd, **kw)
+        assert lib.ccsm_train_embedding_forward(0, *d.values(), None) == INVALID, kw
+    bwd = dict(type=0, id_type=2, tokens=10, ids=A, rows=5, width=8, dy=A, lddy=8, scale=1.0, dt=A, ldt=8)
+    for kw in (dict(type=3), dict(id_type=-1), dict(tokens=-1), dict(ids=None), dict(rows=0), dict(width=-1), dict(dy=None), dict(dt=None), dict(lddy=7), dict(ldt=7), dict(dy=A + 1)):
+        d = dict(bwd, **kw)
+        assert lib.ccsm_train_embedding_backward(0, *d.values(), A, 1 << 40, None) == INVALID, kw
+    pack = dict(type=0, code=1, rows=4, width=40, x=A, ldx=40, codes=A, ldc=64, scales=A, lds=2)
+    for kw in (dict(type=9), dict(code=0), dict(code=3), dict(rows=-1), dict(width=0), dict(x=None), dict(ldx=39), dict(x=A + 2), dict(codes=None), dict(ldc=40), dict(ldc=32),
+               dict(ldc=65), dict(scales=None), dict(lds=1), dict(codes=A + 8)):
+        d = dict(pack, **kw)
+        assert lib.ccsm_train_act8_pack(0, *d.values(), None) == INVALID, kw
+    s = ops.Saved(A, 64, 1, A, 2)
+    assert lib.ccsm_train_act8_unpack(0, 0, 4, 40, None, A, 40, None) == INVALID
+    assert lib.ccsm_train_act8_unpack(0, 0, 4, 40, C.byref(s), A, 39, None) == INVALID
+    assert lib.ccsm_train_act8_unpack(0, 0, 4, 40, C.byref(ops.Saved(A, 64, 0, A, 2)), A, 40, None) == INVALID
+    assert lib.ccsm_train_act8_unpack(0, 0, 4, 65, C.byref(s), A, 65, None) == INVALID
+    assert lib.ccsm_train_act8_pack(0, 0, 1, 0, 40, None, 0, None, 0, None, 0, None) == 0        # no rows
+
+
+def test_python_refuses_before_the_library_is_called():
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.linear(x, w)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.linear_backward(torch.zeros(4, 6), x, w)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.checkpoint8(x)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.embedding(torch.zeros(3, dtype=torch.int64), x)
+    with pytest.raises(ValueError, match="activation"):
+        ops.linear(x, w, activation="softplus")
+    with pytest.raises(ValueError, match="code"):
+        ops.checkpoint8(x, "int4")
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        ops.linear(x.double(), w)
+    with pytest.raises(TypeError):
+        ops.linear([[1.0]], w)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.checkpoint8(torch.zeros(4, 8, requires_grad=True))
+
+
+def test_checkpoint_tensors_are_checked():
+    codes, scales = torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    c = ops.Checkpoint8(codes, scales, (2, 2, 40), torch.float16, "e4m3")
+    assert c.nbytes == 4 * 66 and tuple(c.shape) == (2, 2, 40)
+    for bad in ((codes[:, :40], scales), (codes, scales[:3]), (codes.float(), scales), (codes, scales.int())):
+        with pytest.raises(ValueError):
+            ops.Checkpoint8(*bad, (2, 2, 40), torch.float16, "e4m3")
+    with pytest.raises(ValueError):
+        ops.Checkpoint8(codes, scales, (2, 2, 40), torch.float64, "e4m3")
+    with pytest.raises(ValueError):
+        ops.Checkpoint8(codes, scales, (2, 2, 40), torch.float16, "fp4")

@@ -1,6 +1,7 @@
 // libccsm_train: the training operators' C-ABI (include/ccsm_train_ops.h).  Checks, workspace layout and launches; the kernels are in
 // ccsm_train_ops_linear.hip, ccsm_train_ops_embed.hip and ccsm_train_ops_act8.hip.
 #include <string>
+#include <type_traits>
 
 #include "../../include/ccsm_train_ops.h"
 #include "ccsm_train_ops_act8.hip"
@@ -79,10 +80,73 @@ ccsm_status check_saved(const ccsm_saved& s, int type, int64_t width, const char
 Saved saved_of(const ccsm_saved& s) { return Saved{s.data, s.ld, s.code, s.scales, s.lds}; }
 Saved plain(const void* p, int64_t ld) { return Saved{p, ld, kCodeNone, nullptr, 0}; }
 
-template <typename T>
-void product(hipStream_t st, Operand a, Operand b, int64_t M, int64_t N, int64_t K, const Epilogue& ep) {
-    product_fma_kernel<T><<<dim3((unsigned)cdiv(N, 64), (unsigned)cdiv(M, 64)), 256, 0, st>>>(a, b, M, N, K, ep);
+// An operand as the product kernel takes it: as it is where its rows consist of whole, aligned 16-byte pieces of the product's own 16-bit type,
+// else staged into planes of the scratch (fp32: three of bf16; 8-bit codes: one, bf16 for fp32).
+struct Staged { Plane p; int planes; };
+bool whole_rows(const void* p, int64_t ld, int64_t width, int type) {
+    const int64_t n = 16 / (int64_t)size_of(type);
+    return !off_by(p, 16) && ld % n == 0 && width % n == 0 && ld < (1 << 22);      // (the kernel's 32-bit offsets span a tile's rows)
 }
+template <typename T>
+Staged staged(const Saved& s, int64_t rows, int64_t width, Scratch& ws, hipStream_t st, bool count) {
+    const int type = TypeOf<T>::v;
+    const bool codes = s.code != kCodeNone;
+    if (type != CCSM_TYPE_F32 && !codes && whole_rows(s.data, s.ld, width, type)) return Staged{Plane{s.data, s.ld, 0}, 1};
+    const int planes = type == CCSM_TYPE_F32 && !codes ? 3 : 1;
+    const int64_t ld = (int64_t)up(width, 8), plane = rows * ld;
+    uint16_t* out = ws.take<uint16_t>((size_t)planes * plane);
+    if (!count) {
+        const bool whole = !off_by(s.data, 16) && s.ld % (16 / (int64_t)size_of(type)) == 0;
+        const unsigned grid = grid_of(cdiv(plane / 8, 256), 1 << 16);
+        if (codes) stage_kernel<T, true><<<grid, 256, 0, st>>>(s, rows, (int)width, whole, out, ld, plane);
+        else stage_kernel<T, false><<<grid, 256, 0, st>>>(s, rows, (int)width, whole, out, ld, plane);
+    }
+    return Staged{Plane{out, ld, plane}, planes};
+}
+
+template <typename T, bool TRP, bool TRQ, int B>
+hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
+    constexpr int lds = 4 * 2 * B * 64;
+    auto* f = &product_mfma_kernel<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
+    // (an attribute of the function on the current device; setting it again costs little, and there is no state to share between threads)
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    f<<<(unsigned)(a.tiles_i * a.tiles_j * a.splits), B == 256 ? 512 : 256, lds, st>>>(a);
+    return hipGetLastError();
+}
+// out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue
+template <typename T, bool TRP, bool TRQ>
+hipError_t product(hipStream_t st, const Staged& p, const Staged& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, bool count) {
+    ProductArgs a;
+    a.P = p.p; a.Q = q.p;
+    a.M = (int)M; a.N = (int)N; a.K = (int)K;
+    a.passes = p.planes == 1 ? 1 : q.planes == 1 ? 3 : 6;
+    a.ep = ep;
+    const int64_t steps = cdiv(K, 32) * a.passes;
+    const int64_t big = cdiv(M, 256) * cdiv(N, 256), small = cdiv(M, 128) * cdiv(N, 128);
+    const int B = big >= 200 ? 256 : 128;
+    a.tiles_i = (int)cdiv(M, B); a.tiles_j = (int)cdiv(N, B);
+    const int64_t tiles = B == 256 ? big : small, slots = B == 256 ? 256 : 512;
+    int64_t splits = tiles * 2 <= slots ? slots / tiles : 1;
+    const int64_t least = 16;                                     // steps of a split
+    if (splits > cdiv(steps, least)) splits = cdiv(steps, least);
+    a.steps = (int)(cdiv(cdiv(steps, splits), a.passes) * a.passes);
+    a.splits = (int)cdiv(steps, a.steps);
+    a.part_ld = (int64_t)up(N, 4);
+    a.part = a.splits > 1 ? ws.take<float>((size_t)a.splits * M * a.part_ld) : nullptr;
+    if (count) return hipSuccess;
+    hipError_t e = B == 256 ? launch_product<T, TRP, TRQ, 256>(a, st) : launch_product<T, TRP, TRQ, 128>(a, st);
+    if (e != hipSuccess || a.splits == 1) return e;
+    product_join_kernel<T><<<grid_of(cdiv(M * cdiv(N, 4), 256), 1 << 16), 256, 0, st>>>(a.part, a.splits, M, (int)N, a.part_ld, ep);
+    return hipGetLastError();
+}
+template <typename T>
+Epilogue epilogue(const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, int64_t ldp, int act) {
+    const size_t a = 4 * sizeof(T);
+    const bool vec = !off_by(y, a) && ldy % 4 == 0 && (!residual || (!off_by(residual, a) && ldr % 4 == 0)) && (!pre || (!off_by(pre, a) && ldp % 4 == 0));
+    return Epilogue{bias, residual, ldr, y, ldy, pre, ldp, act, vec};
+}
+#define TRY(x, what) do { hipError_t e_ = (x); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
 
 ccsm_status check_linear(const ccsm_linear* p) {
     REFUSE(!p, "linear: NULL argument");
@@ -97,10 +161,9 @@ ccsm_status check_linear(const ccsm_linear* p) {
 }
 template <typename T>
 ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bool count) {
-    if (count) return CCSM_OK;
-    Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
-    product<T>(st, Operand{plain(p->x, p->ldx), 0}, Operand{plain(p->w, p->ldw), 0}, p->rows, p->outer, p->inner, ep);
-    LAUNCHED("linear_forward");
+    const Staged x = staged<T>(plain(p->x, p->ldx), p->rows, p->inner, ws, st, count), w = staged<T>(plain(p->w, p->ldw), p->outer, p->inner, ws, st, count);
+    const Epilogue ep = epilogue<T>(p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation);
+    TRY((product<T, false, false>(st, x, w, p->rows, p->outer, p->inner, ep, ws, count)), "linear_forward");
     return CCSM_OK;
 }
 
@@ -138,19 +201,31 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         LAUNCHED("linear_backward");
         return CCSM_OK;
     }
-    const bool products = p->dx || p->dw, slope = p->activation != CCSM_ACT_NONE && products;
-    const int64_t parts = cdiv(M, 32);
-    T* d = slope ? ws.take<T>((size_t)M * N) : nullptr;
+    // d as the products take it: dy itself where there is no activation, the type is a 16-bit one and its rows are whole pieces
+    const bool products = p->dx || p->dw;
+    const Saved dy = plain(p->dy, p->lddy);
+    const bool none = p->activation == CCSM_ACT_NONE, direct = none && TypeOf<T>::v != CCSM_TYPE_F32 && whole_rows(p->dy, p->lddy, N, TypeOf<T>::v);
+    const int planes = TypeOf<T>::v == CCSM_TYPE_F32 ? 3 : 1;
+    const int64_t ldd = (int64_t)up(N, 8), plane = M * ldd, parts = cdiv(M, 32);
+    Staged d{Plane{p->dy, p->lddy, 0}, 1};
+    if (products && !direct) d = Staged{Plane{ws.take<uint16_t>((size_t)planes * plane), ldd, plane}, planes};
     float* part = p->dbias ? ws.take<float>((size_t)parts * N) : nullptr;
-    if (count) return CCSM_OK;
-    if (slope || p->dbias) {
-        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 256)), 256, 0, st>>>((const T*)p->dy, p->lddy, saved_of(p->preact), p->activation, M, N, d, N, part);
+    if (!count && (part || (products && !direct))) {
+        const int64_t n = 16 / (int64_t)sizeof(T);
+        const bool whole = !off_by(p->dy, 16) && p->lddy % n == 0, whole_z = !none && !off_by(p->preact.data, 16) && p->preact.ld % n == 0;
+        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 512)), 256, 0, st>>>(dy, whole, none ? dy : saved_of(p->preact), whole_z, p->activation, M, N,
+                                                                                     products && !direct ? const_cast<void*>(d.p.base) : nullptr, ldd, plane, part);
         if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 32), 256, 0, st>>>(part, parts, N, (T*)p->dbias);
+        LAUNCHED("linear_backward");
     }
-    const Saved dm = slope ? plain(d, N) : plain(p->dy, p->lddy);
-    if (p->dx) product<T>(st, Operand{dm, 0}, Operand{plain(p->w, p->ldw), 1}, M, K, N, Epilogue{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone});
-    if (p->dw) product<T>(st, Operand{dm, 1}, Operand{saved_of(p->x), 1}, N, K, M, Epilogue{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone});
-    LAUNCHED("linear_backward");
+    if (p->dx) {
+        const Staged w = staged<T>(plain(p->w, p->ldw), N, K, ws, st, count);
+        TRY((product<T, false, true>(st, d, w, M, K, N, epilogue<T>(nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone), ws, count)), "linear_backward: dx");
+    }
+    if (p->dw) {
+        const Staged x = staged<T>(saved_of(p->x), M, K, ws, st, count);
+        TRY((product<T, true, true>(st, d, x, N, K, M, epilogue<T>(nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone), ws, count)), "linear_backward: dw");
+    }
     return CCSM_OK;
 }
 
@@ -209,7 +284,7 @@ extern "C" {
 const char* ccsm_train_ops_last_error(void) { return g_err.c_str(); }
 
 size_t ccsm_train_linear_workspace(const ccsm_linear* p) {
-    if (check_linear(p) != CCSM_OK) return 0;
+    if (check_linear(p) != CCSM_OK || p->rows == 0) return 0;
     Scratch ws;
     TYPED(p->type, (void)linear_forward<T>(p, ws, nullptr, true));
     return ws.used;

@@ -44,16 +44,31 @@ __device__ __forceinline__ float phi_(float z, float* e) {
     const float q = 0.5f * *e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
     return z >= 0.f ? 1.f - q : q;
 }
-template <bool FAST>
-__device__ __forceinline__ float act_(float z, int act) {
+template <bool FAST, int N>
+__device__ __forceinline__ void act_all(float (&z)[N], int act) {
     float e;
     switch (act) {
-        case kActRelu: return z < 0.f ? 0.f : z;            // (a NaN stays one)
-        case kActTanh: return tanh_<FAST>(z);
-        case kActSigmoid: return sigmoid_<FAST>(z);
-        case kActGelu: return z * phi_<FAST>(z, &e);
-        case kActSilu: return z * sigmoid_<FAST>(z);
-        default: return z;
+        case kActRelu:
+#pragma unroll
+            for (int k = 0; k < N; ++k) z[k] = z[k] < 0.f ? 0.f : z[k];            // (a NaN stays one)
+            break;
+        case kActTanh:
+#pragma unroll
+            for (int k = 0; k < N; ++k) z[k] = tanh_<FAST>(z[k]);
+            break;
+        case kActSigmoid:
+#pragma unroll
+            for (int k = 0; k < N; ++k) z[k] = sigmoid_<FAST>(z[k]);
+            break;
+        case kActGelu:
+#pragma unroll
+            for (int k = 0; k < N; ++k) z[k] *= phi_<FAST>(z[k], &e);
+            break;
+        case kActSilu:
+#pragma unroll
+            for (int k = 0; k < N; ++k) z[k] *= sigmoid_<FAST>(z[k]);
+            break;
+        default: break;
     }
 }
 template <bool FAST>

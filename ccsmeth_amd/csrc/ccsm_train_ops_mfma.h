@@ -1,0 +1,429 @@
+// Training operators: the matrix product on the matrix cores.  out(i, j) = sum over k of P(i, k) Q(j, k), P and Q of 16-bit elements in device
+// memory, fp32 accumulators.
+//
+// Tile and waves.  A workgroup of four waves (2 x 2) owns BI x BJ outputs, a wave a quarter of them as 16 x 16 tiles of v_mfma_f32_16x16x32 (the shape
+// that costs least energy per flop here); the steps along k are 32 deep.  Q is the instruction's first operand, so that a lane ends with four
+// neighbouring j of one i: stores of four elements.
+//
+// Operands go from memory straight to LDS (buffer_load_dwordx4 ... lds, 1 KiB per wave and request), four stages deep: a stage is requested three
+// steps before it is read, and one barrier per step says both that a stage has landed (counted vmcnt) and that the oldest one is free.  The
+// fragments of step s + 1 are read from LDS while step s multiplies, so the matrix pipe waits for neither.
+//
+// Two storage forms of an operand, by which index is contiguous in memory:
+//   k (TR = false)   LDS rows of 32 k = 64 bytes; a fragment is one ds_read_b128 per lane; piece c (16 bytes) of row r lies at c ^ (r >> 1 & 3)
+//   i or j (TR)      LDS rows of BI or BJ elements, one per k; a fragment is two ds_read_b64_tr_b16 (the LDS transposes 4 x 16 blocks); the
+//                    32-byte piece p of row k lies at p ^ s(k), s = k & 3 | k >> 1 & 4: the eight rows that are read together lie in eight
+//                    different parts of the 256 bytes of banks
+// Both permutations are made on the source side (each lane requests the piece that belongs where its 16 bytes land).
+//
+// Ragged sizes: pieces beyond k's end get an offset outside the buffer resource and arrive as zeros; rows and columns beyond i's or j's end
+// repeat the last ones, and their results are not written.  What the kernel needs: 16-byte aligned bases and row strides (multiples of 8
+// elements), the contiguous extent a multiple of 8; other operands are staged first (stage_kernel).
+//
+// Passes.  An fp32 operand is staged as three 16-bit planes (bf16: v = v0 + v1 + v2 exactly, but for values below 2^-110), and the product is
+// six products of planes, (2,0) (0,2) (1,1) (1,0) (0,1) (0,0): what is left out is below 2^-25 of each product.  Each k step runs its passes one behind
+// the other, so that the planes are read again out of L2.
+#pragma once
+#include "ccsm_train_ops_common.h"
+
+namespace ccsm_ops {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+template <typename E> struct Mfma;
+template <> struct Mfma<f16> {
+    static __device__ __forceinline__ f32x4 run(s16x8 a, s16x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mfma<b16> {
+    static __device__ __forceinline__ f32x4 run(s16x8 a, s16x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+    }
+};
+
+// what a product's results go through: z = acc + bias; y = act(z) + residual.  With `part`, the accumulators go there instead (split k)
+struct Epilogue {
+    const void* bias; const void* residual; long long ldr; void* y; long long ldy; void* pre; long long ldp; int act;
+    int vec;                  // every row of y, pre and residual starts 4-element aligned
+};
+struct Plane { const void* base; long long ld; long long plane; };      // elements of 16 bits; `plane`: from one plane to the next
+struct ProductArgs {
+    Plane P, Q;
+    int M, N, K;
+    int passes;               // 1, 3 (P in three planes, Q in one) or 6
+    int tiles_i, tiles_j, splits, steps;      // steps of one split (a multiple of passes)
+    float* part; long long part_ld;           // [split][M][part_ld]
+    Epilogue ep;
+};
+
+// N results (i, j .. j + N - 1), of which the first `left` exist
+template <typename T, int N>
+__device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, int left, float (&z)[N]) {
+    constexpr bool fast = sizeof(T) == 2;
+    typedef Vec<T, 4> V;
+    const bool whole = e.vec && left >= N;
+    if (e.bias) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) if (k < left) z[k] += (float)((const T*)e.bias)[j + k];
+    }
+    if (e.pre) {
+        T* o = (T*)e.pre + i * e.ldp + j;
+        if (whole) {
+#pragma unroll
+            for (int q = 0; q < N; q += 4) {
+                V v;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v.v[k] = (T)z[q + k];
+                *(V*)(o + q) = v;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) if (k < left) o[k] = (T)z[k];
+        }
+    }
+    act_all<fast, N>(z, e.act);
+    if (e.residual) {
+        const T* o = (const T*)e.residual + i * e.ldr + j;
+        if (whole) {
+#pragma unroll
+            for (int q = 0; q < N; q += 4) {
+                const V v = *(const V*)(o + q);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[q + k] += (float)v.v[k];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) if (k < left) z[k] += (float)o[k];
+        }
+    }
+    T* o = (T*)e.y + i * e.ldy + j;
+    if (whole) {
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            V v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v.v[k] = (T)z[q + k];
+            *(V*)(o + q) = v;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) if (k < left) o[k] = (T)z[k];
+    }
+}
+
+// One operand's side of the tile: requests and fragment reads.  B: the tile's extent, W: a wave's, NW waves in the workgroup.
+template <bool TR, int B, int W, int NW>
+struct Side {
+    static constexpr int kStage = B * 64;                  // bytes
+    static constexpr int kReq = kStage / 1024 / NW;        // requests per wave and stage
+    static constexpr int kFrag = W / 16;
+    unsigned off[kReq];                                    // byte offset of this lane's piece from the stage's origin
+    int kpos[kReq];                                        // its k within the stage
+    unsigned rd[TR ? kFrag : 1];                           // LDS byte offsets of the fragments
+
+    __device__ __forceinline__ void init(const Plane& p, int at, int extent, int wave, int lane, int w0, unsigned lds) {
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) {
+            const int q = r * NW + wave;                   // request number within the stage
+            if (!TR) {
+                const int row = q * 16 + (lane >> 2), c = (lane & 3) ^ ((row >> 1) & 3);
+                const int i = at + row < extent ? row : extent - 1 - at;
+                off[r] = (unsigned)(((long long)i * p.ld + 8 * c) * 2);
+                kpos[r] = 8 * c;
+            } else {
+                constexpr int kRow = B / 8;                // 16-byte pieces per row
+                const int k = (q * 64 + lane) / kRow, x = (q * 64 + lane) % kRow;
+                const int s = (k & 3) | ((k >> 1) & 4), c = (((x >> 1) ^ s) << 1) | (x & 1);
+                const int i = at + 8 * c < extent ? 8 * c : ((extent - 1) & ~7) - at;
+                off[r] = (unsigned)(((long long)k * p.ld + i) * 2);
+                kpos[r] = k;
+            }
+        }
+        if (!TR) {
+            rd[0] = lds + (unsigned)((w0 + (lane & 15)) * 64 + (((lane >> 4) ^ ((lane >> 1) & 3)) << 4));
+        } else {
+            const int k = 8 * (lane >> 4) + ((lane & 15) >> 2), s = (k & 3) | ((k >> 1) & 4);
+#pragma unroll
+            for (int f = 0; f < kFrag; ++f) rd[f] = lds + (unsigned)(k * (2 * B) + (((w0 / 16 + f) ^ s) << 5) + (lane & 3) * 8);
+        }
+    }
+    // request r of a stage into LDS at `m0` (the wave's base of that request)
+    __device__ __forceinline__ void request(int r, u32x4 srd, int left, unsigned m0) const {
+        const unsigned o = kpos[r] < left ? off[r] : 0xffffffffu;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m0), "v"(o), "s"(srd) : "memory");
+    }
+    __device__ __forceinline__ s16x8 fragment(int f, int stage) const {
+        typedef __attribute__((address_space(3))) const s16x8* P8;
+        typedef __attribute__((address_space(3))) s16x4* P4;
+        if (!TR) return *(P8)(uintptr_t)(rd[0] + f * 1024 + stage * kStage);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + stage * kStage));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + stage * kStage + 8 * B));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+template <typename T, bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_mfma_kernel(ProductArgs a) {
+    typedef typename std::conditional<sizeof(T) == 4, b16, T>::type E;
+    constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
+    typedef Side<TRP, BI, BI / WI, NW> SP;
+    typedef Side<TRQ, BJ, BJ / WJ, NW> SQ;
+    extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
+    // Workgroups go to the eight XCDs in turn; each XCD takes one contiguous eighth of the tiles (its L2 holds their operands), in columns of eight
+    // tiles along i, so that the 32 tiles of an XCD that run together share eight strips of P and four of Q
+    const int n = a.tiles_i * a.tiles_j * a.splits, b = blockIdx.x;
+    const int each = n >> 3, over = n & 7, x = b & 7;
+    int t = x * each + (x < over ? x : over) + (b >> 3);
+    const int split = t / (a.tiles_i * a.tiles_j);
+    t -= split * (a.tiles_i * a.tiles_j);
+    const int band = t / (8 * a.tiles_j), in = t - band * 8 * a.tiles_j, rows = a.tiles_i - 8 * band < 8 ? a.tiles_i - 8 * band : 8;
+    const int ti = 8 * band + in % rows, tj = in / rows;
+    const int i0 = ti * BI, j0 = tj * BJ;
+
+    const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
+    SP sp;
+    SQ sq;
+    sp.init(a.P, i0, a.M, wave, lane, wi * (BI / WI), lds);
+    sq.init(a.Q, j0, a.N, wave, lane, wj * (BJ / WJ), lds + 4 * SP::kStage);
+
+    const int total = (a.K + 31) / 32 * a.passes, first = split * a.steps, last = first + a.steps < total ? first + a.steps : total;
+    int k = first / a.passes * 32, pass = 0;               // of the next stage to be requested (splits begin with a k step's first pass)
+    const char* pb = (const char*)a.P.base + (TRP ? (long long)i0 * 2 : (long long)i0 * a.P.ld * 2);
+    const char* qb = (const char*)a.Q.base + (TRQ ? (long long)j0 * 2 : (long long)j0 * a.Q.ld * 2);
+    int left_stages = last - first;
+    u32x4 srdp, srdq;
+    int left = 0;
+    auto next = [&]() {                                    // the origins of the next stage
+        const int cp = a.passes == 1 ? 0 : a.passes == 3 ? 2 - pass : (0x010102 >> (4 * pass)) & 3, cq = a.passes == 6 ? (0x001120 >> (4 * pass)) & 3 : 0;
+        const unsigned long long p = (unsigned long long)(pb + ((TRP ? (long long)k * a.P.ld : (long long)k) + cp * a.P.plane) * 2);
+        const unsigned long long q = (unsigned long long)(qb + ((TRQ ? (long long)k * a.Q.ld : (long long)k) + cq * a.Q.plane) * 2);
+        srdp = u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, 0xfffffffeu, 0x00020000u};
+        srdq = u32x4{(unsigned)q, (unsigned)(q >> 32) & 0xffffu, 0xfffffffeu, 0x00020000u};
+        left = left_stages > 0 ? a.K - k : 0;              // behind the last stage: everything is out of range, zeros that nobody reads
+        --left_stages;
+        if (++pass == a.passes) { pass = 0; k += 32; }
+    };
+    constexpr int kReq = SP::kReq + SQ::kReq;
+    auto request = [&](int r, int stage) {
+        if (r < SP::kReq) sp.request(r, srdp, left, lds + stage * SP::kStage + (r * NW + wave) * 1024);
+        else sq.request(r - SP::kReq, srdq, left, lds + 4 * SP::kStage + stage * SQ::kStage + ((r - SP::kReq) * NW + wave) * 1024);
+    };
+
+    f32x4 acc[FI][FJ];
+#pragma unroll
+    for (int p = 0; p < FI; ++p)
+#pragma unroll
+        for (int q = 0; q < FJ; ++q) acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    s16x8 fp[2][FI], fq[2][FJ];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        next();
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) request(r, s);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(3 * kReq) : "memory");
+#pragma unroll
+    for (int p = 0; p < FI; ++p) fp[0][p] = sp.fragment(p, 0);
+#pragma unroll
+    for (int q = 0; q < FJ; ++q) fq[0][q] = sq.fragment(q, 0);
+
+    auto body = [&](auto S) {                              // step s with s % 4 = S
+        constexpr int s = decltype(S)::value, cur = s & 1, nxt = cur ^ 1, stage = (s + 1) & 3;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * kReq) : "memory");
+        next();
+        constexpr int kReads = FI + FJ;
+#pragma unroll
+        for (int p = 0; p < FI; ++p) {
+            // spread over the step: the next step's fragments first, a request of the fourth next stage behind each row of products
+#pragma unroll
+            for (int f = p * kReads / FI; f < (p + 1) * kReads / FI; ++f) {
+                if (f < FJ) fq[nxt][f] = sq.fragment(f, stage);
+                else fp[nxt][f - FJ] = sp.fragment(f - FJ, stage);
+            }
+#pragma unroll
+            for (int q = 0; q < FJ; ++q) acc[p][q] = Mfma<E>::run(fq[cur][q], fp[cur][p], acc[p][q]);
+#pragma unroll
+            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request(r, s);
+        }
+    };
+    // four steps a turn (the steps behind the last one multiply zeros): leaving between them would cost copies of every register at each exit
+    for (int turns = (last - first + 3) >> 2; turns > 0; --turns) {
+        body(std::integral_constant<int, 0>());
+        body(std::integral_constant<int, 1>());
+        body(std::integral_constant<int, 2>());
+        body(std::integral_constant<int, 3>());
+    }
+    // The results leave through the wave's own quarter of LDS, 32 rows of i at a time (rows 16 bytes longer than they need: the lanes' writes fall on
+    // different banks): a row's results then leave in pieces of eight neighbours
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // no request may still write LDS
+    constexpr int WJT = BJ / WJ, kRow = WJT + 4, kPer = WJT / 8;
+    static_assert(32 * kRow * 4 * NW <= 4 * (SP::kStage + SQ::kStage), "the waves' rows fit into the stages");
+    float* out = reinterpret_cast<float*>(ops_smem) + wave * 32 * kRow;
+#pragma unroll 1
+    for (int h = 0; h < FI / 2; ++h) {
+#pragma unroll
+        for (int p = 0; p < FI; ++p) {
+            if (p / 2 != h) continue;
+#pragma unroll
+            for (int q = 0; q < FJ; ++q) *(f32x4*)(out + (16 * (p & 1) + (lane & 15)) * kRow + 16 * q + 4 * (lane >> 4)) = acc[p][q];
+        }
+        const int ih = i0 + wi * (BI / WI) + 32 * h, jw = j0 + wj * WJT;
+#pragma unroll 1
+        for (int e = lane; e < 32 * kPer; e += 64) {
+            const int i = ih + e / kPer, c = e % kPer * 8, j = jw + c;
+            if (i >= a.M || j >= a.N) continue;
+            const f32x4 u = *(const f32x4*)(out + e / kPer * kRow + c), v = *(const f32x4*)(out + e / kPer * kRow + c + 4);
+            if (a.part) {
+                float* o = a.part + ((long long)split * a.M + i) * a.part_ld + j;
+                *(f32x4*)o = u;
+                if (j + 4 < a.N) *(f32x4*)(o + 4) = v;
+            } else {
+                float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                finish<T, 8>(a.ep, i, j, a.N - j, z);
+            }
+        }
+    }
+}
+
+// the splits' parts in order, and the epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void product_join_kernel(const float* part, int splits, long long M, int N, long long ld, Epilogue ep) {
+    const int nj = (N + 3) / 4;
+    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < M * nj; x += (long long)gridDim.x * 256) {
+        const long long i = x / nj;
+        const int j = (int)(x % nj) * 4;
+        f32x4 v = *(const f32x4*)(part + i * ld + j);
+        for (int s = 1; s < splits; ++s) v += *(const f32x4*)(part + ((long long)s * M + i) * ld + j);
+        float z[4] = {v[0], v[1], v[2], v[3]};
+        finish<T, 4>(ep, i, j, N - j, z);
+    }
+}
+
+// v as three bf16 values whose sum it is (each rounded to nearest; a finite value never becomes infinite; infinities and NaN make all of it NaN)
+__device__ __forceinline__ void three(float v, b16 (&p)[3]) {
+    p[0] = (b16)v;
+    if (fabsf(v) < INFINITY && !(fabsf((float)p[0]) < INFINITY)) p[0] = __builtin_bit_cast(b16, (unsigned short)(__float_as_uint(v) >> 16));
+    const float r = v - (float)p[0];
+    p[1] = (b16)r;
+    p[2] = (b16)(r - (float)p[1]);
+}
+template <typename T, int N> struct Planes;       // N values into the planes of a staged operand
+template <int N> struct Planes<float, N> {
+    static constexpr int n = 3;
+    static __device__ __forceinline__ void put(const float (&v)[N], void* out, long long plane, long long at) {
+        Vec<b16, N> o[3];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            b16 p[3];
+            three(v[k], p);
+            o[0].v[k] = p[0]; o[1].v[k] = p[1]; o[2].v[k] = p[2];
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *(Vec<b16, N>*)((b16*)out + q * plane + at) = o[q];
+    }
+};
+template <int N> struct Planes<f16, N> {
+    static constexpr int n = 1;
+    static __device__ __forceinline__ void put(const float (&v)[N], void* out, long long, long long at) {
+        Vec<f16, N> o;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o.v[k] = (f16)v[k];
+        *(Vec<f16, N>*)((f16*)out + at) = o;
+    }
+};
+template <int N> struct Planes<b16, N> {
+    static constexpr int n = 1;
+    static __device__ __forceinline__ void put(const float (&v)[N], void* out, long long, long long at) {
+        Vec<b16, N> o;
+#pragma unroll
+        for (int k = 0; k < N; ++k) o.v[k] = (b16)v[k];
+        *(Vec<b16, N>*)((b16*)out + at) = o;
+    }
+};
+
+// eight values of row r from column c on, zeros beyond the width; whole: aligned pieces can be loaded at once
+template <typename T>
+__device__ __forceinline__ void load8(const Saved& s, long long r, int c, int width, bool whole, float (&v)[8]) {
+    if (s.code != kCodeNone) {                    // (a code row covers whole blocks of 32, 16-byte aligned)
+        const uint2 u = *(const uint2*)((const uint8_t*)s.data + r * s.ld + c);
+        const float k = pow2_of_byte(s.scales[r * s.lds + (c >> 5)]);
+        float a[4], b[4];
+        if (s.code == kCodeInt8) { decode4<kCodeInt8>(u.x, k, a); decode4<kCodeInt8>(u.y, k, b); }
+        else { decode4<kCodeE4m3>(u.x, k, a); decode4<kCodeE4m3>(u.y, k, b); }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+        return;
+    }
+    const T* p = (const T*)s.data + r * s.ld + c;
+    if (whole && c + 8 <= width) {
+        constexpr int P = 16 / sizeof(T);
+#pragma unroll
+        for (int q = 0; q < 8 / P; ++q) {
+            const Vec<T, P> t = *(const Vec<T, P>*)(p + q * P);
+#pragma unroll
+            for (int k = 0; k < P; ++k) v[q * P + k] = (float)t.v[k];
+        }
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = c + q < width ? (float)p[q] : 0.f;
+}
+
+// a kept matrix as planes of 16-bit elements with rows of whole 16-byte pieces (zeros behind the width).  ONE: one plane whatever the type (8-bit
+// codes, whose values bf16 holds exactly)
+template <typename T, bool ONE>
+__global__ __launch_bounds__(256) void stage_kernel(Saved s, long long rows, int width, bool whole, void* out, long long ld, long long plane) {
+    const int n = (int)(ld / 8);
+    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < rows * n; x += (long long)gridDim.x * 256) {
+        const long long r = x / n;
+        const int c = (int)(x % n) * 8;
+        float v[8];
+        load8<T>(s, r, c, width, whole, v);
+        typedef typename std::conditional<ONE && sizeof(T) == 4, b16, T>::type O;
+        Planes<O, 8>::put(v, out, plane, r * ld + c);
+    }
+}
+
+// d = dy act'(z) into planes (16-bit types: one, rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 512 columns: 64 lanes of eight
+// columns, four rows at a time.
+// Rounding d: 16-bit products take 16-bit operands, and this rounding (half a step per factor, independent of each other) moves a gradient by
+// no more than the rounding of the gradient itself does.  The bias gradient takes d before it.
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(Saved dy, bool whole_dy, Saved z, bool whole_z, int act, long long M, int N, void* d, long long ldd, long long plane, float* part) {
+    constexpr bool fast = sizeof(T) == 2;
+    __shared__ float sum[4][512];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 512 + lane * 8;
+    const long long m0 = (long long)blockIdx.x * 32;
+    float acc[8] = {};
+    if (c < N)
+        for (int r = w; r < 32 && m0 + r < M; r += 4) {
+            float v[8];
+            load8<T>(dy, m0 + r, c, N, whole_dy, v);
+            if (act != kActNone) {
+                float u[8];
+                load8<T>(z, m0 + r, c, N, whole_z, u);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = c + k < N ? v[k] * slope_<fast>(u[k], act) : 0.f;
+            }
+            if (d) Planes<T, 8>::put(v, d, plane, (m0 + r) * ldd + c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += v[k];
+        }
+    if (!part) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[w][lane * 8 + k] = acc[k];
+    __syncthreads();
+    for (int k = threadIdx.x; k < 512; k += 256) {
+        const int n = blockIdx.y * 512 + k;
+        if (n < N) part[(long long)blockIdx.x * N + n] = (sum[0][k] + sum[1][k]) + (sum[2][k] + sum[3][k]);
+    }
+}
+
+}  // namespace ccsm_ops

@@ -45,6 +45,8 @@ def test_linear_null_and_empty():
     lib = ops.load()
     assert lib.ccsm_train_linear_forward(0, None, None, 0, None) == INVALID
     assert lib.ccsm_train_linear_forward(0, C.byref(_linear(rows=0, x=None, y=None)), None, 0, None) == 0       # nothing to do: nothing is launched
+    assert lib.ccsm_train_linear_workspace(C.byref(_linear(rows=0))) == 0 and lib.ccsm_train_linear_backward_workspace(C.byref(_grad(rows=0))) == 0
+    assert lib.ccsm_train_embedding_backward_workspace(0, 5, 8) == 0
 
 
 def _grad(**kw):

@@ -215,7 +215,7 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         const bool whole = !off_by(p->dy, 16) && p->lddy % n == 0, whole_z = !none && !off_by(p->preact.data, 16) && p->preact.ld % n == 0;
         slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 512)), 256, 0, st>>>(dy, whole, none ? dy : saved_of(p->preact), whole_z, p->activation, M, N,
                                                                                      products && !direct ? const_cast<void*>(d.p.base) : nullptr, ldd, plane, part);
-        if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 32), 256, 0, st>>>(part, parts, N, (T*)p->dbias);
+        if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 8), 256, 0, st>>>(part, (int)parts, N, (T*)p->dbias);
         LAUNCHED("linear_backward");
     }
     if (p->dx) {
@@ -229,48 +229,58 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
     return CCSM_OK;
 }
 
-struct SortPlan { int bits, passes, digit; int64_t blocks, pieces; };
+// Rows of a call are taken in ranges of at most 2^30 items (a lane's work), so that an item's number fits 31 bits
+constexpr int64_t kMostItems = (int64_t)1 << 30;
+template <typename F>
+void in_ranges(int64_t rows, int64_t per_row, F launch) {
+    const int64_t step = kMostItems / per_row > 0 ? kMostItems / per_row : 1;
+    for (int64_t r = 0; r < rows; r += step) launch(r, rows - r < step ? rows - r : step);
+}
+
+struct SortPlan { int bits, passes, digit, per_lane; int64_t blocks, pieces; };
 SortPlan sort_plan(int64_t tokens, int64_t rows) {
     SortPlan s;
     s.bits = 1;
     while (((int64_t)1 << s.bits) < rows + 1) ++s.bits;          // ids 0 .. rows (rows = no token)
     s.passes = (s.bits + 7) / 8;
     s.digit = (s.bits + s.passes - 1) / s.passes;
-    s.blocks = cdiv(tokens, kSortItems);
+    s.per_lane = tokens <= 262144 ? 4 : 16;                      // 1024 tokens a workgroup until the chip is full of them (19 -> 6 us a pass at 65536), then 4096
+    s.blocks = cdiv(tokens, 256 * s.per_lane);
     s.pieces = cdiv(tokens, kPiece);
     return s;
 }
-struct EmbedScratch { unsigned *keys[2], *at[2], *counts; float* part; };
-EmbedScratch embed_scratch(Scratch& ws, const SortPlan& s, int64_t tokens, int width) {
+struct EmbedScratch { unsigned *keys[2], *at[2], *counts, *marks; int64_t mark_words; float* part; int64_t part_ld; };
+EmbedScratch embed_scratch(Scratch& ws, const SortPlan& s, int64_t tokens, int64_t rows, int width) {
     EmbedScratch e;
     for (int k = 0; k < 2; ++k) {
         e.keys[k] = ws.take<unsigned>(tokens);
         e.at[k] = ws.take<unsigned>(tokens);
     }
     e.counts = ws.take<unsigned>((size_t)s.blocks << s.digit);
-    e.part = ws.take<float>((size_t)2 * s.pieces * width);
+    e.mark_words = cdiv(rows, 4);
+    e.marks = ws.take<unsigned>(e.mark_words);
+    e.part_ld = (int64_t)up(width, 8);
+    e.part = ws.take<float>((size_t)2 * s.pieces * e.part_ld);
     return e;
 }
 ccsm_status check_embedding(int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int width) {
     REFUSE(!good_type(type), "embedding: unknown type");
     REFUSE(id_type < CCSM_ID_U8 || id_type > CCSM_ID_I64, "embedding: unknown type of ids");
     REFUSE(tokens < 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols, "embedding: sizes out of range");
+    REFUSE(tokens * width > ((int64_t)1 << 37), "embedding: more values than a GPU holds");
     REFUSE(tokens && !ids, "embedding: ids must be non-NULL");
     REFUSE(off_by(ids, id_type == CCSM_ID_U8 ? 1 : id_type == CCSM_ID_I32 ? 4 : 8), "embedding: ids are not aligned to their elements");
     return CCSM_OK;
 }
-// 16-byte pieces where every row of both matrices consists of whole, aligned ones
-bool whole_pieces(int type, int width, const void* a, int64_t lda, const void* b, int64_t ldb) {
-    const int n = 16 / (int)size_of(type);
-    return width % n == 0 && lda % n == 0 && ldb % n == 0 && !off_by(a, 16) && !off_by(b, 16);
+template <int Q>
+void sort_pass(hipStream_t st, const SortPlan& s, const EmbedScratch& b, const void* ids, int id_type, int64_t tokens, int64_t rows, int pass, int k) {
+    const unsigned *keys = pass ? b.keys[k] : nullptr, *at = pass ? b.at[k] : nullptr;
+    const int bins = 1 << s.digit;
+    sort_count_kernel<Q><<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, tokens, rows, pass * s.digit, bins, b.counts, pass ? nullptr : b.marks, b.mark_words);
+    sort_scan_kernel<<<1, 1024, 0, st>>>(b.counts, s.blocks << s.digit);
+    sort_scatter_kernel<Q><<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, at, tokens, rows, pass * s.digit, bins, b.counts, b.keys[k ^ 1], b.at[k ^ 1],
+                                                               pass + 1 == s.passes ? (uint8_t*)b.marks : nullptr);
 }
-template <typename T, int N>
-void embedding_sums(hipStream_t st, const SortPlan& s, const EmbedScratch& e, int64_t tokens, int64_t rows, int width, const void* dy, int64_t lddy, float scale, void* dt, int64_t ldt, int k) {
-    const int lanes = width / N;
-    piece_sum_kernel<T, N><<<(unsigned)cdiv(s.pieces * lanes, 256), 256, 0, st>>>(e.keys[k], e.at[k], tokens, rows, lanes, width, (const T*)dy, lddy, scale, (T*)dt, ldt, e.part);
-    join_kernel<T><<<(unsigned)(s.pieces + grid_of(rows, 4096)), 256, 0, st>>>(e.keys[k], tokens, rows, width, scale, (T*)dt, ldt, e.part, s.pieces);
-}
-
 ccsm_status check_room(size_t need, const void* workspace, size_t have) {
     if (need && (!workspace || have < need)) return fail(CCSM_ERR_CAPACITY, "the workspace is too small");
     REFUSE(need && off_by(workspace, 256), "the workspace is not 256-byte aligned");
@@ -323,10 +333,12 @@ ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int6
     REFUSE(off_by(table, size_of(type)) || off_by(y, size_of(type)), "embedding: a pointer is not aligned to its elements");
     ON_DEVICE(device);
     hipStream_t st = (hipStream_t)stream;
-    const bool whole = whole_pieces(type, width, table, ldt, y, ldy);
-    TYPED(type, constexpr int P = 16 / sizeof(T);
-          if (whole) lookup_kernel<T, P><<<grid_of(cdiv(tokens * (width / P), 256)), 256, 0, st>>>(ids, id_type, tokens, rows, width / P, (const T*)table, ldt, scale, (T*)y, ldy);
-          else lookup_kernel<T, 1><<<grid_of(cdiv(tokens * width, 256)), 256, 0, st>>>(ids, id_type, tokens, rows, width, (const T*)table, ldt, scale, (T*)y, ldy));
+    TYPED(type, constexpr int P = 16 / sizeof(T); const int64_t pieces = cdiv(width, P);
+          in_ranges(tokens, pieces, [&](int64_t t, int64_t n) {
+              const char* i = (const char*)ids + t * (id_type == CCSM_ID_U8 ? 1 : id_type == CCSM_ID_I32 ? 4 : 8);
+              lookup_kernel<T, P><<<(unsigned)cdiv(n * pieces, 256), 256, 0, st>>>(i, id_type, (unsigned)(n * pieces), Div::by((unsigned)pieces), rows, width, (const T*)table, ldt,
+                                                                                 scale, (T*)y + t * ldy, ldy);
+          }));
     LAUNCHED("embedding_forward");
     return CCSM_OK;
 }
@@ -334,7 +346,7 @@ ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int6
 size_t ccsm_train_embedding_backward_workspace(int64_t tokens, int64_t rows, int32_t width) {
     if (tokens <= 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols) return 0;
     Scratch ws;
-    (void)embed_scratch(ws, sort_plan(tokens, rows), tokens, width);
+    (void)embed_scratch(ws, sort_plan(tokens, rows), tokens, rows, width);
     return ws.used;
 }
 ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
@@ -355,20 +367,16 @@ ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int
     Scratch ws;
     ws.base = (char*)workspace;
     const SortPlan s = sort_plan(tokens, rows);
-    const EmbedScratch b = embed_scratch(ws, s, tokens, width);
-    const int bins = 1 << s.digit;
+    const EmbedScratch b = embed_scratch(ws, s, tokens, rows, width);
     int k = 0;
-    for (int pass = 0; pass < s.passes; ++pass) {
-        const unsigned *keys = pass ? b.keys[k] : nullptr, *at = pass ? b.at[k] : nullptr;
-        sort_count_kernel<<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, tokens, rows, pass * s.digit, bins, b.counts);
-        sort_scan_kernel<<<1, 1024, 0, st>>>(b.counts, s.blocks << s.digit);
-        sort_scatter_kernel<<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, at, tokens, rows, pass * s.digit, bins, b.counts, b.keys[k ^ 1], b.at[k ^ 1]);
-        k ^= 1;
+    for (int pass = 0; pass < s.passes; ++pass, k ^= 1) {
+        if (s.per_lane == 4) sort_pass<4>(st, s, b, ids, id_type, tokens, rows, pass, k);
+        else sort_pass<16>(st, s, b, ids, id_type, tokens, rows, pass, k);
     }
-    const bool whole = whole_pieces(type, width, dy, lddy, dtable, ldt);
-    TYPED(type, constexpr int P = 16 / sizeof(T);
-          if (whole) embedding_sums<T, P>(st, s, b, tokens, rows, width, dy, lddy, scale, dtable, ldt, k);
-          else embedding_sums<T, 1>(st, s, b, tokens, rows, width, dy, lddy, scale, dtable, ldt, k));
+    TYPED(type, constexpr int P = 16 / sizeof(T); const int64_t lanes = cdiv(width, P); const unsigned sums = (unsigned)cdiv(s.pieces * lanes, 256);
+          piece_sum_kernel<T, P><<<sums + grid_of(cdiv(rows, 8), 4096), 256, 0, st>>>(b.keys[k], b.at[k], tokens, rows, sums, Div::by((unsigned)lanes), width, (const T*)dy, lddy,
+                                                                                    scale, (T*)dtable, ldt, b.part, b.part_ld, (const uint8_t*)b.marks);
+          join_kernel<T><<<(unsigned)s.pieces, 256, 0, st>>>(b.keys[k], tokens, rows, width, scale, (T*)dtable, ldt, b.part, b.part_ld));
     LAUNCHED("embedding_backward");
     return CCSM_OK;
 }
@@ -383,9 +391,12 @@ ccsm_status ccsm_train_act8_pack(int device, int type, int code, int64_t rows, i
     ccsm_status e = check_saved(ccsm_saved{codes, ldc, code, scales, lds}, type, width, "act8_pack: codes must be non-NULL");
     if (e != CCSM_OK) return e;
     ON_DEVICE(device);
-    const unsigned grid = grid_of(cdiv(rows * cdiv(width, 32), 8));
-    TYPED(type, if (code == CCSM_CODE_INT8) act8_pack_kernel<T, kCodeInt8><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)x, ldx, rows, width, (uint8_t*)codes, ldc, scales, lds);
-                else act8_pack_kernel<T, kCodeE4m3><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)x, ldx, rows, width, (uint8_t*)codes, ldc, scales, lds));
+    const int64_t per = 2 * cdiv(width, 32);
+    TYPED(type, in_ranges(rows, per, [&](int64_t r, int64_t n) {
+              auto* f = code == CCSM_CODE_INT8 ? &act8_pack_kernel<T, kCodeInt8> : &act8_pack_kernel<T, kCodeE4m3>;
+              f<<<(unsigned)cdiv(n * per, 256), 256, 0, (hipStream_t)stream>>>((const T*)x + r * ldx, ldx, (unsigned)(n * per), Div::by((unsigned)per), width, (uint8_t*)codes + r * ldc,
+                                                                              ldc, scales + r * lds, lds);
+          }));
     LAUNCHED("act8_pack");
     return CCSM_OK;
 }
@@ -399,7 +410,12 @@ ccsm_status ccsm_train_act8_unpack(int device, int type, int64_t rows, int32_t w
     if (e != CCSM_OK) return e;
     REFUSE(!y || ldy < width || off_by(y, size_of(type)), "act8_unpack: y must be non-NULL and aligned to its elements, its stride at least the width");
     ON_DEVICE(device);
-    TYPED(type, act8_unpack_kernel<T><<<grid_of(cdiv(rows * width, 256)), 256, 0, (hipStream_t)stream>>>(saved_of(*s), rows, width, (T*)y, ldy));
+    const int64_t per = cdiv(width, 16);
+    TYPED(type, in_ranges(rows, per, [&](int64_t r, int64_t n) {
+              auto* f = s->code == CCSM_CODE_INT8 ? &act8_unpack_kernel<T, kCodeInt8> : &act8_unpack_kernel<T, kCodeE4m3>;
+              f<<<(unsigned)cdiv(n * per, 256), 256, 0, (hipStream_t)stream>>>((const uint8_t*)s->data + r * s->ld, s->ld, s->scales + r * s->lds, s->lds, (unsigned)(n * per),
+                                                                              Div::by((unsigned)per), width, (T*)y + r * ldy, ldy);
+          }));
     LAUNCHED("act8_unpack");
     return CCSM_OK;
 }

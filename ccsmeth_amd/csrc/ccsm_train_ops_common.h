@@ -13,8 +13,46 @@ template <> struct TypeOf<float> { static constexpr int v = 0; };
 template <> struct TypeOf<f16> { static constexpr int v = 1; };
 template <> struct TypeOf<b16> { static constexpr int v = 2; };
 
-// N elements that are loaded and stored as one piece of up to 16 bytes
+// N elements that are loaded and stored as one aligned piece of up to 16 bytes
 template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+// ... as the widest pieces that the hardware has, with the alignment of one element (gfx950 takes any)
+template <typename T, int N> struct Loose { T v[N]; };
+
+// N elements of a row from p on, of which the first `left` exist (the others: zeros, not written)
+template <typename T, int N>
+__device__ __forceinline__ void load_row(const T* p, int left, float (&v)[N]) {
+    if (left >= N) {
+        const Loose<T, N> t = *reinterpret_cast<const Loose<T, N>*>(p);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = (float)t.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = k < left ? (float)p[k] : 0.f;
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* p, int left, const float (&v)[N]) {
+    if (left >= N) {
+        Loose<T, N> t;
+#pragma unroll
+        for (int k = 0; k < N; ++k) t.v[k] = (T)v[k];
+        *reinterpret_cast<Loose<T, N>*>(p) = t;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) if (k < left) p[k] = (T)v[k];
+    }
+}
+
+// x / d for x < 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1, s = the bits of d - 1 (Granlund and Montgomery's method for 31 bits)
+struct Div {
+    unsigned d, m, s;
+    static Div by(unsigned d) {
+        unsigned s = 0;
+        while ((1u << s) < d) ++s;
+        return Div{d, (unsigned)(((unsigned long long)1 << (31 + s)) / d + 1), s};
+    }
+    __device__ __forceinline__ unsigned of(unsigned x) const { return __umulhi(2 * x, m) >> s; }
+};
 
 enum { kActNone = 0, kActRelu, kActTanh, kActSigmoid, kActGelu, kActSilu };
 

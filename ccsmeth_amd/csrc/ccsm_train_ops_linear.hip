@@ -6,18 +6,20 @@
 
 namespace ccsm_ops {
 
+// the parts of a bias gradient in a fixed order: a workgroup takes eight columns, each lane every 32nd part; the 32 sums are added in order
 template <typename T>
-__global__ __launch_bounds__(256) void column_join_kernel(const float* part, long long parts, int N, T* out) {
-    // 256 threads = 32 columns x 8 slices of the parts; the slices are added in order
-    __shared__ float s[8][33];
-    const int c = threadIdx.x & 31, q = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
+__global__ __launch_bounds__(256) void column_join_kernel(const float* part, int parts, int N, T* out) {
+    __shared__ float s[32][9];
+    const int c = threadIdx.x & 7, q = threadIdx.x >> 3, n = blockIdx.x * 8 + c;
     float a = 0.f;
-    if (n < N)
-        for (long long p = q; p < parts; p += 8) a += part[p * N + n];
+    if (n < N) {
+#pragma unroll 8
+        for (int p = q; p < parts; p += 32) a += part[(long long)p * N + n];
+    }
     s[q][c] = a;
     __syncthreads();
     if (q == 0 && n < N) {
-        for (int k = 1; k < 8; ++k) a += s[k][c];
+        for (int k = 1; k < 32; ++k) a += s[k][c];
         out[n] = (T)a;
     }
 }

@@ -1,5 +1,6 @@
 // libccsm_train: the training operators' C-ABI (include/ccsm_train_ops.h).  Checks, workspace layout and launches; the kernels are in
 // ccsm_train_ops_linear.hip, ccsm_train_ops_embed.hip and ccsm_train_ops_act8.hip.
+#include <atomic>
 #include <string>
 #include <type_traits>
 
@@ -38,6 +39,7 @@ struct OnDevice {
     OnDevice on_device_(device);               \
     if (on_device_.err != hipSuccess) return hip_fail(on_device_.err, "hipSetDevice")
 
+constexpr int64_t kFewRows = 64;                   // up to here the few-rows kernel
 constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
 
 size_t size_of(int type) { return type == CCSM_TYPE_F32 ? 4 : 2; }
@@ -96,10 +98,9 @@ Staged staged(const Saved& s, int64_t rows, int64_t width, Scratch& ws, hipStrea
     const int64_t ld = (int64_t)up(width, 8), plane = rows * ld;
     uint16_t* out = ws.take<uint16_t>((size_t)planes * plane);
     if (!count) {
-        const bool whole = !off_by(s.data, 16) && s.ld % (16 / (int64_t)size_of(type)) == 0;
         const unsigned grid = grid_of(cdiv(plane / 8, 256), 1 << 16);
-        if (codes) stage_kernel<T, true><<<grid, 256, 0, st>>>(s, rows, (int)width, whole, out, ld, plane);
-        else stage_kernel<T, false><<<grid, 256, 0, st>>>(s, rows, (int)width, whole, out, ld, plane);
+        if (codes) stage_kernel<T, true><<<grid, 256, 0, st>>>(s, rows, (int)width, out, ld, plane);
+        else stage_kernel<T, false><<<grid, 256, 0, st>>>(s, rows, (int)width, out, ld, plane);
     }
     return Staged{Plane{out, ld, plane}, planes};
 }
@@ -108,9 +109,17 @@ template <typename T, bool TRP, bool TRQ, int B>
 hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
     constexpr int lds = 4 * 2 * B * 64;
     auto* f = &product_mfma_kernel<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
-    // (an attribute of the function on the current device; setting it again costs little, and there is no state to share between threads)
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    // an attribute of the function on each device: set once for each (setting it twice, from two threads, does no harm)
+    static std::atomic<uint64_t> known{0};
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return e;
+    const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+    if (!(known.load(std::memory_order_relaxed) & bit)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        known.fetch_or(bit, std::memory_order_relaxed);
+    }
     f<<<(unsigned)(a.tiles_i * a.tiles_j * a.splits), B == 256 ? 512 : 256, lds, st>>>(a);
     return hipGetLastError();
 }
@@ -140,12 +149,6 @@ hipError_t product(hipStream_t st, const Staged& p, const Staged& q, int64_t M, 
     product_join_kernel<T><<<grid_of(cdiv(M * cdiv(N, 4), 256), 1 << 16), 256, 0, st>>>(a.part, a.splits, M, (int)N, a.part_ld, ep);
     return hipGetLastError();
 }
-template <typename T>
-Epilogue epilogue(const void* bias, const void* residual, int64_t ldr, void* y, int64_t ldy, void* pre, int64_t ldp, int act) {
-    const size_t a = 4 * sizeof(T);
-    const bool vec = !off_by(y, a) && ldy % 4 == 0 && (!residual || (!off_by(residual, a) && ldr % 4 == 0)) && (!pre || (!off_by(pre, a) && ldp % 4 == 0));
-    return Epilogue{bias, residual, ldr, y, ldy, pre, ldp, act, vec};
-}
 #define TRY(x, what) do { hipError_t e_ = (x); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
 
 ccsm_status check_linear(const ccsm_linear* p) {
@@ -161,8 +164,15 @@ ccsm_status check_linear(const ccsm_linear* p) {
 }
 template <typename T>
 ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bool count) {
+    const Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
+    if (p->rows <= kFewRows) {
+        if (count) return CCSM_OK;
+        auto* f = p->rows <= 16 ? &few_rows_kernel<T, 1> : p->rows <= 32 ? &few_rows_kernel<T, 2> : &few_rows_kernel<T, 4>;
+        f<<<(unsigned)cdiv(p->outer, 16), 512, 0, st>>>((const T*)p->x, p->ldx, (const T*)p->w, p->ldw, (int)p->rows, p->outer, p->inner, ep);
+        LAUNCHED("linear_forward");
+        return CCSM_OK;
+    }
     const Staged x = staged<T>(plain(p->x, p->ldx), p->rows, p->inner, ws, st, count), w = staged<T>(plain(p->w, p->ldw), p->outer, p->inner, ws, st, count);
-    const Epilogue ep = epilogue<T>(p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation);
     TRY((product<T, false, false>(st, x, w, p->rows, p->outer, p->inner, ep, ws, count)), "linear_forward");
     return CCSM_OK;
 }
@@ -211,20 +221,18 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
     if (products && !direct) d = Staged{Plane{ws.take<uint16_t>((size_t)planes * plane), ldd, plane}, planes};
     float* part = p->dbias ? ws.take<float>((size_t)parts * N) : nullptr;
     if (!count && (part || (products && !direct))) {
-        const int64_t n = 16 / (int64_t)sizeof(T);
-        const bool whole = !off_by(p->dy, 16) && p->lddy % n == 0, whole_z = !none && !off_by(p->preact.data, 16) && p->preact.ld % n == 0;
-        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 512)), 256, 0, st>>>(dy, whole, none ? dy : saved_of(p->preact), whole_z, p->activation, M, N,
+        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 256)), 256, 0, st>>>(dy, none ? dy : saved_of(p->preact), p->activation, M, N,
                                                                                      products && !direct ? const_cast<void*>(d.p.base) : nullptr, ldd, plane, part);
         if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 8), 256, 0, st>>>(part, (int)parts, N, (T*)p->dbias);
         LAUNCHED("linear_backward");
     }
     if (p->dx) {
         const Staged w = staged<T>(plain(p->w, p->ldw), N, K, ws, st, count);
-        TRY((product<T, false, true>(st, d, w, M, K, N, epilogue<T>(nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone), ws, count)), "linear_backward: dx");
+        TRY((product<T, false, true>(st, d, w, M, K, N, Epilogue{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, ws, count)), "linear_backward: dx");
     }
     if (p->dw) {
         const Staged x = staged<T>(saved_of(p->x), M, K, ws, st, count);
-        TRY((product<T, true, true>(st, d, x, N, K, M, epilogue<T>(nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone), ws, count)), "linear_backward: dw");
+        TRY((product<T, true, true>(st, d, x, N, K, M, Epilogue{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone}, ws, count)), "linear_backward: dw");
     }
     return CCSM_OK;
 }

@@ -133,6 +133,23 @@ __device__ __forceinline__ float slope_(float z, int act) {
     }
 }
 
+template <bool FAST, int N>
+__device__ __forceinline__ void slope_all(float (&z)[N], int act) {
+    switch (act) {
+#define CCSM_SLOPES(A)                                               \
+    case A:                                                          \
+        _Pragma("unroll") for (int k = 0; k < N; ++k) z[k] = slope_<FAST>(z[k], A); \
+        break;
+        CCSM_SLOPES(kActRelu)
+        CCSM_SLOPES(kActTanh)
+        CCSM_SLOPES(kActSigmoid)
+        CCSM_SLOPES(kActGelu)
+        CCSM_SLOPES(kActSilu)
+#undef CCSM_SLOPES
+        default: break;
+    }
+}
+
 // ---- 8-bit codes (ccsm_code8) ---------------------------------------------------------------------------------------
 enum { kCodeNone = 0, kCodeInt8 = 1, kCodeE4m3 = 2 };
 

@@ -50,7 +50,6 @@ template <> struct Mfma<b16> {
 // what a product's results go through: z = acc + bias; y = act(z) + residual.  With `part`, the accumulators go there instead (split k)
 struct Epilogue {
     const void* bias; const void* residual; long long ldr; void* y; long long ldy; void* pre; long long ldp; int act;
-    int vec;                  // every row of y, pre and residual starts 4-element aligned
 };
 struct Plane { const void* base; long long ld; long long plane; };      // elements of 16 bits; `plane`: from one plane to the next
 struct ProductArgs {
@@ -62,59 +61,30 @@ struct ProductArgs {
     Epilogue ep;
 };
 
-// N results (i, j .. j + N - 1), of which the first `left` exist
+// N results (i, j .. j + N - 1), of which the first `left` exist; bias and r = the residual's values of them
 template <typename T, int N>
-__device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, int left, float (&z)[N]) {
+__device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, int left, float (&z)[N], const float (&bias)[N], const Loose<T, N>& r) {
     constexpr bool fast = sizeof(T) == 2;
-    typedef Vec<T, 4> V;
-    const bool whole = e.vec && left >= N;
     if (e.bias) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) if (k < left) z[k] += (float)((const T*)e.bias)[j + k];
+        for (int k = 0; k < N; ++k) z[k] += bias[k];
     }
-    if (e.pre) {
-        T* o = (T*)e.pre + i * e.ldp + j;
-        if (whole) {
-#pragma unroll
-            for (int q = 0; q < N; q += 4) {
-                V v;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v.v[k] = (T)z[q + k];
-                *(V*)(o + q) = v;
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k) if (k < left) o[k] = (T)z[k];
-        }
-    }
+    if (e.pre) store_row<T, N>((T*)e.pre + i * e.ldp + j, left, z);
     act_all<fast, N>(z, e.act);
     if (e.residual) {
-        const T* o = (const T*)e.residual + i * e.ldr + j;
-        if (whole) {
 #pragma unroll
-            for (int q = 0; q < N; q += 4) {
-                const V v = *(const V*)(o + q);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) z[q + k] += (float)v.v[k];
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k) if (k < left) z[k] += (float)o[k];
-        }
+        for (int k = 0; k < N; ++k) z[k] += (float)r.v[k];
     }
-    T* o = (T*)e.y + i * e.ldy + j;
-    if (whole) {
+    store_row<T, N>((T*)e.y + i * e.ldy + j, left, z);
+}
+// N elements as they are (the ones behind `left`: zeros)
+template <typename T, int N>
+__device__ __forceinline__ Loose<T, N> raw_row(const T* p, int left) {
+    if (left >= N) return *reinterpret_cast<const Loose<T, N>*>(p);
+    Loose<T, N> t;
 #pragma unroll
-        for (int q = 0; q < N; q += 4) {
-            V v;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v.v[k] = (T)z[q + k];
-            *(V*)(o + q) = v;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) if (k < left) o[k] = (T)z[k];
-    }
+    for (int k = 0; k < N; ++k) t.v[k] = k < left ? p[k] : (T)0.f;
+    return t;
 }
 
 // One operand's side of the tile: requests and fragment reads.  B: the tile's extent, W: a wave's, NW waves in the workgroup.
@@ -260,12 +230,27 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
         body(std::integral_constant<int, 2>());
         body(std::integral_constant<int, 3>());
     }
-    // The results leave through the wave's own quarter of LDS, 32 rows of i at a time (rows 16 bytes longer than they need: the lanes' writes fall on
-    // different banks): a row's results then leave in pieces of eight neighbours
+    // The results leave through the wave's own part of LDS, 32 rows of i at a time (rows 16 bytes longer than they need: the lanes' writes fall on
+    // different banks), and from there in pieces of eight neighbours of a row.  A lane's column does not change, so its bias is loaded once; a
+    // round's residual is loaded a round ahead (one load at a time, 128 loads one behind the other, took 170 of 640 us of a 16384 x 4096 x 4096
+    // product).
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // no request may still write LDS
-    constexpr int WJT = BJ / WJ, kRow = WJT + 4, kPer = WJT / 8;
-    static_assert(32 * kRow * 4 * NW <= 4 * (SP::kStage + SQ::kStage), "the waves' rows fit into the stages");
+    constexpr int WJT = BJ / WJ, kRow = WJT + 4, kPer = WJT / 8, kIt = 32 * kPer / 64, kRows = 64 / kPer;
+    static_assert(32 * kRow * 4 * NW <= 4 * (SP::kStage + SQ::kStage) && 64 % kPer == 0, "the waves' rows fit into the stages");
     float* out = reinterpret_cast<float*>(ops_smem) + wave * 32 * kRow;
+    const int c = lane % kPer * 8, j = j0 + wj * WJT + c, left_j = a.N - j, iw = i0 + wi * (BI / WI) + lane / kPer;
+    const bool res = !a.part && a.ep.residual && left_j > 0;
+    float bias[8];
+    if (!a.part && a.ep.bias && left_j > 0) load_row<T, 8>((const T*)a.ep.bias + j, left_j, bias);
+    Loose<T, 8> r[2][kIt];
+    auto residual = [&](int h, Loose<T, 8> (&o)[kIt]) {
+#pragma unroll
+        for (int q = 0; q < kIt; ++q) {
+            const int i = iw + 32 * h + q * kRows;
+            if (i < a.M) o[q] = raw_row<T, 8>((const T*)a.ep.residual + (long long)i * a.ep.ldr + j, left_j);
+        }
+    };
+    if (res) residual(0, r[0]);
 #pragma unroll 1
     for (int h = 0; h < FI / 2; ++h) {
 #pragma unroll
@@ -274,25 +259,30 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
 #pragma unroll
             for (int q = 0; q < FJ; ++q) *(f32x4*)(out + (16 * (p & 1) + (lane & 15)) * kRow + 16 * q + 4 * (lane >> 4)) = acc[p][q];
         }
-        const int ih = i0 + wi * (BI / WI) + 32 * h, jw = j0 + wj * WJT;
-#pragma unroll 1
-        for (int e = lane; e < 32 * kPer; e += 64) {
-            const int i = ih + e / kPer, c = e % kPer * 8, j = jw + c;
-            if (i >= a.M || j >= a.N) continue;
-            const f32x4 u = *(const f32x4*)(out + e / kPer * kRow + c), v = *(const f32x4*)(out + e / kPer * kRow + c + 4);
-            if (a.part) {
-                float* o = a.part + ((long long)split * a.M + i) * a.part_ld + j;
-                *(f32x4*)o = u;
-                if (j + 4 < a.N) *(f32x4*)(o + 4) = v;
-            } else {
-                float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-                finish<T, 8>(a.ep, i, j, a.N - j, z);
+        if (res && h + 1 < FI / 2) residual(h + 1, r[1]);
+        if (left_j > 0) {
+#pragma unroll
+            for (int q = 0; q < kIt; ++q) {
+                const int i = iw + 32 * h + q * kRows;
+                const float* o = out + (lane / kPer + q * kRows) * kRow + c;
+                const f32x4 u = *(const f32x4*)o, v = *(const f32x4*)(o + 4);
+                if (i >= a.M) continue;
+                if (a.part) {
+                    float* g = a.part + ((long long)split * a.M + i) * a.part_ld + j;
+                    *(f32x4*)g = u;
+                    if (left_j > 4) *(f32x4*)(g + 4) = v;
+                } else {
+                    float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                    finish<T, 8>(a.ep, i, j, left_j, z, bias, r[0][q]);
+                }
             }
         }
+#pragma unroll
+        for (int q = 0; q < kIt; ++q) r[0][q] = r[1][q];
     }
 }
 
-// the splits' parts in order, and the epilogue
+// the splits' parts in order, and the epilogue; a lane takes four neighbours
 template <typename T>
 __global__ __launch_bounds__(256) void product_join_kernel(const float* part, int splits, long long M, int N, long long ld, Epilogue ep) {
     const int nj = (N + 3) / 4;
@@ -300,9 +290,13 @@ __global__ __launch_bounds__(256) void product_join_kernel(const float* part, in
         const long long i = x / nj;
         const int j = (int)(x % nj) * 4;
         f32x4 v = *(const f32x4*)(part + i * ld + j);
+#pragma unroll 8
         for (int s = 1; s < splits; ++s) v += *(const f32x4*)(part + ((long long)s * M + i) * ld + j);
-        float z[4] = {v[0], v[1], v[2], v[3]};
-        finish<T, 4>(ep, i, j, N - j, z);
+        float z[4] = {v[0], v[1], v[2], v[3]}, bias[4];
+        Loose<T, 4> r;
+        if (ep.bias) load_row<T, 4>((const T*)ep.bias + j, N - j, bias);
+        if (ep.residual) r = raw_row<T, 4>((const T*)ep.residual + i * ep.ldr + j, N - j);
+        finish<T, 4>(ep, i, j, N - j, z, bias, r);
     }
 }
 
@@ -348,82 +342,168 @@ template <int N> struct Planes<b16, N> {
     }
 };
 
-// eight values of row r from column c on, zeros beyond the width; whole: aligned pieces can be loaded at once
+// eight values of row r from column c on, zeros beyond the width
 template <typename T>
-__device__ __forceinline__ void load8(const Saved& s, long long r, int c, int width, bool whole, float (&v)[8]) {
-    if (s.code != kCodeNone) {                    // (a code row covers whole blocks of 32, 16-byte aligned)
-        const uint2 u = *(const uint2*)((const uint8_t*)s.data + r * s.ld + c);
-        const float k = pow2_of_byte(s.scales[r * s.lds + (c >> 5)]);
-        float a[4], b[4];
-        if (s.code == kCodeInt8) { decode4<kCodeInt8>(u.x, k, a); decode4<kCodeInt8>(u.y, k, b); }
-        else { decode4<kCodeE4m3>(u.x, k, a); decode4<kCodeE4m3>(u.y, k, b); }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+__device__ __forceinline__ void load8(const Saved& s, long long r, int c, int width, float (&v)[8]) {
+    if (s.code == kCodeNone) {
+        load_row<T, 8>((const T*)s.data + r * s.ld + c, width - c, v);
         return;
     }
-    const T* p = (const T*)s.data + r * s.ld + c;
-    if (whole && c + 8 <= width) {
-        constexpr int P = 16 / sizeof(T);
+    const uint2 u = *(const uint2*)((const uint8_t*)s.data + r * s.ld + c);      // (a code row covers whole blocks of 32, 16-byte aligned)
+    const float k = pow2_of_byte(s.scales[r * s.lds + (c >> 5)]);
+    float a[4], b[4];
+    if (s.code == kCodeInt8) { decode4<kCodeInt8>(u.x, k, a); decode4<kCodeInt8>(u.y, k, b); }
+    else { decode4<kCodeE4m3>(u.x, k, a); decode4<kCodeE4m3>(u.y, k, b); }
 #pragma unroll
-        for (int q = 0; q < 8 / P; ++q) {
-            const Vec<T, P> t = *(const Vec<T, P>*)(p + q * P);
-#pragma unroll
-            for (int k = 0; k < P; ++k) v[q * P + k] = (float)t.v[k];
-        }
-        return;
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = c + q < width ? (float)p[q] : 0.f;
+    for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
 }
 
 // a kept matrix as planes of 16-bit elements with rows of whole 16-byte pieces (zeros behind the width).  ONE: one plane whatever the type (8-bit
 // codes, whose values bf16 holds exactly)
 template <typename T, bool ONE>
-__global__ __launch_bounds__(256) void stage_kernel(Saved s, long long rows, int width, bool whole, void* out, long long ld, long long plane) {
+__global__ __launch_bounds__(256) void stage_kernel(Saved s, long long rows, int width, void* out, long long ld, long long plane) {
     const int n = (int)(ld / 8);
     for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < rows * n; x += (long long)gridDim.x * 256) {
         const long long r = x / n;
         const int c = (int)(x % n) * 8;
         float v[8];
-        load8<T>(s, r, c, width, whole, v);
+        load8<T>(s, r, c, width, v);
         typedef typename std::conditional<ONE && sizeof(T) == 4, b16, T>::type O;
         Planes<O, 8>::put(v, out, plane, r * ld + c);
     }
 }
 
-// d = dy act'(z) into planes (16-bit types: one, rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 512 columns: 64 lanes of eight
-// columns, four rows at a time.
+// d = dy act'(z) into planes (16-bit types: one, rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 256 columns: 32 lanes of eight
+// columns, eight rows at a time, four rows of a lane in flight.
 // Rounding d: 16-bit products take 16-bit operands, and this rounding (half a step per factor, independent of each other) moves a gradient by
 // no more than the rounding of the gradient itself does.  The bias gradient takes d before it.
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(Saved dy, bool whole_dy, Saved z, bool whole_z, int act, long long M, int N, void* d, long long ldd, long long plane, float* part) {
+__global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, long long M, int N, void* d, long long ldd, long long plane, float* part) {
     constexpr bool fast = sizeof(T) == 2;
-    __shared__ float sum[4][512];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 512 + lane * 8;
-    const long long m0 = (long long)blockIdx.x * 32;
+    __shared__ float sum[8][256];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * 256 + lane * 8;
+    const long long m0 = (long long)blockIdx.x * 32 + w;
     float acc[8] = {};
-    if (c < N)
-        for (int r = w; r < 32 && m0 + r < M; r += 4) {
-            float v[8];
-            load8<T>(dy, m0 + r, c, N, whole_dy, v);
-            if (act != kActNone) {
-                float u[8];
-                load8<T>(z, m0 + r, c, N, whole_z, u);
+    if (c < N) {
+        float v[4][8], u[4][8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = c + k < N ? v[k] * slope_<fast>(u[k], act) : 0.f;
-            }
-            if (d) Planes<T, 8>::put(v, d, plane, (m0 + r) * ldd + c);
+        for (int q = 0; q < 4; ++q)
+            if (m0 + 8 * q < M) load8<T>(dy, m0 + 8 * q, c, N, v[q]);
+        if (act != kActNone) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] += v[k];
+            for (int q = 0; q < 4; ++q)
+                if (m0 + 8 * q < M) load8<T>(z, m0 + 8 * q, c, N, u[q]);
         }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (m0 + 8 * q >= M) break;
+            if (act != kActNone) {
+                slope_all<fast, 8>(u[q], act);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[q][k] = c + k < N ? v[q][k] * u[q][k] : 0.f;
+            }
+            if (d) Planes<T, 8>::put(v[q], d, plane, (m0 + 8 * q) * ldd + c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += v[q][k];
+        }
+    }
     if (!part) return;
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[w][lane * 8 + k] = acc[k];
     __syncthreads();
-    for (int k = threadIdx.x; k < 512; k += 256) {
-        const int n = blockIdx.y * 512 + k;
-        if (n < N) part[(long long)blockIdx.x * N + n] = (sum[0][k] + sum[1][k]) + (sum[2][k] + sum[3][k]);
+    const int n = blockIdx.y * 256 + threadIdx.x;
+    if (n >= N) return;
+    float a = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a += sum[k][threadIdx.x];
+    part[(long long)blockIdx.x * N + n] = a;
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------
+// y = act(x w^T + bias) + residual for up to 16 MT rows of x: bound by reading w once.  A workgroup takes 16 rows of w, its eight waves every eighth
+// 32 columns of them, eight pieces in flight; a piece goes from memory straight into the matrix instruction's operand (lane = row, 8 columns; any
+// alignment), x likewise (out of the caches).  The waves' sums are added in order through LDS.  fp32: the three bf16 parts of each operand are made
+// in registers.  At 1 x 512 x 768 bf16 the tile kernel took 9.8 us: four steps through four LDS stages by six of 256 CUs.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void few_rows_kernel(const T* x, long long ldx, const T* w, long long ldw, int M, int N, int K, Epilogue ep) {
+    typedef typename std::conditional<sizeof(T) == 4, b16, T>::type E;
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1, U = 4;
+    __shared__ f32x4 sum[8][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n0 = blockIdx.x * 16, n = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
+    const T* wr = w + n * ldw;
+    const T* xr[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = 16 * t + (lane & 15);
+        xr[t] = x + (m < M ? m : M - 1) * ldx;
     }
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto pieces = [](const Loose<T, 8>& v, s16x8 (&p)[NP]) {
+        if constexpr (NP == 1) p[0] = __builtin_bit_cast(s16x8, v);
+        else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                b16 o[3];
+                three(v.v[k], o);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) p[q][k] = __builtin_bit_cast(short, o[q]);
+            }
+        }
+    };
+    auto multiply = [&](const Loose<T, 8>& wv, const Loose<T, 8> (&xv)[MT]) {
+        s16x8 a[NP], b[NP];
+        pieces(wv, a);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            pieces(xv[t], b);
+            if constexpr (NP == 3) {
+                acc[t] = Mfma<E>::run(a[2], b[0], acc[t]);
+                acc[t] = Mfma<E>::run(a[0], b[2], acc[t]);
+                acc[t] = Mfma<E>::run(a[1], b[1], acc[t]);
+                acc[t] = Mfma<E>::run(a[1], b[0], acc[t]);
+                acc[t] = Mfma<E>::run(a[0], b[1], acc[t]);
+            }
+            acc[t] = Mfma<E>::run(a[0], b[0], acc[t]);
+        }
+    };
+    int k = wave * 32 + 8 * (lane >> 4);
+    const int whole = K & ~255;                                   // all eight waves have whole pieces up to here
+    int k0 = 0;
+    for (; k0 + 256 * U <= whole; k0 += 256 * U, k += 256 * U) {
+        Loose<T, 8> wv[U], xv[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) wv[u] = *reinterpret_cast<const Loose<T, 8>*>(wr + k + 256 * u);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xv[u][t] = *reinterpret_cast<const Loose<T, 8>*>(xr[t] + k + 256 * u);
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(wv[u], xv[u]);
+    }
+    for (; k0 < K; k0 += 256, k += 256) {
+        Loose<T, 8> wv, xv[MT];
+        wv = raw_row<T, 8>(wr + k, K - k);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xv[t] = raw_row<T, 8>(xr[t] + k, K - k);
+        multiply(wv, xv);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sum[wave][t][lane] = acc[t];
+    __syncthreads();
+    if ((int)threadIdx.x >= 64 * MT) return;
+    const int t = wave, m = 16 * t + (lane & 15), j = n0 + 4 * (lane >> 4);
+    if (m >= M || j >= N) return;
+    f32x4 v = sum[0][t][lane];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) v += sum[q][t][lane];
+    float z[4] = {v[0], v[1], v[2], v[3]}, bias[4];
+    Loose<T, 4> r;
+    if (ep.bias) load_row<T, 4>((const T*)ep.bias + j, N - j, bias);
+    if (ep.residual) r = raw_row<T, 4>((const T*)ep.residual + m * ep.ldr + j, N - j);
+    finish<T, 4>(ep, m, j, N - j, z, bias, r);
 }
 
 }  // namespace ccsm_ops

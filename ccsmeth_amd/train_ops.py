@@ -14,8 +14,8 @@ current stream of the tensors' device) and nothing waits for the GPU; calls can 
 they are, other layouts are copied.  There is no autograd: gradients are calls, as in Trainer.forward_backward, and inputs that require a
 gradient are refused while grad mode is on.  There is no CPU path.
 """
-import contextlib
 import ctypes as C
+import struct
 
 from . import _lib
 from . import train as _train
@@ -43,6 +43,12 @@ class LinearGrad(C.Structure):
                 ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64), ("dbias", C.c_void_p)]
 
 
+# the two structures as bytes (the header's layout): one pack call is a third of what filling a ctypes structure costs per call
+_LINEAR = struct.Struct("@iiqiiPqPqPPqPqPq")
+_GRAD = struct.Struct("@iiqiiPqPqiPqPqPqiPqPqPqP")
+assert _LINEAR.size == C.sizeof(Linear) and _GRAD.size == C.sizeof(LinearGrad)
+_NONE = (0, 0, 0, 0, 0)
+
 _ops = None
 
 
@@ -53,12 +59,12 @@ def load():
     lib = _train.load()
     vp, ci, cl, cf, cs = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
     lib.ccsm_train_ops_last_error.restype = C.c_char_p
-    lib.ccsm_train_linear_workspace.argtypes = [C.POINTER(Linear)]
+    lib.ccsm_train_linear_workspace.argtypes = [vp]
     lib.ccsm_train_linear_workspace.restype = cs
-    lib.ccsm_train_linear_forward.argtypes = [ci, C.POINTER(Linear), vp, cs, vp]
-    lib.ccsm_train_linear_backward_workspace.argtypes = [C.POINTER(LinearGrad)]
+    lib.ccsm_train_linear_forward.argtypes = [ci, vp, vp, cs, vp]
+    lib.ccsm_train_linear_backward_workspace.argtypes = [vp]
     lib.ccsm_train_linear_backward_workspace.restype = cs
-    lib.ccsm_train_linear_backward.argtypes = [ci, C.POINTER(LinearGrad), vp, cs, vp]
+    lib.ccsm_train_linear_backward.argtypes = [ci, vp, vp, cs, vp]
     lib.ccsm_train_embedding_forward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp]
     lib.ccsm_train_embedding_backward_workspace.argtypes = [cl, cl, C.c_int32]
     lib.ccsm_train_embedding_backward_workspace.restype = cs
@@ -120,46 +126,35 @@ def _rows(t):
     return t, (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
 
 
-class _Run:
-    """The call's stream: what it allocates belongs to that stream, and what it was given is kept for it until its work is done."""
+def _elsewhere(call, stream, device, given, *args, **kw):
+    """call(*args, **kw) with `stream` as the current stream: what it allocates belongs to that stream, and the tensors that it was given are kept for it until
+    its work is done."""
+    torch = _torch
+    if not isinstance(stream, torch.cuda.Stream):
+        raise TypeError("stream must be a torch.cuda.Stream")
+    if stream.device != device:
+        raise ValueError("stream belongs to %s, the tensors to %s" % (stream.device, device))
+    with torch.cuda.stream(stream):
+        out = call(*args, **kw)
+        for t in given:
+            if isinstance(t, Checkpoint8):
+                t.codes.record_stream(stream)
+                t.scales.record_stream(stream)
+            elif t is not None:
+                t.record_stream(stream)
+    return out
 
-    __slots__ = ("device", "stream", "_with", "_other")
 
-    def __init__(self, device, stream):
-        torch = _torch
-        now = torch.cuda.current_stream(device)
-        if stream is None:
-            stream = now
-        elif not isinstance(stream, torch.cuda.Stream):
-            raise TypeError("stream must be a torch.cuda.Stream")
-        elif stream.device != device:
-            raise ValueError("stream belongs to %s, the tensors to %s" % (stream.device, device))
-        self.device, self.stream = device, stream
-        self._other = stream.cuda_stream != now.cuda_stream
+def _raw_stream(device):
+    return _torch._C._cuda_getCurrentRawStream(device.index)
 
-    def __enter__(self):
-        self._with = _torch.cuda.stream(self.stream) if self._other else contextlib.nullcontext()
-        self._with.__enter__()
-        return self
 
-    def __exit__(self, *a):
-        return self._with.__exit__(*a)
-
-    def keep(self, *tensors):
-        if self._other:
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(self.stream)
-
-    def empty(self, shape, dtype):
-        return _torch.empty(shape, dtype=dtype, device=self.device)
-
-    def scratch(self, n):
-        return _torch.empty(n, dtype=_torch.uint8, device=self.device) if n else None
+def _scratch(n, device):
+    return _torch.empty(n, dtype=_torch.uint8, device=device) if n else None
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _activation(name):
@@ -210,7 +205,7 @@ class Checkpoint8:
         return self.codes.numel() + self.scales.numel()
 
     def _saved(self):
-        return Saved(self.codes.data_ptr(), self.codes.shape[1], CODES[self.code], self.scales.data_ptr(), self.scales.shape[1])
+        return self.codes.data_ptr(), self.codes.shape[1], CODES[self.code], self.scales.data_ptr(), self.scales.shape[1]
 
     def values(self, dtype=None, *, out=None, stream=None):
         """The values that the codes stand for, as a tensor of `dtype` (default: the type it was made of, which holds them exactly)."""
@@ -219,12 +214,13 @@ class Checkpoint8:
             raise ValueError("dtype must be float32, float16 or bfloat16, not %s" % dtype)
         lib = load()
         _on_gpu(self.codes, "the checkpoint")
-        with _Run(self.device, stream) as run:
-            y = run.empty(self.shape, dtype) if out is None else _out(out, self.shape, dtype, self.device, "out")
-            run.keep(self.codes, self.scales, out)
-            y2, ldy = _rows(y)
-            s = self._saved()
-            _check(lib.ccsm_train_act8_unpack(run.device.index, _TYPE[dtype], y2.shape[0], y2.shape[1], C.byref(s), y2.data_ptr(), ldy, run.stream.cuda_stream))
+        dev = self.device
+        if stream is not None:
+            return _elsewhere(self.values, stream, dev, (self, out), dtype, out=out)
+        y = _torch.empty(self.shape, dtype=dtype, device=dev) if out is None else _out(out, self.shape, dtype, dev, "out")
+        y2, ldy = _rows(y)
+        s = Saved(*self._saved())
+        _check(lib.ccsm_train_act8_unpack(dev.index, _TYPE[dtype], y2.shape[0], y2.shape[1], C.byref(s), y2.data_ptr(), ldy, _raw_stream(dev)))
         return y
 
 
@@ -239,15 +235,16 @@ def checkpoint8(x, code="int8", *, stream=None):
     _on_gpu(x, "x")
     if x.dim() == 0 or x.shape[-1] < 1:
         raise ValueError("x must have at least one column")
-    with _Run(x.device, stream) as run:
-        x2, ldx = _rows(x)
-        rows, width = x2.shape
-        blocks = -(-width // 32)
-        codes = run.empty((rows, 32 * blocks), torch.uint8)
-        scales = run.empty((rows, blocks), torch.uint8)
-        run.keep(x)
-        _check(lib.ccsm_train_act8_pack(run.device.index, _TYPE[x.dtype], CODES[code], rows, width, x2.data_ptr(), ldx, codes.data_ptr(), 32 * blocks,
-                                        scales.data_ptr(), blocks, run.stream.cuda_stream))
+    dev = x.device
+    if stream is not None:
+        return _elsewhere(checkpoint8, stream, dev, (x,), x, code)
+    x2, ldx = _rows(x)
+    rows, width = x2.shape
+    blocks = -(-width // 32)
+    codes = torch.empty((rows, 32 * blocks), dtype=torch.uint8, device=dev)
+    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=dev)
+    _check(lib.ccsm_train_act8_pack(dev.index, _TYPE[x.dtype], CODES[code], rows, width, x2.data_ptr(), ldx, codes.data_ptr(), 32 * blocks, scales.data_ptr(), blocks,
+                                    _raw_stream(dev)))
     return Checkpoint8(codes, scales, x.shape, x.dtype, code)
 
 
@@ -270,19 +267,20 @@ def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=F
         raise ValueError("bias must be (%d,)" % outer)
     if residual is not None and _tensor(residual, "residual", t, dev).shape != shape:
         raise ValueError("residual must be %s" % (tuple(shape),))
-    with _Run(dev, stream) as run:
-        y = run.empty(shape, t) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
-        z = run.empty(shape, t) if keep_preact else None
-        run.keep(x, weight, bias, residual, out)
-        x2, ldx = _rows(x)
-        w2, ldw = _rows(weight)
-        b1 = None if bias is None else bias.contiguous()
-        y2, ldy = _rows(y)
-        r2, ldr = (None, 0) if residual is None else _rows(residual)
-        p = Linear(_TYPE[t], act, x2.shape[0], inner, outer, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b1), _ptr(r2), ldr, y2.data_ptr(), ldy, _ptr(z), outer)
-        need = lib.ccsm_train_linear_workspace(C.byref(p))
-        ws = run.scratch(need)
-        _check(lib.ccsm_train_linear_forward(dev.index, C.byref(p), _ptr(ws), need, run.stream.cuda_stream))
+    if stream is not None:
+        return _elsewhere(linear, stream, dev, (x, weight, bias, residual, out), x, weight, bias, residual, activation, keep_preact, out=out)
+    empty = _torch.empty
+    y = empty(shape, dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
+    z = empty(shape, dtype=t, device=dev) if keep_preact else None
+    x2, ldx = _rows(x)
+    w2, ldw = _rows(weight)
+    b1 = None if bias is None else bias.contiguous()
+    y2, ldy = _rows(y)
+    r2, ldr = (None, 0) if residual is None else _rows(residual)
+    p = _LINEAR.pack(_TYPE[t], act, x2.shape[0], inner, outer, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b1), _ptr(r2), ldr, y2.data_ptr(), ldy, _ptr(z), outer)
+    need = lib.ccsm_train_linear_workspace(p)
+    ws = _scratch(need, dev)
+    _check(lib.ccsm_train_linear_forward(dev.index, p, _ptr(ws), need, _raw_stream(dev)))
     return (y, z) if keep_preact else y
 
 
@@ -305,7 +303,7 @@ def linear_backward(dy, x, weight, preact=None, activation="none", *, need_dx=Tr
 
     def saved(v, cols, name):
         if v is None:
-            return Saved(), ()
+            return _NONE, None
         if tuple(v.shape) != tuple(dy.shape[:-1]) + (cols,):
             raise ValueError("%s must be %s, not %s" % (name, tuple(dy.shape[:-1]) + (cols,), tuple(v.shape)))
         if isinstance(v, Checkpoint8):
@@ -313,25 +311,26 @@ def linear_backward(dy, x, weight, preact=None, activation="none", *, need_dx=Tr
                 raise ValueError("%s is on %s, not on %s" % (name, v.device, dev))
             if v.dtype is not t:
                 raise ValueError("%s was made of %s, the call's type is %s" % (name, v.dtype, t))
-            return v._saved(), (v.codes, v.scales)
+            return v._saved(), None
         v2, ld = _rows(_tensor(v, name, t, dev))
-        return Saved(v2.data_ptr(), ld, 0, None, 0), (v, v2)
+        return (v2.data_ptr(), ld, 0, 0, 0), v2
 
     if need_dw and x is None:
         raise ValueError("x is needed for dw")
-    with _Run(dev, stream) as run:
-        xs, keep_x = saved(x if need_dw else None, inner, "x")
-        zs, keep_z = saved(preact if act else None, outer, "preact")
-        dx = run.empty(dy.shape[:-1] + (inner,), t) if need_dx else None
-        dw = run.empty((outer, inner), t) if need_dw else None
-        db = run.empty((outer,), t) if need_db else None
-        run.keep(dy, weight, *keep_x, *keep_z)
-        d2, ldd = _rows(dy)
-        w2, ldw = _rows(weight)
-        p = LinearGrad(_TYPE[t], act, d2.shape[0], inner, outer, d2.data_ptr(), ldd, xs, w2.data_ptr(), ldw, zs, _ptr(dx), inner, _ptr(dw), inner, _ptr(db))
-        need = lib.ccsm_train_linear_backward_workspace(C.byref(p))
-        ws = run.scratch(need)
-        _check(lib.ccsm_train_linear_backward(dev.index, C.byref(p), _ptr(ws), need, run.stream.cuda_stream))
+    if stream is not None:
+        return _elsewhere(linear_backward, stream, dev, (dy, x, weight, preact), dy, x, weight, preact, activation, need_dx=need_dx, need_dw=need_dw, need_db=need_db)
+    empty = _torch.empty
+    xs, _x = saved(x if need_dw else None, inner, "x")
+    zs, _z = saved(preact if act else None, outer, "preact")
+    dx = empty(dy.shape[:-1] + (inner,), dtype=t, device=dev) if need_dx else None
+    dw = empty((outer, inner), dtype=t, device=dev) if need_dw else None
+    db = empty((outer,), dtype=t, device=dev) if need_db else None
+    d2, ldd = _rows(dy)
+    w2, ldw = _rows(weight)
+    p = _GRAD.pack(_TYPE[t], act, d2.shape[0], inner, outer, d2.data_ptr(), ldd, *xs, w2.data_ptr(), ldw, *zs, _ptr(dx), inner, _ptr(dw), inner, _ptr(db))
+    need = lib.ccsm_train_linear_backward_workspace(p)
+    ws = _scratch(need, dev)
+    _check(lib.ccsm_train_linear_backward(dev.index, p, _ptr(ws), need, _raw_stream(dev)))
     return dx, dw, db
 
 
@@ -352,15 +351,15 @@ def embedding(ids, table, scale=1.0, *, out=None, stream=None):
     _on_gpu(table, "table")
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError("table must be (rows, width)")
-    with _Run(dev, stream) as run:
-        i = _ids(ids, dev)
-        shape = ids.shape + (table.shape[1],)
-        y = run.empty(shape, t) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
-        run.keep(ids, table, out)
-        t2, ldt = _rows(table)
-        y2, ldy = _rows(y)
-        _check(lib.ccsm_train_embedding_forward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), t2.shape[0], t2.shape[1], t2.data_ptr(), ldt, float(scale),
-                                                y2.data_ptr(), ldy, run.stream.cuda_stream))
+    if stream is not None:
+        return _elsewhere(embedding, stream, dev, (ids, table, out), ids, table, scale, out=out)
+    i = _ids(ids, dev)
+    shape = ids.shape + (table.shape[1],)
+    y = _torch.empty(shape, dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
+    t2, ldt = _rows(table)
+    y2, ldy = _rows(y)
+    _check(lib.ccsm_train_embedding_forward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), t2.shape[0], t2.shape[1], t2.data_ptr(), ldt, float(scale), y2.data_ptr(),
+                                            ldy, _raw_stream(dev)))
     return y
 
 
@@ -377,14 +376,14 @@ def embedding_backward(dy, ids, rows, scale=1.0, *, out=None, stream=None):
     if dy.dim() < 1 or dy.shape[-1] < 1 or not hasattr(ids, "shape") or dy.shape[:-1] != ids.shape:
         raise ValueError("dy must be (*ids.shape, width)")
     width = dy.shape[-1]
-    with _Run(dev, stream) as run:
-        i = _ids(ids, dev)
-        dt = run.empty((rows, width), t) if out is None else _out(_tensor(out, "out"), _torch.Size((rows, width)), t, dev, "out")
-        run.keep(dy, ids, out)
-        d2, ldd = _rows(dy)
-        t2, ldt = _rows(dt)
-        need = lib.ccsm_train_embedding_backward_workspace(i.numel(), rows, width)
-        ws = run.scratch(need)
-        _check(lib.ccsm_train_embedding_backward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), rows, width, d2.data_ptr(), ldd, float(scale),
-                                                 t2.data_ptr(), ldt, _ptr(ws), need, run.stream.cuda_stream))
+    if stream is not None:
+        return _elsewhere(embedding_backward, stream, dev, (dy, ids, out), dy, ids, rows, scale, out=out)
+    i = _ids(ids, dev)
+    dt = _torch.empty((rows, width), dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), _torch.Size((rows, width)), t, dev, "out")
+    d2, ldd = _rows(dy)
+    t2, ldt = _rows(dt)
+    need = lib.ccsm_train_embedding_backward_workspace(i.numel(), rows, width)
+    ws = _scratch(need, dev)
+    _check(lib.ccsm_train_embedding_backward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), rows, width, d2.data_ptr(), ldd, float(scale), t2.data_ptr(), ldt,
+                                             _ptr(ws), need, _raw_stream(dev)))
     return dt

@@ -107,7 +107,7 @@ Staged staged(const Saved& s, int64_t rows, int64_t width, Scratch& ws, hipStrea
 
 template <typename T, bool TRP, bool TRQ, int B>
 hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
-    constexpr int lds = 4 * 2 * B * 64;
+    constexpr int lds = 5 * B * 128;                    // two chunks of P, three of Q
     auto* f = &product_mfma_kernel<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
     // an attribute of the function on each device: set once for each (setting it twice, from two threads, does no harm)
     static std::atomic<uint64_t> known{0};
@@ -131,16 +131,16 @@ hipError_t product(hipStream_t st, const Staged& p, const Staged& q, int64_t M, 
     a.M = (int)M; a.N = (int)N; a.K = (int)K;
     a.passes = p.planes == 1 ? 1 : q.planes == 1 ? 3 : 6;
     a.ep = ep;
-    const int64_t steps = cdiv(K, 32) * a.passes;
+    const int64_t chunks = cdiv(K, 64) * a.passes;
     const int64_t big = cdiv(M, 256) * cdiv(N, 256), small = cdiv(M, 128) * cdiv(N, 128);
     const int B = big >= 200 ? 256 : 128;
     a.tiles_i = (int)cdiv(M, B); a.tiles_j = (int)cdiv(N, B);
     const int64_t tiles = B == 256 ? big : small, slots = B == 256 ? 256 : 512;
     int64_t splits = tiles * 2 <= slots ? slots / tiles : 1;
-    const int64_t least = 16;                                     // steps of a split
-    if (splits > cdiv(steps, least)) splits = cdiv(steps, least);
-    a.steps = (int)(cdiv(cdiv(steps, splits), a.passes) * a.passes);
-    a.splits = (int)cdiv(steps, a.steps);
+    const int64_t least = 8;                                      // chunks of a split
+    if (splits > cdiv(chunks, least)) splits = cdiv(chunks, least);
+    a.chunks = (int)(cdiv(cdiv(chunks, splits), a.passes) * a.passes);
+    a.splits = (int)cdiv(chunks, a.chunks);
     a.part_ld = (int64_t)up(N, 4);
     a.part = a.splits > 1 ? ws.take<float>((size_t)a.splits * M * a.part_ld) : nullptr;
     if (count) return hipSuccess;

@@ -1,17 +1,21 @@
 // Training operators: the matrix product on the matrix cores.  out(i, j) = sum over k of P(i, k) Q(j, k), P and Q of 16-bit elements in device
 // memory, fp32 accumulators.
 //
-// Tile and waves.  A workgroup of four waves (2 x 2) owns BI x BJ outputs, a wave a quarter of them as 16 x 16 tiles of v_mfma_f32_16x16x32 (the shape
-// that costs least energy per flop here); the steps along k are 32 deep.  Q is the instruction's first operand, so that a lane ends with four
-// neighbouring j of one i: stores of four elements.
+// Tiles.  256 x 256 outputs by eight waves (2 x 4, one workgroup a CU) or 128 x 128 by four (2 x 2, two workgroups a CU); a wave owns a grid of 16 x 16
+// tiles of v_mfma_f32_16x16x32 (the shape that costs least energy per flop here).  Q is the instruction's first operand, so that a lane ends with
+// four neighbouring j of one i.
 //
-// Operands go from memory straight to LDS (buffer_load_dwordx4 ... lds, 1 KiB per wave and request), four stages deep: a stage is requested three
-// steps before it is read, and one barrier per step says both that a stage has landed (counted vmcnt) and that the oldest one is free.  The
-// fragments of step s + 1 are read from LDS while step s multiplies, so the matrix pipe waits for neither.
+// Measured (16384 x 4096 x 4096 bf16): x w^T 400 us (1373 TFLOP/s), d w 403, d^T x 389; at 1.95 GHz the matrix pipe is busy 66 % of the cycles.  Without the
+// requests the loop takes 8 % fewer cycles, without the fragment reads as many as with them.
+//
+// Operands go from memory straight to LDS (buffer_load_dwordx4 ... lds, 1 KiB per wave and request) in chunks of 64 k, so that a row of an operand
+// whose k is contiguous is read as whole 128-byte lines: with chunks of 32 k each line was fetched twice (75 instead of 38 M L2 requests for a 16384 x
+// 4096 x 4096 product) and the requests alone took 1770 cycles per 32 k, matrix instructions or not.  Two chunks of P and three of Q are in LDS (all
+// of its 160 KB): P's next chunk is requested two steps of 32 k before it is read, Q's next but one four.
 //
 // Two storage forms of an operand, by which index is contiguous in memory:
-//   k (TR = false)   LDS rows of 32 k = 64 bytes; a fragment is one ds_read_b128 per lane; piece c (16 bytes) of row r lies at c ^ (r >> 1 & 3)
-//   i or j (TR)      LDS rows of BI or BJ elements, one per k; a fragment is two ds_read_b64_tr_b16 (the LDS transposes 4 x 16 blocks); the
+//   k (TR = false)   LDS rows of 64 k = 128 bytes; a fragment is one ds_read_b128 per lane; piece c (16 bytes) of row r lies at c ^ (r & 7)
+//   i or j (TR)      LDS rows of the tile's i or j, one per k; a fragment is two ds_read_b64_tr_b16 (the LDS transposes 4 x 16 blocks); the
 //                    32-byte piece p of row k lies at p ^ s(k), s = k & 3 | k >> 1 & 4: the eight rows that are read together lie in eight
 //                    different parts of the 256 bytes of banks
 // Both permutations are made on the source side (each lane requests the piece that belongs where its 16 bytes land).
@@ -35,16 +39,20 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
+// run: the compiler's own form.  tied: the accumulator stays in its registers (left to itself the compiler gives most products another destination and
+// copies 200 accumulators a step around); what reads or writes such an accumulator by another instruction waits by itself (below).
 template <typename E> struct Mfma;
 template <> struct Mfma<f16> {
     static __device__ __forceinline__ f32x4 run(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void tied(s16x8 a, s16x8 b, f32x4& c) { asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b)); }
 };
 template <> struct Mfma<b16> {
     static __device__ __forceinline__ f32x4 run(s16x8 a, s16x8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void tied(s16x8 a, s16x8 b, f32x4& c) { asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b)); }
 };
 
 // what a product's results go through: z = acc + bias; y = act(z) + residual.  With `part`, the accumulators go there instead (split k)
@@ -56,7 +64,7 @@ struct ProductArgs {
     Plane P, Q;
     int M, N, K;
     int passes;               // 1, 3 (P in three planes, Q in one) or 6
-    int tiles_i, tiles_j, splits, steps;      // steps of one split (a multiple of passes)
+    int tiles_i, tiles_j, splits, chunks;     // chunks of 64 k times passes of one split (a multiple of passes)
     float* part; long long part_ld;           // [split][M][part_ld]
     Epilogue ep;
 };
@@ -87,22 +95,22 @@ __device__ __forceinline__ Loose<T, N> raw_row(const T* p, int left) {
     return t;
 }
 
-// One operand's side of the tile: requests and fragment reads.  B: the tile's extent, W: a wave's, NW waves in the workgroup.
+// One operand's side: requests by NW waves (this one is number `wave` of them) for B rows or columns, and the fragments of this wave's W of them
 template <bool TR, int B, int W, int NW>
 struct Side {
-    static constexpr int kStage = B * 64;                  // bytes
-    static constexpr int kReq = kStage / 1024 / NW;        // requests per wave and stage
+    static constexpr unsigned kChunk = B * 128;            // bytes
+    static constexpr int kReq = kChunk / 1024 / NW;        // requests per wave and chunk
     static constexpr int kFrag = W / 16;
-    unsigned off[kReq];                                    // byte offset of this lane's piece from the stage's origin
-    int kpos[kReq];                                        // its k within the stage
-    unsigned rd[TR ? kFrag : 1];                           // LDS byte offsets of the fragments
+    unsigned off[kReq];                                    // byte offset of this lane's piece from the chunk's origin
+    int kpos[kReq];                                        // its k within the chunk
+    unsigned rd[TR ? kFrag : 2];                           // LDS byte offsets of the fragments (k contiguous: of the two halves of a chunk)
 
     __device__ __forceinline__ void init(const Plane& p, int at, int extent, int wave, int lane, int w0, unsigned lds) {
 #pragma unroll
         for (int r = 0; r < kReq; ++r) {
-            const int q = r * NW + wave;                   // request number within the stage
+            const int q = r * NW + wave;                   // request number within the chunk
             if (!TR) {
-                const int row = q * 16 + (lane >> 2), c = (lane & 3) ^ ((row >> 1) & 3);
+                const int row = q * 8 + (lane >> 3), c = (lane & 7) ^ (row & 7);
                 const int i = at + row < extent ? row : extent - 1 - at;
                 off[r] = (unsigned)(((long long)i * p.ld + 8 * c) * 2);
                 kpos[r] = 8 * c;
@@ -116,34 +124,53 @@ struct Side {
             }
         }
         if (!TR) {
-            rd[0] = lds + (unsigned)((w0 + (lane & 15)) * 64 + (((lane >> 4) ^ ((lane >> 1) & 3)) << 4));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) rd[h] = lds + (unsigned)((w0 + (lane & 15)) * 128 + (((4 * h + (lane >> 4)) ^ (lane & 7)) << 4));
         } else {
             const int k = 8 * (lane >> 4) + ((lane & 15) >> 2), s = (k & 3) | ((k >> 1) & 4);
 #pragma unroll
             for (int f = 0; f < kFrag; ++f) rd[f] = lds + (unsigned)(k * (2 * B) + (((w0 / 16 + f) ^ s) << 5) + (lane & 3) * 8);
         }
     }
-    // request r of a stage into LDS at `m0` (the wave's base of that request)
+    // request r of a chunk into LDS at `m0` (the wave's base of that request)
     __device__ __forceinline__ void request(int r, u32x4 srd, int left, unsigned m0) const {
         const unsigned o = kpos[r] < left ? off[r] : 0xffffffffu;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m0), "v"(o), "s"(srd) : "memory");
     }
-    __device__ __forceinline__ s16x8 fragment(int f, int stage) const {
+    // fragment f of half h (32 k) of the chunk at byte `base` of this operand's ring
+    __device__ __forceinline__ s16x8 fragment(int f, int h, unsigned base) const {
         typedef __attribute__((address_space(3))) const s16x8* P8;
         typedef __attribute__((address_space(3))) s16x4* P4;
-        if (!TR) return *(P8)(uintptr_t)(rd[0] + f * 1024 + stage * kStage);
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + stage * kStage));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + stage * kStage + 8 * B));
+        if (!TR) return *(P8)(uintptr_t)(rd[h] + base + f * 2048);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + base + h * 64 * B));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + base + h * 64 * B + 8 * B));
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+// where an operand's next chunk comes from
+template <bool TR>
+struct Cursor {
+    const char* base;
+    long long ld, plane;
+    int k, pass, left_chunks;
+    unsigned codes;                                        // the plane of each pass, four bits each
+    __device__ __forceinline__ u32x4 next(int K, int passes, int* left) {
+        const unsigned long long p = (unsigned long long)(base + ((TR ? (long long)k * ld : (long long)k) + (long long)((codes >> (4 * pass)) & 15u) * plane) * 2);
+        *left = left_chunks > 0 ? K - k : 0;               // behind the last chunk everything is out of range: zeros that nobody reads
+        --left_chunks;
+        if (++pass == passes) { pass = 0; k += 64; }
+        return u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, 0xfffffffeu, 0x00020000u};
     }
 };
 
 template <typename T, bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
 __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_mfma_kernel(ProductArgs a) {
     typedef typename std::conditional<sizeof(T) == 4, b16, T>::type E;
-    constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
-    typedef Side<TRP, BI, BI / WI, NW> SP;
+    constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16, HW = BI / WI;
+    typedef Side<TRP, BI, HW, NW> SP;
     typedef Side<TRQ, BJ, BJ / WJ, NW> SQ;
+    constexpr int kReq = SP::kReq;
+    static_assert(SP::kReq == SQ::kReq, "");
     extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
     // Workgroups go to the eight XCDs in turn; each XCD takes one contiguous eighth of the tiles (its L2 holds their operands), in columns of eight
@@ -158,85 +185,102 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
     const int i0 = ti * BI, j0 = tj * BJ;
 
     const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
+    constexpr unsigned kP = SP::kChunk, kQ = SQ::kChunk, kQ0 = 2 * kP;                      // LDS: P's two chunks, then Q's three
+    const unsigned lq = lds + kQ0;
     SP sp;
     SQ sq;
-    sp.init(a.P, i0, a.M, wave, lane, wi * (BI / WI), lds);
-    sq.init(a.Q, j0, a.N, wave, lane, wj * (BJ / WJ), lds + 4 * SP::kStage);
+    sp.init(a.P, i0, a.M, wave, lane, wi * HW, lds);
+    sq.init(a.Q, j0, a.N, wave, lane, wj * (BJ / WJ), lq);
 
-    const int total = (a.K + 31) / 32 * a.passes, first = split * a.steps, last = first + a.steps < total ? first + a.steps : total;
-    int k = first / a.passes * 32, pass = 0;               // of the next stage to be requested (splits begin with a k step's first pass)
-    const char* pb = (const char*)a.P.base + (TRP ? (long long)i0 * 2 : (long long)i0 * a.P.ld * 2);
-    const char* qb = (const char*)a.Q.base + (TRQ ? (long long)j0 * 2 : (long long)j0 * a.Q.ld * 2);
-    int left_stages = last - first;
-    u32x4 srdp, srdq;
-    int left = 0;
-    auto next = [&]() {                                    // the origins of the next stage
-        const int cp = a.passes == 1 ? 0 : a.passes == 3 ? 2 - pass : (0x010102 >> (4 * pass)) & 3, cq = a.passes == 6 ? (0x001120 >> (4 * pass)) & 3 : 0;
-        const unsigned long long p = (unsigned long long)(pb + ((TRP ? (long long)k * a.P.ld : (long long)k) + cp * a.P.plane) * 2);
-        const unsigned long long q = (unsigned long long)(qb + ((TRQ ? (long long)k * a.Q.ld : (long long)k) + cq * a.Q.plane) * 2);
-        srdp = u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, 0xfffffffeu, 0x00020000u};
-        srdq = u32x4{(unsigned)q, (unsigned)(q >> 32) & 0xffffu, 0xfffffffeu, 0x00020000u};
-        left = left_stages > 0 ? a.K - k : 0;              // behind the last stage: everything is out of range, zeros that nobody reads
-        --left_stages;
-        if (++pass == a.passes) { pass = 0; k += 32; }
-    };
-    constexpr int kReq = SP::kReq + SQ::kReq;
-    auto request = [&](int r, int stage) {
-        if (r < SP::kReq) sp.request(r, srdp, left, lds + stage * SP::kStage + (r * NW + wave) * 1024);
-        else sq.request(r - SP::kReq, srdq, left, lds + 4 * SP::kStage + stage * SQ::kStage + ((r - SP::kReq) * NW + wave) * 1024);
-    };
+    const int total = (a.K + 63) / 64 * a.passes, first = split * a.chunks, last = first + a.chunks < total ? first + a.chunks : total;
+    // passes (P's plane, Q's): 6: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); 3: (2,0) (1,0) (0,0); 1: (0,0).  Splits begin with a chunk's first pass.
+    const int k0 = first / a.passes * 64;
+    Cursor<TRP> cp{(const char*)a.P.base + (TRP ? (long long)i0 : (long long)i0 * a.P.ld) * 2, a.P.ld, a.P.plane, k0, 0, last - first, a.passes == 6 ? 0x001102u : a.passes == 3 ? 0x012u : 0u};
+    Cursor<TRQ> cq{(const char*)a.Q.base + (TRQ ? (long long)j0 : (long long)j0 * a.Q.ld) * 2, a.Q.ld, a.Q.plane, k0, 0, last - first, a.passes == 6 ? 0x010120u : 0u};
+    u32x4 srd;
+    int left;
+    auto request_p = [&](int r, unsigned base) { sp.request(r, srd, left, lds + base + (r * NW + wave) * 1024); };
+    auto request_q = [&](int r, unsigned base) { sq.request(r, srd, left, lq + base + (r * NW + wave) * 1024); };
 
     f32x4 acc[FI][FJ];
 #pragma unroll
     for (int p = 0; p < FI; ++p)
 #pragma unroll
-        for (int q = 0; q < FJ; ++q) acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < FJ; ++q) {
+            acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+            asm volatile("" : "+v"(acc[p][q]));            // (written here, far from the first product)
+        }
+    // Chunk c = steps 2c and 2c + 1.  The fragments of a step are read while the step before multiplies; one barrier a chunk, in front of step 2c + 1, behind
+    // which chunk c + 1 has landed (every wave has waited for all but its last four requests) and chunk c has been read.  Its place in P's ring is
+    // requested for chunk c + 2 in step 2c + 1, the one of chunk c - 1 in Q's ring for chunk c + 2 in step 2c.
     s16x8 fp[2][FI], fq[2][FJ];
+    auto all_p = [&](unsigned base) {
+        srd = cp.next(a.K, a.passes, &left);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        next();
+        for (int r = 0; r < kReq; ++r) request_p(r, base);
+    };
+    auto all_q = [&](unsigned base) {
+        srd = cq.next(a.K, a.passes, &left);
 #pragma unroll
-        for (int r = 0; r < kReq; ++r) request(r, s);
-    }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(3 * kReq) : "memory");
+        for (int r = 0; r < kReq; ++r) request_q(r, base);
+    };
+    all_p(0);
+    all_q(0);
+    all_q(kQ);
+    all_p(kP);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * kReq) : "memory");
 #pragma unroll
-    for (int p = 0; p < FI; ++p) fp[0][p] = sp.fragment(p, 0);
+    for (int q = 0; q < FJ; ++q) fq[0][q] = sq.fragment(q, 0, 0);
 #pragma unroll
-    for (int q = 0; q < FJ; ++q) fq[0][q] = sq.fragment(q, 0);
-
-    auto body = [&](auto S) {                              // step s with s % 4 = S
-        constexpr int s = decltype(S)::value, cur = s & 1, nxt = cur ^ 1, stage = (s + 1) & 3;
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(2 * kReq) : "memory");
-        next();
-        constexpr int kReads = FI + FJ;
+    for (int p = 0; p < FI; ++p) fp[0][p] = sp.fragment(p, 0, 0);
+    unsigned bp = 0, bq = 0, free_q = 2 * kQ;              // the current chunk's places in the rings, Q's free one
+    constexpr int kReads = FI + FJ, kRows = FI == 8 ? 6 : FI;
+    for (int c = first; c < last; ++c) {
+        srd = cq.next(a.K, a.passes, &left);
 #pragma unroll
-        for (int p = 0; p < FI; ++p) {
-            // spread over the step: the next step's fragments first, a request of the fourth next stage behind each row of products
+        for (int p = 0; p < FI; ++p) {                     // fragments of the step's other half first, then requests, between rows of products
 #pragma unroll
-            for (int f = p * kReads / FI; f < (p + 1) * kReads / FI; ++f) {
-                if (f < FJ) fq[nxt][f] = sq.fragment(f, stage);
-                else fp[nxt][f - FJ] = sp.fragment(f - FJ, stage);
+            for (int f = p * kReads / kRows; f < (p + 1) * kReads / kRows && f < kReads; ++f) {
+                if (f < FJ) fq[1][f] = sq.fragment(f, 1, bq);
+                else fp[1][f - FJ] = sp.fragment(f - FJ, 1, bp);
             }
 #pragma unroll
-            for (int q = 0; q < FJ; ++q) acc[p][q] = Mfma<E>::run(fq[cur][q], fp[cur][p], acc[p][q]);
+            for (int q = 0; q < FJ; ++q) Mfma<E>::tied(fq[0][q], fp[0][p], acc[p][q]);
 #pragma unroll
-            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request(r, s);
+            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request_q(r, free_q);
+            __builtin_amdgcn_sched_barrier(0);             // (left to itself the compiler begins the next step's products here and waits for their operands)
         }
-    };
-    // four steps a turn (the steps behind the last one multiply zeros): leaving between them would cost copies of every register at each exit
-    for (int turns = (last - first + 3) >> 2; turns > 0; --turns) {
-        body(std::integral_constant<int, 0>());
-        body(std::integral_constant<int, 1>());
-        body(std::integral_constant<int, 2>());
-        body(std::integral_constant<int, 3>());
+        free_q = bq;
+        bq = bq == 2 * kQ ? 0 : bq + kQ;
+        bp ^= kP;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kReq) : "memory");
+        srd = cp.next(a.K, a.passes, &left);
+#pragma unroll
+        for (int p = 0; p < FI; ++p) {
+#pragma unroll
+            for (int f = p * kReads / kRows; f < (p + 1) * kReads / kRows && f < kReads; ++f) {
+                if (f < FJ) fq[0][f] = sq.fragment(f, 0, bq);
+                else fp[0][f - FJ] = sp.fragment(f - FJ, 0, bp);
+            }
+#pragma unroll
+            for (int q = 0; q < FJ; ++q) Mfma<E>::tied(fq[1][q], fp[1][p], acc[p][q]);
+#pragma unroll
+            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request_p(r, bp ^ kP);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
+    asm volatile("s_nop 15\n\ts_nop 15");                    // the last products' results are there (16 passes at most), for whatever reads them below
+#pragma unroll
+    for (int p = 0; p < FI; ++p)
+#pragma unroll
+        for (int q = 0; q < FJ; ++q) asm volatile("" : "+v"(acc[p][q]));
     // The results leave through the wave's own part of LDS, 32 rows of i at a time (rows 16 bytes longer than they need: the lanes' writes fall on
     // different banks), and from there in pieces of eight neighbours of a row.  A lane's column does not change, so its bias is loaded once; a
     // round's residual is loaded a round ahead (one load at a time, 128 loads one behind the other, took 170 of 640 us of a 16384 x 4096 x 4096
     // product).
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // no request may still write LDS
-    constexpr int WJT = BJ / WJ, kRow = WJT + 4, kPer = WJT / 8, kIt = 32 * kPer / 64, kRows = 64 / kPer;
-    static_assert(32 * kRow * 4 * NW <= 4 * (SP::kStage + SQ::kStage) && 64 % kPer == 0, "the waves' rows fit into the stages");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (no request may still write LDS)
+    constexpr int WJT = BJ / WJ, kRow = WJT + 4, kPer = WJT / 8, kIt = 32 * kPer / 64, kRowsIt = 64 / kPer;
+    static_assert(32 * kRow * 4 * NW <= kQ0 + 3 * kQ && 64 % kPer == 0, "the waves' rows fit into the stages");
     float* out = reinterpret_cast<float*>(ops_smem) + wave * 32 * kRow;
     const int c = lane % kPer * 8, j = j0 + wj * WJT + c, left_j = a.N - j, iw = i0 + wi * (BI / WI) + lane / kPer;
     const bool res = !a.part && a.ep.residual && left_j > 0;
@@ -246,7 +290,7 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
     auto residual = [&](int h, Loose<T, 8> (&o)[kIt]) {
 #pragma unroll
         for (int q = 0; q < kIt; ++q) {
-            const int i = iw + 32 * h + q * kRows;
+            const int i = iw + 32 * h + q * kRowsIt;
             if (i < a.M) o[q] = raw_row<T, 8>((const T*)a.ep.residual + (long long)i * a.ep.ldr + j, left_j);
         }
     };
@@ -263,8 +307,8 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
         if (left_j > 0) {
 #pragma unroll
             for (int q = 0; q < kIt; ++q) {
-                const int i = iw + 32 * h + q * kRows;
-                const float* o = out + (lane / kPer + q * kRows) * kRow + c;
+                const int i = iw + 32 * h + q * kRowsIt;
+                const float* o = out + (lane / kPer + q * kRowsIt) * kRow + c;
                 const f32x4 u = *(const f32x4*)o, v = *(const f32x4*)(o + 4);
                 if (i >= a.M) continue;
                 if (a.part) {

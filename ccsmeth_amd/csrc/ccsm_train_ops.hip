@@ -245,19 +245,23 @@ void in_ranges(int64_t rows, int64_t per_row, F launch) {
     for (int64_t r = 0; r < rows; r += step) launch(r, rows - r < step ? rows - r : step);
 }
 
-struct SortPlan { int bits, passes, digit, per_lane; int64_t blocks, pieces; };
-SortPlan sort_plan(int64_t tokens, int64_t rows) {
+struct SortPlan { int bits, passes, digit, per_lane, piece, lanes, groups; int64_t blocks, sums; };
+SortPlan sort_plan(int type, int64_t tokens, int64_t rows, int width) {
     SortPlan s;
     s.bits = 1;
     while (((int64_t)1 << s.bits) < rows + 1) ++s.bits;          // ids 0 .. rows (rows = no token)
     s.passes = (s.bits + 7) / 8;
     s.digit = (s.bits + s.passes - 1) / s.passes;
-    s.per_lane = tokens <= 262144 ? 4 : 16;                      // 1024 tokens a workgroup until the chip is full of them (19 -> 6 us a pass at 65536), then 4096
+    s.per_lane = tokens <= 131072 ? 4 : 16;                      // 1024 tokens a workgroup up to kFewBlocks workgroups (19 -> 6 us a pass at 65536), then 4096
     s.blocks = cdiv(tokens, 256 * s.per_lane);
-    s.pieces = cdiv(tokens, kPiece);
+    const int64_t all = cdiv(width, 16 / (int64_t)size_of(type));
+    s.piece = tokens / kLongPiece * all >= 65536 ? kLongPiece : kShortPiece;      // a wave for each SIMD at least
+    s.lanes = (int)(all < 256 ? all : 256);
+    s.groups = 256 / s.lanes;
+    s.sums = cdiv(tokens, (int64_t)s.piece * s.groups);
     return s;
 }
-struct EmbedScratch { unsigned *keys[2], *at[2], *counts, *marks; int64_t mark_words; float* part; int64_t part_ld; };
+struct EmbedScratch { unsigned *keys[2], *at[2], *counts, *list, *marks; int64_t mark_words; float* part; int64_t part_ld; };
 EmbedScratch embed_scratch(Scratch& ws, const SortPlan& s, int64_t tokens, int64_t rows, int width) {
     EmbedScratch e;
     for (int k = 0; k < 2; ++k) {
@@ -265,10 +269,11 @@ EmbedScratch embed_scratch(Scratch& ws, const SortPlan& s, int64_t tokens, int64
         e.at[k] = ws.take<unsigned>(tokens);
     }
     e.counts = ws.take<unsigned>((size_t)s.blocks << s.digit);
+    e.list = ws.take<unsigned>(1 + s.sums);
     e.mark_words = cdiv(rows, 4);
     e.marks = ws.take<unsigned>(e.mark_words);
     e.part_ld = (int64_t)up(width, 8);
-    e.part = ws.take<float>((size_t)2 * s.pieces * e.part_ld);
+    e.part = ws.take<float>((size_t)2 * s.sums * e.part_ld);
     return e;
 }
 ccsm_status check_embedding(int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int width) {
@@ -284,8 +289,8 @@ template <int Q>
 void sort_pass(hipStream_t st, const SortPlan& s, const EmbedScratch& b, const void* ids, int id_type, int64_t tokens, int64_t rows, int pass, int k) {
     const unsigned *keys = pass ? b.keys[k] : nullptr, *at = pass ? b.at[k] : nullptr;
     const int bins = 1 << s.digit;
-    sort_count_kernel<Q><<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, tokens, rows, pass * s.digit, bins, b.counts, pass ? nullptr : b.marks, b.mark_words);
-    sort_scan_kernel<<<1, 1024, 0, st>>>(b.counts, s.blocks << s.digit);
+    sort_count_kernel<Q><<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, tokens, rows, pass * s.digit, bins, b.counts, pass ? nullptr : b.marks, b.mark_words, b.list);
+    if (s.blocks > kFewBlocks) sort_scan_kernel<<<1, 1024, 0, st>>>(b.counts, s.blocks << s.digit);
     sort_scatter_kernel<Q><<<(unsigned)s.blocks, 256, 0, st>>>(ids, id_type, keys, at, tokens, rows, pass * s.digit, bins, b.counts, b.keys[k ^ 1], b.at[k ^ 1],
                                                                pass + 1 == s.passes ? (uint8_t*)b.marks : nullptr);
 }
@@ -344,17 +349,17 @@ ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int6
     TYPED(type, constexpr int P = 16 / sizeof(T); const int64_t pieces = cdiv(width, P);
           in_ranges(tokens, pieces, [&](int64_t t, int64_t n) {
               const char* i = (const char*)ids + t * (id_type == CCSM_ID_U8 ? 1 : id_type == CCSM_ID_I32 ? 4 : 8);
-              lookup_kernel<T, P><<<(unsigned)cdiv(n * pieces, 256), 256, 0, st>>>(i, id_type, (unsigned)(n * pieces), Div::by((unsigned)pieces), rows, width, (const T*)table, ldt,
+              lookup_kernel<T, P><<<(unsigned)cdiv(n * pieces, 1024), 256, 0, st>>>(i, id_type, (unsigned)(n * pieces), Div::by((unsigned)pieces), rows, width, (const T*)table, ldt,
                                                                                  scale, (T*)y + t * ldy, ldy);
           }));
     LAUNCHED("embedding_forward");
     return CCSM_OK;
 }
 
-size_t ccsm_train_embedding_backward_workspace(int64_t tokens, int64_t rows, int32_t width) {
-    if (tokens <= 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols) return 0;
+size_t ccsm_train_embedding_backward_workspace(int type, int64_t tokens, int64_t rows, int32_t width) {
+    if (!good_type(type) || tokens <= 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols) return 0;
     Scratch ws;
-    (void)embed_scratch(ws, sort_plan(tokens, rows), tokens, rows, width);
+    (void)embed_scratch(ws, sort_plan(type, tokens, rows, width), tokens, rows, width);
     return ws.used;
 }
 ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
@@ -364,7 +369,7 @@ ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int
     if (e != CCSM_OK) return e;
     REFUSE(!dtable || ldt < width || (tokens && (!dy || lddy < width)), "embedding: dy and dtable must be non-NULL, their strides at least the width");
     REFUSE(off_by(dtable, size_of(type)) || off_by(dy, size_of(type)), "embedding: a pointer is not aligned to its elements");
-    if ((e = check_room(ccsm_train_embedding_backward_workspace(tokens, rows, width), workspace, workspace_bytes)) != CCSM_OK) return e;
+    if ((e = check_room(ccsm_train_embedding_backward_workspace(type, tokens, rows, width), workspace, workspace_bytes)) != CCSM_OK) return e;
     ON_DEVICE(device);
     hipStream_t st = (hipStream_t)stream;
     if (tokens == 0) {
@@ -374,17 +379,20 @@ ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int
     }
     Scratch ws;
     ws.base = (char*)workspace;
-    const SortPlan s = sort_plan(tokens, rows);
+    const SortPlan s = sort_plan(type, tokens, rows, width);
     const EmbedScratch b = embed_scratch(ws, s, tokens, rows, width);
     int k = 0;
     for (int pass = 0; pass < s.passes; ++pass, k ^= 1) {
         if (s.per_lane == 4) sort_pass<4>(st, s, b, ids, id_type, tokens, rows, pass, k);
         else sort_pass<16>(st, s, b, ids, id_type, tokens, rows, pass, k);
     }
-    TYPED(type, constexpr int P = 16 / sizeof(T); const int64_t lanes = cdiv(width, P); const unsigned sums = (unsigned)cdiv(s.pieces * lanes, 256);
-          piece_sum_kernel<T, P><<<sums + grid_of(cdiv(rows, 8), 4096), 256, 0, st>>>(b.keys[k], b.at[k], tokens, rows, sums, Div::by((unsigned)lanes), width, (const T*)dy, lddy,
-                                                                                    scale, (T*)dtable, ldt, b.part, b.part_ld, (const uint8_t*)b.marks);
-          join_kernel<T><<<(unsigned)s.pieces, 256, 0, st>>>(b.keys[k], tokens, rows, width, scale, (T*)dtable, ldt, b.part, b.part_ld));
+    TYPED(type, constexpr int P = 16 / sizeof(T); const int chunks = (int)cdiv(width, 256);
+          auto* f = s.piece == kLongPiece ? &piece_sum_kernel<T, P, kLongPiece> : &piece_sum_kernel<T, P, kShortPiece>;
+          f<<<dim3((unsigned)s.sums + grid_of(cdiv(rows, 8), 4096), (unsigned)cdiv(width, 256 * P)), 256, 0, st>>>(
+              b.keys[k], b.at[k], tokens, rows, (unsigned)s.sums, s.groups, Div::by((unsigned)s.lanes), width, (const T*)dy, lddy, scale, (T*)dtable, ldt, b.part, b.part_ld,
+              (const uint8_t*)b.marks, b.list);
+          if (s.sums > 1) join_kernel<T><<<grid_of(s.sums * chunks, 1024), 256, 0, st>>>(b.keys[k], tokens, s.piece * s.groups, width, scale, (T*)dtable, ldt, b.part, b.part_ld,
+                                                                                         b.list, chunks));
     LAUNCHED("embedding_backward");
     return CCSM_OK;
 }

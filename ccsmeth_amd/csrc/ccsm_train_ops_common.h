@@ -43,6 +43,16 @@ __device__ __forceinline__ void store_row(T* p, int left, const float (&v)[N]) {
     }
 }
 
+// N elements as they are (the ones behind `left`: zeros)
+template <typename T, int N>
+__device__ __forceinline__ Loose<T, N> raw_row(const T* p, int left) {
+    if (left >= N) return *reinterpret_cast<const Loose<T, N>*>(p);
+    Loose<T, N> t;
+#pragma unroll
+    for (int k = 0; k < N; ++k) t.v[k] = k < left ? p[k] : (T)0.f;
+    return t;
+}
+
 // x / d for x < 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1, s = the bits of d - 1 (Granlund and Montgomery's method for 31 bits)
 struct Div {
     unsigned d, m, s;

@@ -1,8 +1,8 @@
 // Training operators: embedding lookup with scaling, and the table's gradient by sorted tokens (include/ccsm_train_ops.h).
 //
 // Gradient: dtable[v] = scale * sum of dy[i] over the tokens i with ids[i] = v.  The tokens are sorted by id with a stable radix sort (8 bits at
-// most a pass), so that the rows of one sum lie next to each other in token order; each group of lanes then walks a piece of kPiece sorted
-// tokens and adds rows up in fp32 registers, eight rows in flight.  A sum that lies inside a piece is written at once; what crosses a piece's
+// most a pass), so that the rows of one sum lie next to each other in token order; each group of lanes then walks a piece of sorted tokens and adds
+// rows up in fp32 registers, the next ones in flight.  A sum that lies inside a piece is written at once; what crosses a piece's
 // border goes to two partial rows of the workspace (its head, its tail), which a second kernel adds in a fixed order.  Rows of the table that no
 // token names are marked by the sort's last pass (a byte for each row) and cleared by further workgroups of the sums' launch, so the table
 // is written once.  No floating-point atomics: the order of a sum depends on the ids alone.
@@ -10,38 +10,47 @@
 
 namespace ccsm_ops {
 
-constexpr int kPiece = 32;              // sorted tokens per group of lanes
-
 __device__ __forceinline__ unsigned id_at(const void* ids, int type, long long i, long long rows) {      // rows: no token
     const long long v = type == 0 ? ((const uint8_t*)ids)[i] : type == 1 ? ((const int32_t*)ids)[i] : ((const int64_t*)ids)[i];
     return v >= 0 && v < rows ? (unsigned)v : (unsigned)rows;
 }
 
-// one lane: N neighbouring values of one token's row
+// a lane takes N neighbouring values of a token's row, four tokens (or parts of one) a workgroup apart: four ids, then four rows in flight
 template <typename T, int N>
 __global__ __launch_bounds__(256) void lookup_kernel(const void* ids, int id_type, unsigned items, Div pieces, long long rows, int width, const T* table, long long ldt,
                                                      float scale, T* y, long long ldy) {
-    const unsigned i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= items) return;
-    const unsigned t = pieces.of(i);
-    const int c = (int)(i - t * pieces.d) * N;
-    const unsigned id = id_at(ids, id_type, t, rows);
-    float v[N] = {};
-    if (id < rows) load_row<T, N>(table + (long long)id * ldt + c, width - c, v);
+    constexpr int U = 4;
+    const unsigned first = blockIdx.x * (256u * U) + threadIdx.x;
+    unsigned t[U], id[U];
+    int c[U];
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] *= scale;
-    if (id >= rows) {
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = 0.f;                  // (whatever the scale is)
+    for (int u = 0; u < U; ++u) {
+        const unsigned i = first + 256u * u;
+        t[u] = pieces.of(i < items ? i : 0);
+        c[u] = (int)((i < items ? i : 0) - t[u] * pieces.d) * N;
+        id[u] = id_at(ids, id_type, t[u], rows);
     }
-    store_row<T, N>(y + (long long)t * ldy + c, width - c, v);
+    float v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (id[u] < rows) load_row<T, N>(table + (long long)id[u] * ldt + c[u], width - c[u], v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[u][k] = id[u] < rows ? v[u][k] * scale : 0.f;
+        if (first + 256u * u < items) store_row<T, N>(y + (long long)t[u] * ldy + c[u], width - c[u], v[u]);
+    }
 }
 
 // ---- the sort -------------------------------------------------------------------------------------------------------
-// A workgroup takes 256 Q tokens, a wave 64 Q of them in order.  counts[digit][block] of this pass's digit; the first pass also clears the marks.
+// A workgroup takes 256 Q tokens, a wave 64 Q of them in order.  Up to kFewBlocks workgroups each sums up the counts itself (counts[block][digit]: a lane per
+// digit; a kernel for that alone took 10 us at 65536 tokens, the sums inside the scatter 3); above, that square of reads costs more than the kernel, and
+// counts[digit][block] are scanned.  The first pass also clears the marks and the list's length.
+constexpr int kFewBlocks = 128;
 template <int Q>
 __global__ __launch_bounds__(256) void sort_count_kernel(const void* ids, int id_type, const unsigned* keys, long long n, long long rows, int shift, int bins,
-                                                         unsigned* counts, unsigned* marks, long long mark_words) {
+                                                         unsigned* counts, unsigned* marks, long long mark_words, unsigned* list) {
     __shared__ unsigned h[256];
     h[threadIdx.x] = 0;
     __syncthreads();
@@ -55,10 +64,11 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const void* ids, int id
 #pragma unroll
     for (int q = 0; q < Q; ++q)
         if (base + q * 256 + threadIdx.x < n) atomicAdd(&h[(k[q] >> shift) & (bins - 1)], 1u);
+    if (marks && blockIdx.x == 0 && threadIdx.x == 0) *list = 0;
     if (marks)
         for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < mark_words; i += (long long)gridDim.x * 256) marks[i] = 0;
     __syncthreads();
-    if ((int)threadIdx.x < bins) counts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = h[threadIdx.x];
+    if ((int)threadIdx.x < bins) counts[gridDim.x <= kFewBlocks ? (long long)blockIdx.x * bins + threadIdx.x : (long long)threadIdx.x * gridDim.x + blockIdx.x] = h[threadIdx.x];
 }
 // exclusive running sum of c[0 .. n), in place, one workgroup, four values a lane
 __global__ __launch_bounds__(1024) void sort_scan_kernel(unsigned* c, long long n) {
@@ -98,6 +108,7 @@ template <int Q>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const void* ids, int id_type, const unsigned* keys, const unsigned* at, long long n, long long rows, int shift,
                                                            int bins, const unsigned* starts, unsigned* keys_out, unsigned* at_out, uint8_t* marks) {
     __shared__ unsigned next[4][256];
+    __shared__ unsigned wave_sum[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int d = threadIdx.x; d < 1024; d += 256) (&next[0][0])[d] = 0;
     __syncthreads();
@@ -112,9 +123,33 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const void* ids, int 
 #pragma unroll
     for (int q = 0; q < Q; ++q)
         if (base + q * 64 + lane < n) atomicAdd(&next[wave][(k[q] >> shift) & (bins - 1)], 1u);
-    __syncthreads();
+    unsigned start = 0;
+    if (gridDim.x <= kFewBlocks) {
+        unsigned all = 0;
+        if ((int)threadIdx.x < bins) {
+#pragma unroll 16
+            for (int b = 0; b < (int)gridDim.x; ++b) {
+                const unsigned t = starts[b * bins + threadIdx.x];
+                all += t;
+                start += b < (int)blockIdx.x ? t : 0;
+            }
+        }
+        unsigned s = all;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned t = __shfl_up(s, o);
+            if (lane >= o) s += t;
+        }
+        if (lane == 63) wave_sum[wave] = s;
+        __syncthreads();
+        start += s - all;
+        for (int w = 0; w < wave; ++w) start += wave_sum[w];
+    } else {
+        __syncthreads();
+        if ((int)threadIdx.x < bins) start = starts[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+    }
     if ((int)threadIdx.x < bins) {
-        unsigned s = starts[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+        unsigned s = start;
         for (int w = 0; w < 4; ++w) {
             const unsigned t = next[w][threadIdx.x];
             next[w][threadIdx.x] = s;
@@ -145,101 +180,163 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const void* ids, int 
 }
 
 // ---- the sums -------------------------------------------------------------------------------------------------------
-// workgroups [0, sums): a group of lanes = one piece of sorted tokens, a lane of it = N neighbouring columns.  The others clear the rows of the
-// table that have no mark.
-template <typename T, int N>
-__global__ __launch_bounds__(256) void piece_sum_kernel(const unsigned* keys, const unsigned* at, long long n, long long rows, unsigned sums, Div lanes, int width, const T* dy,
-                                                        long long lddy, float scale, T* dt, long long ldt, float* part, long long part_ld, const uint8_t* marks) {
+// Pieces of 32 sorted tokens, or of 8 where those would leave most of the chip idle (86016 x 72 fp16 in 32s are 378 waves of 32 rows each).
+constexpr int kLongPiece = 32, kShortPiece = 8;
+// Workgroups [0, sums) of a column block: `groups` groups of lanes with a piece of sorted tokens each, a lane = N neighbouring columns.  A sum that lies
+// inside a piece is written at once.  What crosses pieces is put together in LDS by the group whose piece it starts in, and written if it ends in
+// this workgroup; else it leaves as the workgroup's head or tail.  The other workgroups clear the rows of the table that have no mark.
+template <typename T, int N, int kPiece>
+__global__ __launch_bounds__(256, 4) void piece_sum_kernel(const unsigned* keys, const unsigned* at, long long n, long long rows, unsigned sums, int groups, Div lanes, int width,
+                                                        const T* dy, long long lddy, float scale, T* dt, long long ldt, float* part, long long part_ld, const uint8_t* marks,
+                                                        unsigned* list) {
+    const int c0 = blockIdx.y * 256 * N;
     if (blockIdx.x >= sums) {
-        // eight rows' marks at a time
-        for (long long r0 = (blockIdx.x - sums) * 8ll; r0 < rows; r0 += (gridDim.x - sums) * 8ll)
+        for (long long r0 = (blockIdx.x - sums) * 8ll; r0 < rows; r0 += (gridDim.x - sums) * 8ll)      // eight rows' marks at a time
             for (unsigned i = threadIdx.x; i < 8 * lanes.d; i += 256) {
                 const unsigned q = lanes.of(i);
                 const long long r = r0 + q;
-                const int c = (int)(i - q * lanes.d) * N;
+                const int c = c0 + (int)(i - q * lanes.d) * N;
                 const float z[N] = {};
-                if (r < rows && !marks[r]) store_row<T, N>(dt + r * ldt + c, width - c, z);
+                if (r < rows && c < width && !marks[r]) store_row<T, N>(dt + r * ldt + c, width - c, z);
             }
         return;
     }
-    const unsigned id = blockIdx.x * 256u + threadIdx.x, g = lanes.of(id);
-    const int c = (int)(id - g * lanes.d) * N;
-    const long long s = (long long)g * kPiece;
-    if (s >= n) return;
-    const long long e = s + kPiece < n ? s + kPiece : n;
-    float acc[N];
+    __shared__ float head[N][256], tail[N][256];
+    __shared__ unsigned char kind[256];                    // of a group: 1 its head belongs to an earlier piece's sum, 2 the whole piece does and so does more, 4 it has a tail
+    const int j = (int)lanes.of(threadIdx.x), c = c0 + ((int)threadIdx.x - j * (int)lanes.d) * N;
+    const long long s = ((long long)blockIdx.x * groups + j) * kPiece;
+    const bool on = j < groups && s < n && c < width;
+    unsigned cur = 0;
+    if (on) {
+        const long long e = s + kPiece < n ? s + kPiece : n;
+        constexpr int kAhead = 8;
+        unsigned k[kAhead], from[kAhead];
+        auto ahead = [&](long long b) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    unsigned cur = keys[s];
-    bool open = s > 0 && keys[s - 1] == cur;       // this sum began in an earlier piece
-    auto flush = [&](bool goes_on) {
-        if (cur >= rows) return;
-        if (open || goes_on) {
-            float* o = part + (2ll * g + (open ? 0 : 1)) * part_ld + c;
-#pragma unroll
-            for (int k = 0; k < N; k += 4) {
-                if constexpr (N >= 4) *(Vec<float, 4>*)(o + k) = Vec<float, 4>{{acc[k], acc[k + 1], acc[k + 2], acc[k + 3]}};
-                else o[k] = acc[k];
+            for (int q = 0; q < kAhead; ++q) {
+                k[q] = b + q < e ? keys[b + q] : (unsigned)rows;
+                from[q] = b + q < e ? at[b + q] : 0;
             }
+        };
+        ahead(s);
+        const unsigned before = s > 0 ? keys[s - 1] : ~0u, after = e < n ? keys[e] : ~0u;
+        float acc[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc[q] = 0.f;
+        cur = k[0];
+        bool open = before == cur && cur < rows;           // this sum began in an earlier piece
+        unsigned char is = open ? 1 : 0;
+        auto flush = [&](bool goes_on) {
+            if (cur >= rows) return;
+            if (open) {
+#pragma unroll
+                for (int q = 0; q < N; ++q) head[q][threadIdx.x] = acc[q];
+                if (goes_on) is |= 2;
+            } else if (goes_on) {
+#pragma unroll
+                for (int q = 0; q < N; ++q) tail[q][threadIdx.x] = acc[q];
+                is |= 4;
+            } else {
+                float v[N];
+#pragma unroll
+                for (int q = 0; q < N; ++q) v[q] = acc[q] * scale;
+                store_row<T, N>(dt + (long long)cur * ldt + c, width - c, v);
+            }
+        };
+#pragma unroll 1
+        for (long long b = s; b < e; b += kAhead) {
+            Loose<T, N> v[kAhead];
+            unsigned now[kAhead];
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                now[q] = k[q];
+                if (now[q] < rows) v[q] = raw_row<T, N>(dy + (long long)from[q] * lddy + c, width - c);
+            }
+            if (kPiece > kAhead && b + kAhead < e) ahead(b + kAhead);
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                if (b + q >= e) break;
+                if (now[q] != cur) {
+                    flush(false);
+                    cur = now[q];
+                    open = false;
+#pragma unroll
+                    for (int t = 0; t < N; ++t) acc[t] = 0.f;
+                }
+                if (cur < rows) {
+#pragma unroll
+                    for (int t = 0; t < N; ++t) acc[t] += (float)v[q].v[t];
+                }
+            }
+        }
+        flush(after == cur);
+        kind[j] = is;                                      // (every lane of the group writes the same)
+    }
+    __syncthreads();
+    if (!on) return;
+    // head[j] <- what the pieces from j on add to a sum that is open in front of j: a scan from behind, in steps of 1, 2, 4 ... groups (one by one, 128
+    // groups of two lanes took 16 us)
+    const int live = (int)(((n - (long long)blockIdx.x * groups * kPiece) + kPiece - 1) / kPiece), end = live < groups ? live : groups;
+    for (int d = 1; d < end; d <<= 1) {
+        const bool more = on && j + d < end && (kind[j] & 2);
+        float a[N];
+        unsigned char is = 0;
+        if (more) {
+            is = kind[j + d];
+#pragma unroll
+            for (int q = 0; q < N; ++q) a[q] = head[q][threadIdx.x + d * (int)lanes.d];
+        }
+        __syncthreads();
+        if (more) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) head[q][threadIdx.x] += a[q];
+            if (!(is & 2)) kind[j] &= 5;                   // (every lane of the group writes the same)
+        }
+        __syncthreads();
+    }
+    if (!on) return;
+    if (kind[j] & 4) {                                     // the group's tail and what follows it
+        float a[N];
+        const bool inside = j + 1 < end, closed = inside && !(kind[j + 1] & 2);
+#pragma unroll
+        for (int q = 0; q < N; ++q) a[q] = tail[q][threadIdx.x] + (inside ? head[q][threadIdx.x + (int)lanes.d] : 0.f);
+        if (closed) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) a[q] *= scale;
+            store_row<T, N>(dt + (long long)cur * ldt + c, width - c, a);
         } else {
-            float v[N];
+            float* o = part + (2ll * blockIdx.x + 1) * part_ld + c;
 #pragma unroll
-            for (int k = 0; k < N; ++k) v[k] = acc[k] * scale;
-            store_row<T, N>(dt + (long long)cur * ldt + c, width - c, v);
-        }
-    };
-    constexpr int kAhead = 8;
-    for (long long b = s; b < e; b += kAhead) {
-        unsigned k[kAhead];
-        float v[kAhead][N];
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q) k[q] = b + q < e ? keys[b + q] : (unsigned)rows;
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            const long long i = b + q < e ? at[b + q] : 0;
-            if (k[q] < rows) load_row<T, N>(dy + i * lddy + c, width - c, v[q]);
-        }
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            if (b + q >= e) break;
-            if (k[q] != cur) {
-                flush(false);
-                cur = k[q];
-                open = false;
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] = 0.f;
-            }
-            if (cur < rows) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] += v[q][j];
-            }
+            for (int q = 0; q < N; q += 4) *(Vec<float, 4>*)(o + q) = Vec<float, 4>{{a[q], a[q + 1], a[q + 2], a[q + 3]}};
+            if (c == 0) list[1 + atomicAdd(list, 1u)] = blockIdx.x;      // (the order of the list does not matter: each of its sums is complete by itself)
         }
     }
-    flush(e < n && keys[e] == cur);
+    if (j == 0 && (kind[0] & 1)) {                         // the workgroup's head
+        float* o = part + 2ll * blockIdx.x * part_ld + c;
+#pragma unroll
+        for (int q = 0; q < N; q += 4)
+            *(Vec<float, 4>*)(o + q) = Vec<float, 4>{{head[q][threadIdx.x], head[q + 1][threadIdx.x], head[q + 2][threadIdx.x], head[q + 3][threadIdx.x]}};
+    }
 }
-// One workgroup per piece: the sum that starts in it and leaves it, if there is one = tail of the piece + heads of the following ones.  The lanes
-// take four columns each and share the heads between them; their sums are added in order.
+// The listed workgroups: the sum that leaves one = its tail + the heads of the following ones, as far as they begin with the same key.  A
+// workgroup takes 256 columns of one at a time; four columns a lane, the heads shared between the slices of lanes, whose sums are added in a
+// fixed order.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const unsigned* keys, long long n, long long rows, int width, float scale, T* dt, long long ldt, const float* part,
-                                                   long long part_ld) {
-    const long long g = blockIdx.x, s = g * kPiece, e = s + kPiece;
-    if (e >= n) return;
-    const unsigned k = keys[e - 1];
-    if (k >= rows || keys[e] != k) return;
-    if (keys[s] == k && s > 0 && keys[s - 1] == k) return;         // it began earlier
-    long long lo = e + 1, hi = n;                                  // the first token behind the sum
-    bool near = true;
-    for (long long step = kPiece; lo < hi; step = near ? 4 * step : step) {            // (most sums are short: look nearby first, then further and further, then between)
-        near = near && lo + step < hi;
-        const long long m = near ? lo + step : (lo + hi) >> 1;
-        if (keys[m] == k) lo = m + 1; else { hi = m; near = false; }
-    }
-    const long long last = (lo - 1) / kPiece;                      // the piece of its last token
+__global__ __launch_bounds__(256) void join_kernel(const unsigned* keys, long long n, int piece, int width, float scale, T* dt, long long ldt, const float* part,
+                                                   long long part_ld, const unsigned* list, int chunks) {
     __shared__ Vec<float, 4> sum[256];
-    const int cols = (width + 3) / 4, wide = cols < 256 ? cols : 256, slices = 256 / wide;
+    const int cols = (width + 3) / 4, wide = cols < 64 ? cols : 64, slices = 256 / wide;
     const int slice = threadIdx.x / wide, lane = threadIdx.x % wide;
-    for (int c0 = 0; c0 < cols; c0 += wide) {
-        const int c = 4 * (c0 + lane);
+    const long long items = (long long)list[0] * chunks;
+    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+        const long long g = list[1 + it / chunks];
+        const unsigned k = keys[(g + 1) * piece];
+        long long last = g;                                        // the piece of its last token
+        for (int more = 256; more == 256; last += more) {
+            const long long i = (last + 1 + threadIdx.x) * piece;
+            more = __syncthreads_count(i < n && keys[i] == k);     // (keys are sorted: the pieces that begin with k are the next ones)
+        }
+        const int c = 4 * ((int)(it % chunks) * 64 + lane);
         float a[4] = {};
         if (slice < slices && c < width) {
             if (slice == 0) {
@@ -257,8 +354,7 @@ __global__ __launch_bounds__(256) void join_kernel(const unsigned* keys, long lo
         __syncthreads();
         sum[threadIdx.x] = Vec<float, 4>{{a[0], a[1], a[2], a[3]}};
         __syncthreads();
-        // halves are added together, slice by slice
-        for (int w = 1; w < slices; w <<= 1) {
+        for (int w = 1; w < slices; w <<= 1) {                     // neighbours are added together
             if (slice < slices && slice % (2 * w) == 0 && slice + w < slices) {
                 const Vec<float, 4> v = sum[threadIdx.x + w * wide];
 #pragma unroll

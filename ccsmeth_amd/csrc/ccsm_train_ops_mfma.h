@@ -85,16 +85,6 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, in
     }
     store_row<T, N>((T*)e.y + i * e.ldy + j, left, z);
 }
-// N elements as they are (the ones behind `left`: zeros)
-template <typename T, int N>
-__device__ __forceinline__ Loose<T, N> raw_row(const T* p, int left) {
-    if (left >= N) return *reinterpret_cast<const Loose<T, N>*>(p);
-    Loose<T, N> t;
-#pragma unroll
-    for (int k = 0; k < N; ++k) t.v[k] = k < left ? p[k] : (T)0.f;
-    return t;
-}
-
 // One operand's side: requests by NW waves (this one is number `wave` of them) for B rows or columns, and the fragments of this wave's W of them
 template <bool TR, int B, int W, int NW>
 struct Side {

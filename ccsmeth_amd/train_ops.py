@@ -66,7 +66,7 @@ def load():
     lib.ccsm_train_linear_backward_workspace.restype = cs
     lib.ccsm_train_linear_backward.argtypes = [ci, vp, vp, cs, vp]
     lib.ccsm_train_embedding_forward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp]
-    lib.ccsm_train_embedding_backward_workspace.argtypes = [cl, cl, C.c_int32]
+    lib.ccsm_train_embedding_backward_workspace.argtypes = [ci, cl, cl, C.c_int32]
     lib.ccsm_train_embedding_backward_workspace.restype = cs
     lib.ccsm_train_embedding_backward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp, cs, vp]
     lib.ccsm_train_act8_pack.argtypes = [ci, ci, ci, cl, C.c_int32, vp, cl, vp, cl, vp, cl, vp]
@@ -119,6 +119,8 @@ def _on_gpu(t, name):
 
 def _rows(t):
     """(2-D view or copy with contiguous rows, its row stride)"""
+    if t.dim() == 2 and t.is_contiguous():
+        return t, t.shape[1]
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1]) if t.dim() else t.reshape(1, 1)
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
@@ -245,7 +247,9 @@ def checkpoint8(x, code="int8", *, stream=None):
     scales = torch.empty((rows, blocks), dtype=torch.uint8, device=dev)
     _check(lib.ccsm_train_act8_pack(dev.index, _TYPE[x.dtype], CODES[code], rows, width, x2.data_ptr(), ldx, codes.data_ptr(), 32 * blocks, scales.data_ptr(), blocks,
                                     _raw_stream(dev)))
-    return Checkpoint8(codes, scales, x.shape, x.dtype, code)
+    c = Checkpoint8.__new__(Checkpoint8)                    # (what __init__ checks holds here)
+    c.codes, c.scales, c.shape, c.dtype, c.code = codes, scales, x.shape, x.dtype, code
+    return c
 
 
 def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=False, *, out=None, stream=None):
@@ -382,7 +386,7 @@ def embedding_backward(dy, ids, rows, scale=1.0, *, out=None, stream=None):
     dt = _torch.empty((rows, width), dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), _torch.Size((rows, width)), t, dev, "out")
     d2, ldd = _rows(dy)
     t2, ldt = _rows(dt)
-    need = lib.ccsm_train_embedding_backward_workspace(i.numel(), rows, width)
+    need = lib.ccsm_train_embedding_backward_workspace(_TYPE[t], i.numel(), rows, width)
     ws = _scratch(need, dev)
     _check(lib.ccsm_train_embedding_backward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), rows, width, d2.data_ptr(), ldd, float(scale), t2.data_ptr(), ldt,
                                              _ptr(ws), need, _raw_stream(dev)))

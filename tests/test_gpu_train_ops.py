@@ -368,6 +368,18 @@ def test_embedding_extremes(t):
     assert torch.equal(ops.embedding(ids, view), ops.embedding(ids, view.contiguous()))
 
 
+@pytest.mark.parametrize("tokens,rows,width", [(131073, 300, 2), (140000, 70000, 1), (524289, 3000, 1), (700001, 5, 3)])
+def test_embedding_many_tokens(tokens, rows, width):
+    """the sort's larger workgroups, and more of them than add the counts up themselves"""
+    for t in (F32, BF16):
+        g = torch.Generator().manual_seed(tokens)
+        ids = (torch.rand(tokens, generator=g) ** 2 * rows).long().clamp_max(rows - 1)
+        ids[::1001] = -7
+        ids = ids.to(torch.int32).to(DEV)
+        table, dy = normal(1, rows, width, t=t), normal(2, tokens, width, t=t, by=0.1)
+        check_embedding(ids, table, dy, 1.5, ops.embedding(ids, table, 1.5), ops.embedding_backward(dy, ids, rows, 1.5), t)
+
+
 # ---- how the calls are used -----------------------------------------------------------------------------------------
 def _step(s, stream=None):
     """tokens -> embedding -> two layers with a residual -> gradients from 8-bit checkpoints -> the table's gradient"""

@@ -46,7 +46,7 @@ def test_linear_null_and_empty():
     assert lib.ccsm_train_linear_forward(0, None, None, 0, None) == INVALID
     assert lib.ccsm_train_linear_forward(0, C.byref(_linear(rows=0, x=None, y=None)), None, 0, None) == 0       # nothing to do: nothing is launched
     assert lib.ccsm_train_linear_workspace(C.byref(_linear(rows=0))) == 0 and lib.ccsm_train_linear_backward_workspace(C.byref(_grad(rows=0))) == 0
-    assert lib.ccsm_train_embedding_backward_workspace(0, 5, 8) == 0
+    assert lib.ccsm_train_embedding_backward_workspace(0, 0, 5, 8) == 0
 
 
 def _grad(**kw):
@@ -78,7 +78,7 @@ def test_too_small_a_workspace_is_refused():
     assert lib.ccsm_train_linear_backward(0, C.byref(p), None, need, None) == CAPACITY
     assert lib.ccsm_train_linear_backward(0, C.byref(p), A, need - 1, None) == CAPACITY
     assert lib.ccsm_train_linear_backward(0, C.byref(p), A + 8, need, None) == INVALID
-    need = lib.ccsm_train_embedding_backward_workspace(1000, 5, 8)
+    need = lib.ccsm_train_embedding_backward_workspace(0, 1000, 5, 8)
     assert need > 0
     args = (0, 0, 1, 1000, A, 5, 8, A, 8, 1.0, A, 8)
     assert lib.ccsm_train_embedding_backward(*args, None, 0, None) == CAPACITY

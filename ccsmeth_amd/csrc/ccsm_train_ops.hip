@@ -39,7 +39,12 @@ struct OnDevice {
     OnDevice on_device_(device);               \
     if (on_device_.err != hipSuccess) return hip_fail(on_device_.err, "hipSetDevice")
 
-constexpr int64_t kFewRows = 64;                   // up to here the few-rows kernel
+// Where direct_kernel takes a product: forward ones of at most 64 rows, and products of at most 2^27 multiplications whose contraction is short, since
+// its steps follow each other without a tile's prefetch.  Measured (bf16 | fp32, us a call, tile way -> direct): 512^3 forward 12.8 -> 11.0 |
+// 24.6 -> 11.5, gradients 40 -> 30 | 66 -> 54; 255^3 forward 19 -> 13 | 22 -> 12, gradients 50 -> 33 | 90 -> 53; beyond: 1024^3 forward
+// 17.7 -> 25.6 | 38 -> 63; 128 x 128 with a contraction of 4096 forward 15.7 -> 21.8, as a gradient 22 -> 75; results of 13377 x 768 (stored in
+// pieces of 16 columns) 26 -> 51.
+constexpr int64_t kFewRows = 64, kSmallProduct = 1 << 27, kSmallResult = 1 << 21, kShortForward = 1024, kShortBackward = 512;
 constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
 
 size_t size_of(int type) { return type == CCSM_TYPE_F32 ? 4 : 2; }
@@ -151,6 +156,17 @@ hipError_t product(hipStream_t st, const Staged& p, const Staged& q, int64_t M, 
 }
 #define TRY(x, what) do { hipError_t e_ = (x); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
 
+bool small_product(int64_t M, int64_t N, int64_t K) { return M * N <= kSmallResult && M * N * K <= kSmallProduct; }
+template <typename T, bool TRP, bool TRQ>
+hipError_t direct(hipStream_t st, const Saved& p, const Saved& z, int act, const Saved& q, int64_t M, int64_t N, int64_t K, void* sums, const Epilogue& ep) {
+    DirectArgs a{p, z, q, act, M, N, K, 1, sums, ep};
+    while (a.kw < 8 && 32 * 2 * a.kw <= K) a.kw *= 2;             // (a wave has a whole step of 32 at least)
+    const int mt = M <= 16 ? 1 : 4;
+    auto* f = mt == 1 ? &direct_kernel<T, TRP, TRQ, 1> : &direct_kernel<T, TRP, TRQ, 4>;
+    f<<<dim3((unsigned)cdiv(N, 16), (unsigned)cdiv(M, 16 * mt * (8 / a.kw))), 512, 0, st>>>(a);
+    return hipGetLastError();
+}
+
 ccsm_status check_linear(const ccsm_linear* p) {
     REFUSE(!p, "linear: NULL argument");
     REFUSE(!good_type(p->type), "linear: unknown type");
@@ -165,11 +181,9 @@ ccsm_status check_linear(const ccsm_linear* p) {
 template <typename T>
 ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bool count) {
     const Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
-    if (p->rows <= kFewRows) {
+    if (p->rows <= kFewRows || (p->inner <= kShortForward && small_product(p->rows, p->outer, p->inner))) {
         if (count) return CCSM_OK;
-        auto* f = p->rows <= 16 ? &few_rows_kernel<T, 1> : p->rows <= 32 ? &few_rows_kernel<T, 2> : &few_rows_kernel<T, 4>;
-        f<<<(unsigned)cdiv(p->outer, 16), 512, 0, st>>>((const T*)p->x, p->ldx, (const T*)p->w, p->ldw, (int)p->rows, p->outer, p->inner, ep);
-        LAUNCHED("linear_forward");
+        TRY((direct<T, false, false>(st, plain(p->x, p->ldx), plain(p->x, p->ldx), CCSM_ACT_NONE, plain(p->w, p->ldw), p->rows, p->outer, p->inner, nullptr, ep)), "linear_forward");
         return CCSM_OK;
     }
     const Staged x = staged<T>(plain(p->x, p->ldx), p->rows, p->inner, ws, st, count), w = staged<T>(plain(p->w, p->ldw), p->outer, p->inner, ws, st, count);
@@ -211,6 +225,15 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         LAUNCHED("linear_backward");
         return CCSM_OK;
     }
+    const Epilogue to_dx{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, to_dw{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone};
+    if (M <= kShortBackward && N <= kShortBackward && small_product(M, N, K)) {
+        if (count) return CCSM_OK;
+        const Saved dy = plain(p->dy, p->lddy), z = p->activation == CCSM_ACT_NONE ? dy : saved_of(p->preact);
+        if (p->dx) TRY((direct<T, false, true>(st, dy, z, p->activation, plain(p->w, p->ldw), M, K, N, nullptr, to_dx)), "linear_backward: dx");
+        if (p->dw || p->dbias)                                     // (the bias gradient comes with dw's product, or by the same sums without it)
+            TRY((direct<T, true, true>(st, dy, z, p->activation, p->dw ? saved_of(p->x) : dy, N, p->dw ? K : 1, M, p->dbias, to_dw)), "linear_backward: dw");
+        return CCSM_OK;
+    }
     // d as the products take it: dy itself where there is no activation, the type is a 16-bit one and its rows are whole pieces
     const bool products = p->dx || p->dw;
     const Saved dy = plain(p->dy, p->lddy);
@@ -228,11 +251,11 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
     }
     if (p->dx) {
         const Staged w = staged<T>(plain(p->w, p->ldw), N, K, ws, st, count);
-        TRY((product<T, false, true>(st, d, w, M, K, N, Epilogue{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, ws, count)), "linear_backward: dx");
+        TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, count)), "linear_backward: dx");
     }
     if (p->dw) {
         const Staged x = staged<T>(saved_of(p->x), M, K, ws, st, count);
-        TRY((product<T, true, true>(st, d, x, N, K, M, Epilogue{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone}, ws, count)), "linear_backward: dw");
+        TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, count)), "linear_backward: dw");
     }
     return CCSM_OK;
 }

@@ -453,28 +453,38 @@ __global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, 
     part[(long long)blockIdx.x * N + n] = a;
 }
 
-// ---- few rows -------------------------------------------------------------------------------------------------------
-// y = act(x w^T + bias) + residual for up to 16 MT rows of x: bound by reading w once.  A workgroup takes 16 rows of w, its eight waves every eighth
-// 32 columns of them, eight pieces in flight; a piece goes from memory straight into the matrix instruction's operand (lane = row, 8 columns; any
-// alignment), x likewise (out of the caches).  The waves' sums are added in order through LDS.  fp32: the three bf16 parts of each operand are made
-// in registers.  At 1 x 512 x 768 bf16 the tile kernel took 9.8 us: four steps through four LDS stages by six of 256 CUs.
-template <typename T, int MT>
-__global__ __launch_bounds__(512) void few_rows_kernel(const T* x, long long ldx, const T* w, long long ldw, int M, int N, int K, Epilogue ep) {
+// ---- small products and few rows ------------------------------------------------------------------------------------
+// The same products straight from memory into the matrix instructions' operands, without staging, LDS or a kernel in front: any type, alignment and
+// storage form, checkpoints and an activation's slope included.  A wave owns 16 j x 16 MT i; a workgroup's eight waves share the contraction (kw of
+// them) and the i between them; their sums are added in order through LDS.  fp32: the three bf16 parts of each operand are made in
+// registers.
+// For up to 64 rows it is bound by reading w once (1 x 512 x 768 bf16: 3.8 us; the tile kernel 9.8, four steps through LDS by six of 256 CUs); for
+// small products by its one launch (the tile kernel's way takes up to three for a product and eight for a backward pass).
+struct DirectArgs {
+    Saved P, Z, Q;                // Z, act: P's elements are multiplied by act'(Z)
+    int act;
+    long long M, N, K;
+    int kw;                       // waves along k: 1, 2, 4 or 8
+    void* sums;                   // NULL, or (M): the sum over k of P(i, k), before its rounding
+    Epilogue ep;                  // y NULL: the sums alone
+};
+template <typename T, bool TRP, bool TRQ, int MT>
+__global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
     typedef typename std::conditional<sizeof(T) == 4, b16, T>::type E;
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, U = 4;
+    constexpr bool fast = sizeof(T) == 2;
     __shared__ f32x4 sum[8][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n0 = blockIdx.x * 16, n = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
-    const T* wr = w + n * ldw;
-    const T* xr[MT];
+    __shared__ float total[8][MT][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave & (a.kw - 1), wm = wave / a.kw, mw = 8 / a.kw;
+    const long long j0 = (long long)blockIdx.x * 16, i0 = ((long long)blockIdx.y * mw + wm) * (16 * MT);
+    const long long j = j0 + (lane & 15) < a.N ? j0 + (lane & 15) : a.N - 1;
+    long long i[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = 16 * t + (lane & 15);
-        xr[t] = x + (m < M ? m : M - 1) * ldx;
-    }
+    for (int t = 0; t < MT; ++t) i[t] = i0 + 16 * t + (lane & 15) < a.M ? i0 + 16 * t + (lane & 15) : a.M - 1;
     f32x4 acc[MT];
+    float tot[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < MT; ++t) { acc[t] = f32x4{0.f, 0.f, 0.f, 0.f}; tot[t] = 0.f; }
     auto pieces = [](const Loose<T, 8>& v, s16x8 (&p)[NP]) {
         if constexpr (NP == 1) p[0] = __builtin_bit_cast(s16x8, v);
         else {
@@ -487,57 +497,118 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const T* x, long long ldx
             }
         }
     };
-    auto multiply = [&](const Loose<T, 8>& wv, const Loose<T, 8> (&xv)[MT]) {
-        s16x8 a[NP], b[NP];
-        pieces(wv, a);
+    // eight neighbours along k of one row (TR: column) of a kept matrix, zeros behind its end
+    auto eight = [&](const Saved& s, bool tr, long long r, long long k) -> Loose<T, 8> {
+        const int left = (int)(a.K - k < 8 ? a.K - k : 8);
+        if (s.code == kCodeNone) {
+            if (!tr) return raw_row<T, 8>((const T*)s.data + r * s.ld + k, left);
+            Loose<T, 8> o;
+            const T* p = (const T*)s.data + k * s.ld + r;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            pieces(xv[t], b);
-            if constexpr (NP == 3) {
-                acc[t] = Mfma<E>::run(a[2], b[0], acc[t]);
-                acc[t] = Mfma<E>::run(a[0], b[2], acc[t]);
-                acc[t] = Mfma<E>::run(a[1], b[1], acc[t]);
-                acc[t] = Mfma<E>::run(a[1], b[0], acc[t]);
-                acc[t] = Mfma<E>::run(a[0], b[1], acc[t]);
-            }
-            acc[t] = Mfma<E>::run(a[0], b[0], acc[t]);
+            for (int q = 0; q < 8; ++q) o.v[q] = q < left ? p[q * s.ld] : (T)0.f;
+            return o;
+        }
+        Loose<T, 8> o;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) o.v[q] = q < left ? (T)saved_at<T>(s, tr ? k + q : r, tr ? r : k + q) : (T)0.f;
+        return o;
+    };
+    auto sloped = [&](Loose<T, 8>& v, const Loose<T, 8>& z, float& t) {
+        float u[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) u[q] = (float)z.v[q];
+        slope_all<fast, 8>(u, a.act);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float d = (float)v.v[q] * u[q];
+            t += d;
+            v.v[q] = (T)d;
         }
     };
-    int k = wave * 32 + 8 * (lane >> 4);
-    const int whole = K & ~255;                                   // all eight waves have whole pieces up to here
-    int k0 = 0;
-    for (; k0 + 256 * U <= whole; k0 += 256 * U, k += 256 * U) {
-        Loose<T, 8> wv[U], xv[U][MT];
+    auto multiply = [&](const Loose<T, 8>& qv, const Loose<T, 8> (&pv)[MT]) {
+        s16x8 x[NP], y[NP];
+        pieces(qv, x);
 #pragma unroll
-        for (int u = 0; u < U; ++u) wv[u] = *reinterpret_cast<const Loose<T, 8>*>(wr + k + 256 * u);
+        for (int t = 0; t < MT; ++t) {
+            pieces(pv[t], y);
+            if constexpr (NP == 3) {
+                acc[t] = Mfma<E>::run(x[2], y[0], acc[t]);
+                acc[t] = Mfma<E>::run(x[0], y[2], acc[t]);
+                acc[t] = Mfma<E>::run(x[1], y[1], acc[t]);
+                acc[t] = Mfma<E>::run(x[1], y[0], acc[t]);
+                acc[t] = Mfma<E>::run(x[0], y[1], acc[t]);
+            }
+            acc[t] = Mfma<E>::run(x[0], y[0], acc[t]);
+        }
+    };
+    const bool slope = a.act != kActNone, want = a.sums != nullptr && blockIdx.x == 0;
+    const int step = 32 * a.kw;
+    long long k0 = 0, k = wk * 32 + 8 * (lane >> 4);
+    if (!TRP && !TRQ && !slope && a.P.code == kCodeNone && a.Q.code == kCodeNone) {       // four steps of whole pieces in flight
+        for (; k0 + step * U <= a.K; k0 += step * U, k += step * U) {
+            Loose<T, 8> qv[U], pv[U][MT];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) qv[u] = *reinterpret_cast<const Loose<T, 8>*>((const T*)a.Q.data + j * a.Q.ld + k + step * u);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xv[u][t] = *reinterpret_cast<const Loose<T, 8>*>(xr[t] + k + 256 * u);
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int u = 0; u < U; ++u) multiply(wv[u], xv[u]);
+                for (int t = 0; t < MT; ++t) pv[u][t] = *reinterpret_cast<const Loose<T, 8>*>((const T*)a.P.data + i[t] * a.P.ld + k + step * u);
+#pragma unroll
+            for (int u = 0; u < U; ++u) multiply(qv[u], pv[u]);
+        }
     }
-    for (; k0 < K; k0 += 256, k += 256) {
-        Loose<T, 8> wv, xv[MT];
-        wv = raw_row<T, 8>(wr + k, K - k);
+    for (; k0 < a.K; k0 += step, k += step) {
+        Loose<T, 8> pv[MT], zv[MT];
+        Loose<T, 8> qv = {};
+        if (a.ep.y) qv = eight(a.Q, TRQ, j, k);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) xv[t] = raw_row<T, 8>(xr[t] + k, K - k);
-        multiply(wv, xv);
+        for (int t = 0; t < MT; ++t) pv[t] = eight(a.P, TRP, i[t], k);
+        if (slope) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) zv[t] = eight(a.Z, TRP, i[t], k);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) sloped(pv[t], zv[t], tot[t]);
+        } else if (want) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) tot[t] += (float)pv[t].v[q];
+        }
+        multiply(qv, pv);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) sum[wave][t][lane] = acc[t];
-    __syncthreads();
-    if ((int)threadIdx.x >= 64 * MT) return;
-    const int t = wave, m = 16 * t + (lane & 15), j = n0 + 4 * (lane >> 4);
-    if (m >= M || j >= N) return;
-    f32x4 v = sum[0][t][lane];
+    if (want) {
 #pragma unroll
-    for (int q = 1; q < 8; ++q) v += sum[q][t][lane];
-    float z[4] = {v[0], v[1], v[2], v[3]}, bias[4];
-    Loose<T, 4> r;
-    if (ep.bias) load_row<T, 4>((const T*)ep.bias + j, N - j, bias);
-    if (ep.residual) r = raw_row<T, 4>((const T*)ep.residual + m * ep.ldr + j, N - j);
-    finish<T, 4>(ep, m, j, N - j, z, bias, r);
+        for (int t = 0; t < MT; ++t) {
+            tot[t] += __shfl_xor(tot[t], 16);
+            tot[t] += __shfl_xor(tot[t], 32);
+            if (lane < 16) total[wave][t][lane] = tot[t];
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < mw * MT * 64; e += 512) {
+        const int l = e & 63, t = (e >> 6) % MT, w = (e >> 6) / MT;
+        const long long m = ((long long)blockIdx.y * mw + w) * (16 * MT) + 16 * t + (l & 15), n = j0 + 4 * (l >> 4);
+        if (m >= a.M || n >= a.N || !a.ep.y) continue;
+        const int left = (int)(a.N - n < 4 ? a.N - n : 4);
+        f32x4 v = sum[w * a.kw][t][l];
+        for (int q = 1; q < a.kw; ++q) v += sum[w * a.kw + q][t][l];
+        float z[4] = {v[0], v[1], v[2], v[3]}, bias[4];
+        Loose<T, 4> r;
+        if (a.ep.bias) load_row<T, 4>((const T*)a.ep.bias + n, left, bias);
+        if (a.ep.residual) r = raw_row<T, 4>((const T*)a.ep.residual + m * a.ep.ldr + n, left);
+        finish<T, 4>(a.ep, m, (int)n, left, z, bias, r);
+    }
+    if (want)
+        for (int e = threadIdx.x; e < mw * MT * 16; e += 512) {
+            const int l = e & 15, t = (e >> 4) % MT, w = (e >> 4) / MT;
+            const long long m = ((long long)blockIdx.y * mw + w) * (16 * MT) + 16 * t + l;
+            if (m >= a.M) continue;
+            float v = total[w * a.kw][t][l];
+            for (int q = 1; q < a.kw; ++q) v += total[w * a.kw + q][t][l];
+            ((T*)a.sums)[m] = (T)v;
+        }
 }
 
 }  // namespace ccsm_ops

@@ -72,7 +72,7 @@ def test_linear_backward_refuses(kw):
 
 def test_too_small_a_workspace_is_refused():
     lib = ops.load()
-    p = _grad()
+    p = _grad(rows=1 << 16)
     need = lib.ccsm_train_linear_backward_workspace(C.byref(p))
     assert need > 0
     assert lib.ccsm_train_linear_backward(0, C.byref(p), None, need, None) == CAPACITY

@@ -24,6 +24,7 @@ constexpr int rocblas_status_success = 0, rocblas_status_internal_error = 6;
 #include <vector>
 
 #include "../../include/ccsm_train.h"
+#include "../../include/ccsm_train_ops.h"
 #include "ccsm_train_gemm.hip"
 
 // Where a matrix product of the step runs.  The product library: ccsm_train_gemm.hip, the library's three-pass split-fp16 MFMA kernel, for
@@ -427,6 +428,11 @@ struct ccsm_trainer {
     float* out[L] = {nullptr, nullptr, nullptr};
     float* xdrop[L] = {nullptr, nullptr, nullptr};     // dropout(out[l]) = input of layer l + 1 (rate > 0 only)
     float* sav[L][2][4];
+    // activation_bits 8: the four gate arrays of every layer and direction are kept as int8 checkpoints (ccsm_train_act8_pack behind a direction's
+    // forward, _unpack in front of its backward); the layers then share one set of fp32 arrays for each direction (sav[l] = sav[0])
+    int act_bits = 32;
+    uint8_t* codes[L][2][4];
+    uint8_t* scales[L][2][4];
     float *gi[2] = {nullptr, nullptr}, *gh[2] = {nullptr, nullptr}, *dgi[2] = {nullptr, nullptr}, *dgh[2] = {nullptr, nullptr},
           *carry[2] = {nullptr, nullptr}, *cpart[2] = {nullptr, nullptr};            // per direction
     float *hn = nullptr, *q = nullptr, *KS = nullptr, *e = nullptr, *a = nullptr, *c = nullptr, *feat = nullptr, *logits = nullptr,
@@ -568,6 +574,20 @@ ccsm_status join(ccsm_trainer* t) {
     return CCSM_OK;
 }
 
+// the gates of one layer and direction into their checkpoints, or out of them again
+ccsm_status keep_gates(ccsm_trainer* t, int M, int l, int d, bool back) {
+    if (t->act_bits != 8) return CCSM_OK;
+    hipStream_t st = d == 0 ? t->stream : t->stream1;
+    for (int k = 0; k < 4; ++k) {
+        const ccsm_saved s{t->codes[l][d][k], H, CCSM_CODE_INT8, t->scales[l][d][k], H / 32};
+        const ccsm_status e = back ? ccsm_train_act8_unpack(t->device, CCSM_TYPE_F32, (int64_t)T * M, H, &s, t->sav[l][d][k], H, st)
+                                   : ccsm_train_act8_pack(t->device, CCSM_TYPE_F32, CCSM_CODE_INT8, (int64_t)T * M, H, t->sav[l][d][k], H, t->codes[l][d][k], H, t->scales[l][d][k],
+                                                          H / 32, st);
+        if (e != CCSM_OK) return fail(e, std::string("the gates' checkpoints: ") + ccsm_train_ops_last_error());
+    }
+    return CCSM_OK;
+}
+
 ccsm_status forward_dir(ccsm_trainer* t, int M, int l, int d, const float* X, int in, bool train) {
     const float* P = t->params;
     blas_t blas = d == 0 ? t->blas : t->blas1;
@@ -578,7 +598,7 @@ ccsm_status forward_dir(ccsm_trainer* t, int M, int l, int d, const float* X, in
                                                                P + kOff.b_ih[l][d], P + kOff.b_hh[l][d], t->out[l] + d * H, t->sav[l][d][0], t->sav[l][d][1],
                                                                t->sav[l][d][2], t->sav[l][d][3], M, d, train ? 1 : 0);
         HIPCHK(hipGetLastError());
-        return CCSM_OK;
+        return train ? keep_gates(t, M, l, d, false) : CCSM_OK;
     }
     for (int s = 0; s < T; ++s) {
         const int tt = d == 0 ? s : T - 1 - s;
@@ -592,7 +612,7 @@ ccsm_status forward_dir(ccsm_trainer* t, int M, int l, int d, const float* X, in
                                                                    hprev, ld, t->out[l] + (size_t)tt * M * H2 + d * H, t->sav[l][d][0] + so,
                                                                    t->sav[l][d][1] + so, t->sav[l][d][2] + so, t->sav[l][d][3] + so, M, train ? 1 : 0);
     }
-    return CCSM_OK;
+    return train ? keep_gates(t, M, l, d, false) : CCSM_OK;
 }
 
 ccsm_status forward(ccsm_trainer* t, int N, bool train, float rate, bool have_labels) {
@@ -648,6 +668,7 @@ ccsm_status backward_dir(ccsm_trainer* t, int M, int l, int d, const float* dO, 
     const bool own_atb = t->gctx[0].mode == 1;
     const int sp20 = t->sp20 ? t->sp20 : own_atb ? 1 : (M <= 2048 ? 2 : 4), sp21 = t->sp21 ? t->sp21 : own_atb ? 1 : 3;
     float* cpart = t->cpart[d];
+    { const ccsm_status e = keep_gates(t, M, l, d, true); if (e != CCSM_OK) return e; }
     if (!t->stepwise_bwd_for(M)) {     // all 21 steps in one launch (ccsm_train_seq.hip)
         gru_seq_bwd_kernel<<<(M + 31) / 32, 512, kSbLds, st>>>(dO + d * H, t->out[l] + d * H, t->h0 + (size_t)(2 * l + d) * M * H,
                                                                t->whh_t_frag + (size_t)(2 * l + d) * kSqFragPerDir, t->sav[l][d][0], t->sav[l][d][1],
@@ -779,13 +800,21 @@ int ccsm_train_param_offsets(int64_t* offsets, int n) {
 }
 
 ccsm_status ccsm_train_create(const ccsm_weights* w, int device, int max_sites, float* d_grads, ccsm_trainer** out) {
+    return ccsm_train_create_act(w, device, max_sites, d_grads, 32, out);
+}
+ccsm_status ccsm_train_create_act(const ccsm_weights* w, int device, int max_sites, float* d_grads, int activation_bits, ccsm_trainer** out) {
     if (!w || !out || max_sites <= 0) return fail(CCSM_ERR_INVALID_ARG, "weights, out must be non-NULL and max_sites > 0");
+    if (activation_bits != 32 && activation_bits != 8) return fail(CCSM_ERR_INVALID_ARG, "activation_bits must be 32 or 8");
     *out = nullptr;
     HIPCHK(hipSetDevice(device));
     ccsm_trainer* t = new ccsm_trainer();
     t->device = device;
     t->max_sites = max_sites;
+    t->act_bits = activation_bits;
     const size_t M = 2 * (size_t)max_sites;
+    for (int l = 0; l < L; ++l)
+        for (int d = 0; d < 2; ++d)
+            for (int k = 0; k < 4; ++k) { t->sav[l][d][k] = nullptr; t->codes[l][d][k] = t->scales[l][d][k] = nullptr; }
 #define TRY(x) do { ccsm_status s__ = (x); if (s__ != CCSM_OK) { ccsm_train_destroy(t); return s__; } } while (0)
     HIPCHK(hipStreamCreate(&t->stream));
     HIPCHK(hipStreamCreate(&t->stream1));
@@ -832,7 +861,11 @@ ccsm_status ccsm_train_create(const ccsm_weights* w, int device, int max_sites, 
         TRY(dalloc(&t->out[l], T * M * H2 + 32 * H2));
         if (l + 1 < L) TRY(dalloc(&t->xdrop[l], T * M * H2));
         for (int d = 0; d < 2; ++d)
-            for (int k = 0; k < 4; ++k) { t->sav[l][d][k] = nullptr; TRY(dalloc(&t->sav[l][d][k], T * M * H + 32 * H)); }
+            for (int k = 0; k < 4; ++k) {
+                if (l == 0 || t->act_bits != 8) TRY(dalloc(&t->sav[l][d][k], T * M * H + 32 * H));
+                else t->sav[l][d][k] = t->sav[0][d][k];
+                if (t->act_bits == 8) { TRY(dalloc(&t->codes[l][d][k], T * M * H)); TRY(dalloc(&t->scales[l][d][k], T * M * (H / 32))); }
+            }
     }
     for (int d = 0; d < 2; ++d) {
         TRY(dalloc(&t->gi[d], T * M * G + 32 * G));     // + 32 rows of slack: gru_seq_fwd_kernel reads whole 32-row tiles
@@ -897,7 +930,11 @@ void ccsm_train_destroy(ccsm_trainer* t) {
         if (t->out[l]) (void)hipFree(t->out[l]);
         if (t->xdrop[l]) (void)hipFree(t->xdrop[l]);
         for (int d = 0; d < 2; ++d)
-            for (int k = 0; k < 4; ++k) if (t->sav[l][d][k]) (void)hipFree(t->sav[l][d][k]);
+            for (int k = 0; k < 4; ++k) {
+                if (t->sav[l][d][k] && (l == 0 || t->act_bits != 8)) (void)hipFree(t->sav[l][d][k]);
+                if (t->codes[l][d][k]) (void)hipFree(t->codes[l][d][k]);
+                if (t->scales[l][d][k]) (void)hipFree(t->scales[l][d][k]);
+            }
     }
 #ifdef CCSM_TRAIN_WITH_ROCBLAS
     for (int k = 0; k < 2; ++k)

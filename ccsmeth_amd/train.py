@@ -17,7 +17,7 @@ from . import _lib
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CCSM_TRAIN_LIB_PATH") or os.path.join(_HERE, "lib", "libccsm_train.so")   # the variable: A/B builds (tools/)
-EXPORTS = ("ccsm_train_last_error", "ccsm_train_num_params", "ccsm_train_param_offsets", "ccsm_train_create", "ccsm_train_destroy",
+EXPORTS = ("ccsm_train_last_error", "ccsm_train_num_params", "ccsm_train_param_offsets", "ccsm_train_create", "ccsm_train_create_act", "ccsm_train_destroy",
            "ccsm_train_forward_backward", "ccsm_train_eval", "ccsm_train_step", "ccsm_train_grad_ptr", "ccsm_train_get_params",
            "ccsm_train_set_params", "ccsm_train_get_grads", "ccsm_train_fused_fallbacks", "ccsm_train_selftest_gemm")
 
@@ -52,6 +52,7 @@ def load():
     lib.ccsm_train_num_params.restype = C.c_int64
     lib.ccsm_train_param_offsets.argtypes = [vp, ci]
     lib.ccsm_train_create.argtypes = [C.POINTER(_lib.Weights), ci, ci, vp, C.POINTER(vp)]
+    lib.ccsm_train_create_act.argtypes = [C.POINTER(_lib.Weights), ci, ci, vp, ci, C.POINTER(vp)]
     lib.ccsm_train_destroy.argtypes = [vp]
     lib.ccsm_train_destroy.restype = None
     lib.ccsm_train_forward_backward.argtypes = [vp, ci, C.POINTER(_lib.Batch), vp, C.POINTER(_lib.H0), cf, cf, C.c_uint64, C.POINTER(cf), vp]
@@ -85,9 +86,10 @@ def _f32(a):
 
 class Trainer:
     """One ccsm_trainer: parameters, Adam moments and activation buffers for batches of up to max_sites sites on `device`.
-    grads_tensor: optional torch CUDA float32 tensor of num_params elements that receives the gradients (for all_reduce)."""
+    grads_tensor: optional torch CUDA float32 tensor of num_params elements that receives the gradients (for all_reduce).
+    activation_bits: 32, or 8 to keep the GRU gates as int8 checkpoints between forward and backward (include/ccsm_train.h)."""
 
-    def __init__(self, state_dict, device=0, max_sites=512, grads_tensor=None):
+    def __init__(self, state_dict, device=0, max_sites=512, grads_tensor=None, activation_bits=32):
         self._lib = load()
         sd = {}
         for k, v in state_dict.items():
@@ -119,8 +121,8 @@ class Trainer:
                 raise ValueError("grads_tensor must be a CUDA float32 tensor of %d elements" % self.num_params)
             gptr = grads_tensor.data_ptr()
         self.handle = C.c_void_p()
-        _check(self._lib.ccsm_train_create(C.byref(w), int(device), int(max_sites), gptr, C.byref(self.handle)))
-        self.device, self.max_sites = int(device), int(max_sites)
+        _check(self._lib.ccsm_train_create_act(C.byref(w), int(device), int(max_sites), gptr, int(activation_bits), C.byref(self.handle)))
+        self.device, self.max_sites, self.activation_bits = int(device), int(max_sites), int(activation_bits)
 
     def close(self):
         if self.handle:

@@ -65,6 +65,8 @@ def build_parser():
     p.add_argument('--dist-url', dest="dist_url", type=str, default="tcp://127.0.0.1:12315")
     p.add_argument('--node_rank', type=int, default=0)
     p.add_argument('--epoch_sync', action="store_true", default=False)
+    p.add_argument('--activation_bits', type=int, default=32, choices=(32, 8),
+                   help="what the forward pass keeps of the GRU gates: fp32, or int8 checkpoints (a fifth less memory per site; not a flag of the reference)")
     return p
 
 
@@ -265,7 +267,7 @@ def train(args, log=sys.stderr):
     if world > 1:
         dist.barrier()
     grads = torch.zeros(3043114, dtype=torch.float32, device="cuda:%d" % local_rank)
-    trainer = Trainer(sd, device=local_rank, max_sites=args.batch_size, grads_tensor=grads)
+    trainer = Trainer(sd, device=local_rank, max_sites=args.batch_size, grads_tensor=grads, activation_bits=args.activation_bits)
     train_data, valid_data = read_feature_file(args.train_file), read_feature_file(args.valid_file)
     n_train, n_valid = len(train_data["labels"]), len(valid_data["labels"])
     sched = StepLR(args.lr, args.lr_decay_step, args.lr_decay) if args.lr_scheduler == "StepLR" else \

@@ -36,6 +36,11 @@ int ccsm_train_param_offsets(int64_t* offsets, int n);
  * state.  w = host fp32 tensors (ccsm.h).  max_sites = largest batch.  d_grads = device pointer to a flat fp32 buffer of
  * ccsm_train_num_params() values that receives the gradients, or NULL to let the trainer own one. */
 ccsm_status ccsm_train_create(const ccsm_weights* w, int device, int max_sites, float* d_grads, ccsm_trainer** out);
+/* The same with the width of what the forward pass keeps of the GRU gates (r, z, n, W_hn h + b_hn of every layer, direction and step: two fifths
+ * of a trainer's memory).  32: fp32, as above.  8: int8 checkpoints (ccsm_train_ops.h: blocks of 32 units of a row share a power of two), taken
+ * out again one layer and direction at a time; the forward pass is the same, gradients carry the checkpoints' rounding (half a step of
+ * 2^-6 .. 2^-7 of a block's largest gate). */
+ccsm_status ccsm_train_create_act(const ccsm_weights* w, int device, int max_sites, float* d_grads, int activation_bits, ccsm_trainer** out);
 void ccsm_train_destroy(ccsm_trainer* t);
 
 /* One forward + backward of a batch in HOST memory.  labels: (N) 0/1.  h0: as ccsm_forward_host (EXPLICIT / ZERO /

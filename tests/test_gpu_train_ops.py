@@ -503,3 +503,49 @@ def test_refusals_on_the_gpu():
                  lambda: ops.checkpoint8(x.double()), lambda: ops.checkpoint8(x).values(torch.float64)):
         with pytest.raises(ValueError):
             call()
+
+
+# ---- the trainer with its gates in 8 bits ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,dropout", [(64, 0.0), (64, 0.5), (512, 0.0), (512, 0.5)])
+def test_trainer_with_gates_in_8_bits(n, dropout):
+    """64 sites: the stepwise kernels, 512: the fused ones.  The forward pass is the same; each of the 21 backward steps multiplies by four gates that are off
+    by 2^-7 at most (half a step of 2^-6: blocks whose largest gate is near 1), with errors that are independent of each other: sqrt(84) 2^-7 /
+    sqrt(3) = 0.041 of a gradient's norm at most, below 2^-4."""
+    import numpy as np
+    from ccsmeth_amd.train import Trainer, PARAM_NAMES
+    from ccsmeth_amd.utils import synth
+    w, sites = synth.synth_weights(5), synth.synth_sites(n, 6)
+    labels = np.random.default_rng(7).integers(0, 2, n)
+    h0 = synth.synth_h0(n, 8)
+    res = []
+    for bits in (32, 8, 8):
+        tr = Trainer(w, device=0, max_sites=n + 3, activation_bits=bits)
+        loss, logits = tr.forward_backward(sites, labels, h0=h0, dropout_rate=dropout, seed=9, want_logits=True)
+        res.append((loss, logits, tr.grads()))
+        norm = tr.step(1e-3)
+        assert np.isfinite(norm)
+        assert np.isfinite(tr.forward_backward(sites, labels, h0=h0, dropout_rate=dropout, seed=9, step=1)[0])
+        tr.close()
+    (la, ga, a), (lb, gb, b), (lc, gc, c) = res
+    assert la == lb == lc and np.array_equal(ga, gb)
+    differ = 0
+    for k in PARAM_NAMES:
+        assert np.array_equal(b[k], c[k])                            # the same bits every time
+        off = np.linalg.norm(b[k].astype(np.float64) - a[k]) / np.linalg.norm(a[k].astype(np.float64))
+        assert off <= 2.0 ** -4, (k, off)
+        differ += off > 0
+    assert differ > 20                                               # (the checkpoints are what the gradients are computed from)
+
+
+def test_trainer_with_gates_in_8_bits_takes_less_memory():
+    from ccsmeth_amd.train import Trainer
+    from ccsmeth_amd.utils import synth
+    w, n, took = synth.synth_weights(5), 2048, []
+    for bits in (32, 8):
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        tr = Trainer(w, device=0, max_sites=n, activation_bits=bits)
+        took.append(before - torch.cuda.mem_get_info()[0])
+        tr.close()
+    rows = 21 * 2 * n * 256                                          # values of one gate array: 24 arrays in fp32 against 8, and 24 of 33 / 32 bytes
+    assert abs((took[0] - took[1]) - rows * (16 * 4 - 24 * 33 / 32)) < 64 << 20, took

@@ -142,3 +142,22 @@ def test_checkpoint_tensors_are_checked():
         ops.Checkpoint8(codes, scales, (2, 2, 40), torch.float64, "e4m3")
     with pytest.raises(ValueError):
         ops.Checkpoint8(codes, scales, (2, 2, 40), torch.float16, "fp4")
+
+
+def test_trainm_offers_the_gates_in_8_bits():
+    from ccsmeth_amd import trainm
+    base = ["--train_file", "t", "--valid_file", "v", "--model_dir", "d"]
+    for parser in (trainm.build_parser(), trainm.build_train_parser()):
+        assert parser.parse_args(base).activation_bits == 32
+        assert parser.parse_args(base + ["--activation_bits", "8"]).activation_bits == 8
+        with pytest.raises(SystemExit):
+            parser.parse_args(base + ["--activation_bits", "16"])
+
+
+def test_trainer_refuses_other_widths():
+    from ccsmeth_amd import train
+    lib = train.load()
+    out, w = C.c_void_p(), _lib.Weights()
+    for bits in (0, 4, 16, 64):
+        assert lib.ccsm_train_create_act(C.byref(w), 0, 16, None, bits, C.byref(out)) == INVALID
+        assert b"activation_bits" in lib.ccsm_train_last_error()

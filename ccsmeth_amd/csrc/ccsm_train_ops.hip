@@ -87,33 +87,27 @@ ccsm_status check_saved(const ccsm_saved& s, int type, int64_t width, const char
 Saved saved_of(const ccsm_saved& s) { return Saved{s.data, s.ld, s.code, s.scales, s.lds}; }
 Saved plain(const void* p, int64_t ld) { return Saved{p, ld, kCodeNone, nullptr, 0}; }
 
-// An operand as the product kernel takes it: as it is where its rows consist of whole, aligned 16-byte pieces of the product's own 16-bit type,
-// else staged into planes of the scratch (fp32: three of bf16; 8-bit codes: one, bf16 for fp32).
-struct Staged { Plane p; int planes; };
+// An operand as the tile kernels take it: as it is where its rows consist of whole, aligned 16-byte pieces of the call's type, else a staged copy in the
+// scratch (8-bit codes too: the values that they stand for)
 bool whole_rows(const void* p, int64_t ld, int64_t width, int type) {
     const int64_t n = 16 / (int64_t)size_of(type);
-    return !off_by(p, 16) && ld % n == 0 && width % n == 0 && ld < (1 << 22);      // (the kernel's 32-bit offsets span a tile's rows)
+    return !off_by(p, 16) && ld % n == 0 && width % n == 0 && ld < (1 << 21);      // (the kernels' 32-bit offsets span a tile's rows)
 }
 template <typename T>
-Staged staged(const Saved& s, int64_t rows, int64_t width, Scratch& ws, hipStream_t st, bool count) {
-    const int type = TypeOf<T>::v;
-    const bool codes = s.code != kCodeNone;
-    if (type != CCSM_TYPE_F32 && !codes && whole_rows(s.data, s.ld, width, type)) return Staged{Plane{s.data, s.ld, 0}, 1};
-    const int planes = type == CCSM_TYPE_F32 && !codes ? 3 : 1;
-    const int64_t ld = (int64_t)up(width, 8), plane = rows * ld;
-    uint16_t* out = ws.take<uint16_t>((size_t)planes * plane);
-    if (!count) {
-        const unsigned grid = grid_of(cdiv(plane / 8, 256), 1 << 16);
-        if (codes) stage_kernel<T, true><<<grid, 256, 0, st>>>(s, rows, (int)width, out, ld, plane);
-        else stage_kernel<T, false><<<grid, 256, 0, st>>>(s, rows, (int)width, out, ld, plane);
-    }
-    return Staged{Plane{out, ld, plane}, planes};
+Plane staged(const Saved& s, int64_t rows, int64_t width, Scratch& ws, hipStream_t st, bool count) {
+    if (s.code == kCodeNone && whole_rows(s.data, s.ld, width, TypeOf<T>::v)) return Plane{s.data, s.ld};
+    const int64_t ld = (int64_t)up(width, 8);
+    T* out = ws.take<T>((size_t)rows * ld);
+    if (!count) stage_kernel<T><<<grid_of(cdiv(rows * ld / 8, 256), 1 << 16), 256, 0, st>>>(s, rows, (int)width, out, ld);
+    return Plane{out, ld};
 }
 
 template <typename T, bool TRP, bool TRQ, int B>
 hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
     constexpr int lds = 5 * B * 128;                    // two chunks of P, three of Q
-    auto* f = &product_mfma_kernel<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
+    void (*f)(ProductArgs);
+    if constexpr (sizeof(T) == 4) f = &product_f32_kernel<TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
+    else f = &product_mfma_kernel<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
     // an attribute of the function on each device: set once for each (setting it twice, from two threads, does no harm)
     static std::atomic<uint64_t> known{0};
     int device = 0;
@@ -130,22 +124,22 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
 }
 // out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue
 template <typename T, bool TRP, bool TRQ>
-hipError_t product(hipStream_t st, const Staged& p, const Staged& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, bool count) {
+hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, bool count) {
     ProductArgs a;
-    a.P = p.p; a.Q = q.p;
+    a.P = p; a.Q = q;
     a.M = (int)M; a.N = (int)N; a.K = (int)K;
-    a.passes = p.planes == 1 ? 1 : q.planes == 1 ? 3 : 6;
     a.ep = ep;
-    const int64_t chunks = cdiv(K, 64) * a.passes;
+    constexpr int64_t chunk = 128 / (int64_t)sizeof(T);
+    const int64_t chunks = cdiv(K, chunk);
     const int64_t big = cdiv(M, 256) * cdiv(N, 256), small = cdiv(M, 128) * cdiv(N, 128);
     const int B = big >= 200 ? 256 : 128;
     a.tiles_i = (int)cdiv(M, B); a.tiles_j = (int)cdiv(N, B);
     const int64_t tiles = B == 256 ? big : small, slots = B == 256 ? 256 : 512;
     int64_t splits = tiles * 2 <= slots ? slots / tiles : 1;
-    const int64_t least = 8;                                      // chunks of a split
+    const int64_t least = sizeof(T) == 4 ? 4 : 8;                 // chunks of a split
     if (splits > cdiv(chunks, least)) splits = cdiv(chunks, least);
-    a.chunks = (int)(cdiv(cdiv(chunks, splits), a.passes) * a.passes);
-    a.splits = (int)cdiv(chunks, a.chunks);
+    a.depth = (int)(cdiv(chunks, splits) * chunk);
+    a.splits = (int)cdiv(K, a.depth);
     a.part_ld = (int64_t)up(N, 4);
     a.part = a.splits > 1 ? ws.take<float>((size_t)a.splits * M * a.part_ld) : nullptr;
     if (count) return hipSuccess;
@@ -186,7 +180,7 @@ ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bo
         TRY((direct<T, false, false>(st, plain(p->x, p->ldx), plain(p->x, p->ldx), CCSM_ACT_NONE, plain(p->w, p->ldw), p->rows, p->outer, p->inner, nullptr, ep)), "linear_forward");
         return CCSM_OK;
     }
-    const Staged x = staged<T>(plain(p->x, p->ldx), p->rows, p->inner, ws, st, count), w = staged<T>(plain(p->w, p->ldw), p->outer, p->inner, ws, st, count);
+    const Plane x = staged<T>(plain(p->x, p->ldx), p->rows, p->inner, ws, st, count), w = staged<T>(plain(p->w, p->ldw), p->outer, p->inner, ws, st, count);
     TRY((product<T, false, false>(st, x, w, p->rows, p->outer, p->inner, ep, ws, count)), "linear_forward");
     return CCSM_OK;
 }
@@ -234,27 +228,25 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
             TRY((direct<T, true, true>(st, dy, z, p->activation, p->dw ? saved_of(p->x) : dy, N, p->dw ? K : 1, M, p->dbias, to_dw)), "linear_backward: dw");
         return CCSM_OK;
     }
-    // d as the products take it: dy itself where there is no activation, the type is a 16-bit one and its rows are whole pieces
+    // d as the products take it: dy itself where there is no activation and its rows are whole pieces
     const bool products = p->dx || p->dw;
     const Saved dy = plain(p->dy, p->lddy);
-    const bool none = p->activation == CCSM_ACT_NONE, direct = none && TypeOf<T>::v != CCSM_TYPE_F32 && whole_rows(p->dy, p->lddy, N, TypeOf<T>::v);
-    const int planes = TypeOf<T>::v == CCSM_TYPE_F32 ? 3 : 1;
-    const int64_t ldd = (int64_t)up(N, 8), plane = M * ldd, parts = cdiv(M, 32);
-    Staged d{Plane{p->dy, p->lddy, 0}, 1};
-    if (products && !direct) d = Staged{Plane{ws.take<uint16_t>((size_t)planes * plane), ldd, plane}, planes};
+    const bool none = p->activation == CCSM_ACT_NONE, as_is = none && whole_rows(p->dy, p->lddy, N, TypeOf<T>::v), make = products && !as_is;
+    const int64_t ldd = (int64_t)up(N, 8), parts = cdiv(M, 32);
+    T* made = make ? ws.take<T>((size_t)M * ldd) : nullptr;
+    const Plane d = make ? Plane{made, ldd} : Plane{p->dy, p->lddy};
     float* part = p->dbias ? ws.take<float>((size_t)parts * N) : nullptr;
-    if (!count && (part || (products && !direct))) {
-        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 256)), 256, 0, st>>>(dy, none ? dy : saved_of(p->preact), p->activation, M, N,
-                                                                                     products && !direct ? const_cast<void*>(d.p.base) : nullptr, ldd, plane, part);
+    if (!count && (part || make)) {
+        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 256)), 256, 0, st>>>(dy, none ? dy : saved_of(p->preact), p->activation, M, N, made, ldd, part);
         if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 8), 256, 0, st>>>(part, (int)parts, N, (T*)p->dbias);
         LAUNCHED("linear_backward");
     }
     if (p->dx) {
-        const Staged w = staged<T>(plain(p->w, p->ldw), N, K, ws, st, count);
+        const Plane w = staged<T>(plain(p->w, p->ldw), N, K, ws, st, count);
         TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, count)), "linear_backward: dx");
     }
     if (p->dw) {
-        const Staged x = staged<T>(saved_of(p->x), M, K, ws, st, count);
+        const Plane x = staged<T>(saved_of(p->x), M, K, ws, st, count);
         TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, count)), "linear_backward: dw");
     }
     return CCSM_OK;

@@ -23,10 +23,6 @@
 // Ragged sizes: pieces beyond k's end get an offset outside the buffer resource and arrive as zeros; rows and columns beyond i's or j's end
 // repeat the last ones, and their results are not written.  What the kernel needs: 16-byte aligned bases and row strides (multiples of 8
 // elements), the contiguous extent a multiple of 8; other operands are staged first (stage_kernel).
-//
-// Passes.  An fp32 operand is staged as three 16-bit planes (bf16: v = v0 + v1 + v2 exactly, but for values below 2^-110), and the product is
-// six products of planes, (2,0) (0,2) (1,1) (1,0) (0,1) (0,0): what is left out is below 2^-25 of each product.  Each k step runs its passes one behind
-// the other, so that the planes are read again out of L2.
 #pragma once
 #include "ccsm_train_ops_common.h"
 
@@ -59,12 +55,11 @@ template <> struct Mfma<b16> {
 struct Epilogue {
     const void* bias; const void* residual; long long ldr; void* y; long long ldy; void* pre; long long ldp; int act;
 };
-struct Plane { const void* base; long long ld; long long plane; };      // elements of 16 bits; `plane`: from one plane to the next
+struct Plane { const void* base; long long ld; };
 struct ProductArgs {
     Plane P, Q;
     int M, N, K;
-    int passes;               // 1, 3 (P in three planes, Q in one) or 6
-    int tiles_i, tiles_j, splits, chunks;     // chunks of 64 k times passes of one split (a multiple of passes)
+    int tiles_i, tiles_j, splits, depth;      // k of one split (a multiple of the kernel's chunk)
     float* part; long long part_ld;           // [split][M][part_ld]
     Epilogue ep;
 };
@@ -85,8 +80,9 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, in
     }
     store_row<T, N>((T*)e.y + i * e.ldy + j, left, z);
 }
-// One operand's side: requests by NW waves (this one is number `wave` of them) for B rows or columns, and the fragments of this wave's W of them
-template <bool TR, int B, int W, int NW>
+// One operand's side: requests by NW waves (this one is number `wave` of them) for B rows or columns, and the fragments of this wave's W of them; ES =
+// bytes of an element (a chunk is 128 / ES deep)
+template <int ES, bool TR, int B, int W, int NW>
 struct Side {
     static constexpr unsigned kChunk = B * 128;            // bytes
     static constexpr int kReq = kChunk / 1024 / NW;        // requests per wave and chunk
@@ -96,30 +92,36 @@ struct Side {
     unsigned rd[TR ? kFrag : 2];                           // LDS byte offsets of the fragments (k contiguous: of the two halves of a chunk)
 
     __device__ __forceinline__ void init(const Plane& p, int at, int extent, int wave, int lane, int w0, unsigned lds) {
+        constexpr int kPer = 16 / ES;                      // elements of a 16-byte piece
 #pragma unroll
         for (int r = 0; r < kReq; ++r) {
             const int q = r * NW + wave;                   // request number within the chunk
             if (!TR) {
                 const int row = q * 8 + (lane >> 3), c = (lane & 7) ^ (row & 7);
                 const int i = at + row < extent ? row : extent - 1 - at;
-                off[r] = (unsigned)(((long long)i * p.ld + 8 * c) * 2);
-                kpos[r] = 8 * c;
+                off[r] = (unsigned)(((long long)i * p.ld + kPer * c) * ES);
+                kpos[r] = kPer * c;
             } else {
-                constexpr int kRow = B / 8;                // 16-byte pieces per row
+                constexpr int kRow = B / kPer;             // pieces per row
                 const int k = (q * 64 + lane) / kRow, x = (q * 64 + lane) % kRow;
-                const int s = (k & 3) | ((k >> 1) & 4), c = (((x >> 1) ^ s) << 1) | (x & 1);
-                const int i = at + 8 * c < extent ? 8 * c : ((extent - 1) & ~7) - at;
-                off[r] = (unsigned)(((long long)k * p.ld + i) * 2);
+                const int c = ES == 2 ? (((x >> 1) ^ ((k & 3) | ((k >> 1) & 4))) << 1) | (x & 1) : ((x >> 2) ^ ((k >> 3) & 3)) << 2 | (x & 3);
+                const int i = at + kPer * c < extent ? kPer * c : ((extent - 1) & ~(kPer - 1)) - at;
+                off[r] = (unsigned)(((long long)k * p.ld + i) * ES);
                 kpos[r] = k;
             }
         }
         if (!TR) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) rd[h] = lds + (unsigned)((w0 + (lane & 15)) * 128 + (((4 * h + (lane >> 4)) ^ (lane & 7)) << 4));
-        } else {
+            for (int h = 0; h < 2; ++h)
+                rd[h] = lds + (unsigned)((w0 + (lane & 15)) * 128 + (((ES == 2 ? 4 * h + (lane >> 4) : 2 * (lane >> 4) + h) ^ (lane & 7)) << 4));
+        } else if (ES == 2) {
             const int k = 8 * (lane >> 4) + ((lane & 15) >> 2), s = (k & 3) | ((k >> 1) & 4);
 #pragma unroll
             for (int f = 0; f < kFrag; ++f) rd[f] = lds + (unsigned)(k * (2 * B) + (((w0 / 16 + f) ^ s) << 5) + (lane & 3) * 8);
+        } else {
+            const int g = lane >> 4;
+#pragma unroll
+            for (int f = 0; f < kFrag; ++f) rd[f] = lds + (unsigned)(8 * g * (4 * B) + (((w0 / 16 + f) ^ g) << 6) + (lane & 15) * 4);
         }
     }
     // request r of a chunk into LDS at `m0` (the wave's base of that request)
@@ -136,143 +138,62 @@ struct Side {
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(rd[f] + base + h * 64 * B + 8 * B));
         return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    // ES = 4: the eight values of fragment f
+    __device__ __forceinline__ void values(int f, unsigned base, float (&v)[8]) const {
+        typedef __attribute__((address_space(3))) const f32x4* P4;
+        typedef __attribute__((address_space(3))) const float* P1;
+        if (!TR) {
+            const f32x4 a = *(P4)(uintptr_t)(rd[0] + base + f * 2048), b = *(P4)(uintptr_t)(rd[1] + base + f * 2048);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+            return;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = *(P1)(uintptr_t)(rd[f] + base + q * 4 * B);
+    }
 };
 // where an operand's next chunk comes from
-template <bool TR>
+template <int ES, bool TR>
 struct Cursor {
     const char* base;
-    long long ld, plane;
-    int k, pass, left_chunks;
-    unsigned codes;                                        // the plane of each pass, four bits each
-    __device__ __forceinline__ u32x4 next(int K, int passes, int* left) {
-        const unsigned long long p = (unsigned long long)(base + ((TR ? (long long)k * ld : (long long)k) + (long long)((codes >> (4 * pass)) & 15u) * plane) * 2);
-        *left = left_chunks > 0 ? K - k : 0;               // behind the last chunk everything is out of range: zeros that nobody reads
-        --left_chunks;
-        if (++pass == passes) { pass = 0; k += 64; }
+    long long step;                                        // bytes from one chunk to the next
+    int left;                                              // k left in the split, and behind it: everything out of range, zeros that nobody reads
+    __device__ __forceinline__ u32x4 next(int* l) {
+        const unsigned long long p = (unsigned long long)base;
+        *l = left;
+        base += step;
+        left -= 128 / ES;
         return u32x4{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, 0xfffffffeu, 0x00020000u};
     }
 };
-
-template <typename T, bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_mfma_kernel(ProductArgs a) {
-    typedef typename std::conditional<sizeof(T) == 4, b16, T>::type E;
-    constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16, HW = BI / WI;
-    typedef Side<TRP, BI, HW, NW> SP;
-    typedef Side<TRQ, BJ, BJ / WJ, NW> SQ;
-    constexpr int kReq = SP::kReq;
-    static_assert(SP::kReq == SQ::kReq, "");
-    extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
-    // Workgroups go to the eight XCDs in turn; each XCD takes one contiguous eighth of the tiles (its L2 holds their operands), in columns of eight
-    // tiles along i, so that the 32 tiles of an XCD that run together share eight strips of P and four of Q
-    const int n = a.tiles_i * a.tiles_j * a.splits, b = blockIdx.x;
-    const int each = n >> 3, over = n & 7, x = b & 7;
+template <int ES, bool TR>
+__device__ __forceinline__ Cursor<ES, TR> cursor(const Plane& p, int at, int k0, int k1) {
+    return Cursor<ES, TR>{(const char*)p.base + (TR ? (long long)k0 * p.ld + at : (long long)at * p.ld + k0) * ES, (TR ? p.ld * (128 / ES) : 128 / ES) * ES, k1 - k0};
+}
+// Workgroups go to the eight XCDs in turn; each XCD takes one contiguous eighth of the tiles (its L2 holds their operands), in columns of eight tiles
+// along i, so that the 32 tiles of an XCD that run together share eight strips of P and four of Q
+struct Place { int i, j, split; };
+__device__ __forceinline__ Place place_of(int b, int tiles_i, int tiles_j, int splits) {
+    const int n = tiles_i * tiles_j * splits, each = n >> 3, over = n & 7, x = b & 7;
     int t = x * each + (x < over ? x : over) + (b >> 3);
-    const int split = t / (a.tiles_i * a.tiles_j);
-    t -= split * (a.tiles_i * a.tiles_j);
-    const int band = t / (8 * a.tiles_j), in = t - band * 8 * a.tiles_j, rows = a.tiles_i - 8 * band < 8 ? a.tiles_i - 8 * band : 8;
-    const int ti = 8 * band + in % rows, tj = in / rows;
-    const int i0 = ti * BI, j0 = tj * BJ;
+    const int split = t / (tiles_i * tiles_j);
+    t -= split * (tiles_i * tiles_j);
+    const int band = t / (8 * tiles_j), in = t - band * 8 * tiles_j, rows = tiles_i - 8 * band < 8 ? tiles_i - 8 * band : 8;
+    return Place{8 * band + in % rows, in / rows, split};
+}
 
-    const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
-    constexpr unsigned kP = SP::kChunk, kQ = SQ::kChunk, kQ0 = 2 * kP;                      // LDS: P's two chunks, then Q's three
-    const unsigned lq = lds + kQ0;
-    SP sp;
-    SQ sq;
-    sp.init(a.P, i0, a.M, wave, lane, wi * HW, lds);
-    sq.init(a.Q, j0, a.N, wave, lane, wj * (BJ / WJ), lq);
-
-    const int total = (a.K + 63) / 64 * a.passes, first = split * a.chunks, last = first + a.chunks < total ? first + a.chunks : total;
-    // passes (P's plane, Q's): 6: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); 3: (2,0) (1,0) (0,0); 1: (0,0).  Splits begin with a chunk's first pass.
-    const int k0 = first / a.passes * 64;
-    Cursor<TRP> cp{(const char*)a.P.base + (TRP ? (long long)i0 : (long long)i0 * a.P.ld) * 2, a.P.ld, a.P.plane, k0, 0, last - first, a.passes == 6 ? 0x001102u : a.passes == 3 ? 0x012u : 0u};
-    Cursor<TRQ> cq{(const char*)a.Q.base + (TRQ ? (long long)j0 : (long long)j0 * a.Q.ld) * 2, a.Q.ld, a.Q.plane, k0, 0, last - first, a.passes == 6 ? 0x010120u : 0u};
-    u32x4 srd;
-    int left;
-    auto request_p = [&](int r, unsigned base) { sp.request(r, srd, left, lds + base + (r * NW + wave) * 1024); };
-    auto request_q = [&](int r, unsigned base) { sq.request(r, srd, left, lq + base + (r * NW + wave) * 1024); };
-
-    f32x4 acc[FI][FJ];
-#pragma unroll
-    for (int p = 0; p < FI; ++p)
-#pragma unroll
-        for (int q = 0; q < FJ; ++q) {
-            acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
-            asm volatile("" : "+v"(acc[p][q]));            // (written here, far from the first product)
-        }
-    // Chunk c = steps 2c and 2c + 1.  The fragments of a step are read while the step before multiplies; one barrier a chunk, in front of step 2c + 1, behind
-    // which chunk c + 1 has landed (every wave has waited for all but its last four requests) and chunk c has been read.  Its place in P's ring is
-    // requested for chunk c + 2 in step 2c + 1, the one of chunk c - 1 in Q's ring for chunk c + 2 in step 2c.
-    s16x8 fp[2][FI], fq[2][FJ];
-    auto all_p = [&](unsigned base) {
-        srd = cp.next(a.K, a.passes, &left);
-#pragma unroll
-        for (int r = 0; r < kReq; ++r) request_p(r, base);
-    };
-    auto all_q = [&](unsigned base) {
-        srd = cq.next(a.K, a.passes, &left);
-#pragma unroll
-        for (int r = 0; r < kReq; ++r) request_q(r, base);
-    };
-    all_p(0);
-    all_q(0);
-    all_q(kQ);
-    all_p(kP);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * kReq) : "memory");
-#pragma unroll
-    for (int q = 0; q < FJ; ++q) fq[0][q] = sq.fragment(q, 0, 0);
-#pragma unroll
-    for (int p = 0; p < FI; ++p) fp[0][p] = sp.fragment(p, 0, 0);
-    unsigned bp = 0, bq = 0, free_q = 2 * kQ;              // the current chunk's places in the rings, Q's free one
-    constexpr int kReads = FI + FJ, kRows = FI == 8 ? 6 : FI;
-    for (int c = first; c < last; ++c) {
-        srd = cq.next(a.K, a.passes, &left);
-#pragma unroll
-        for (int p = 0; p < FI; ++p) {                     // fragments of the step's other half first, then requests, between rows of products
-#pragma unroll
-            for (int f = p * kReads / kRows; f < (p + 1) * kReads / kRows && f < kReads; ++f) {
-                if (f < FJ) fq[1][f] = sq.fragment(f, 1, bq);
-                else fp[1][f - FJ] = sp.fragment(f - FJ, 1, bp);
-            }
-#pragma unroll
-            for (int q = 0; q < FJ; ++q) Mfma<E>::tied(fq[0][q], fp[0][p], acc[p][q]);
-#pragma unroll
-            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request_q(r, free_q);
-            __builtin_amdgcn_sched_barrier(0);             // (left to itself the compiler begins the next step's products here and waits for their operands)
-        }
-        free_q = bq;
-        bq = bq == 2 * kQ ? 0 : bq + kQ;
-        bp ^= kP;
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kReq) : "memory");
-        srd = cp.next(a.K, a.passes, &left);
-#pragma unroll
-        for (int p = 0; p < FI; ++p) {
-#pragma unroll
-            for (int f = p * kReads / kRows; f < (p + 1) * kReads / kRows && f < kReads; ++f) {
-                if (f < FJ) fq[0][f] = sq.fragment(f, 0, bq);
-                else fp[0][f - FJ] = sp.fragment(f - FJ, 0, bp);
-            }
-#pragma unroll
-            for (int q = 0; q < FJ; ++q) Mfma<E>::tied(fq[1][q], fp[1][p], acc[p][q]);
-#pragma unroll
-            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request_p(r, bp ^ kP);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    asm volatile("s_nop 15\n\ts_nop 15");                    // the last products' results are there (16 passes at most), for whatever reads them below
-#pragma unroll
-    for (int p = 0; p < FI; ++p)
-#pragma unroll
-        for (int q = 0; q < FJ; ++q) asm volatile("" : "+v"(acc[p][q]));
+// a wave's 16 FI x 16 FJ results from (i_wave, jw) on
+template <typename T, int FI, int FJ, int NW>
+__device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, int wave, int lane, int i_wave, int jw, int split, const f32x4 (&acc)[FI][FJ]) {
     // The results leave through the wave's own part of LDS, 32 rows of i at a time (rows 16 bytes longer than they need: the lanes' writes fall on
     // different banks), and from there in pieces of eight neighbours of a row.  A lane's column does not change, so its bias is loaded once; a
     // round's residual is loaded a round ahead (one load at a time, 128 loads one behind the other, took 170 of 640 us of a 16384 x 4096 x 4096
     // product).
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (no request may still write LDS)
-    constexpr int WJT = BJ / WJ, kRow = WJT + 4, kPer = WJT / 8, kIt = 32 * kPer / 64, kRowsIt = 64 / kPer;
-    static_assert(32 * kRow * 4 * NW <= kQ0 + 3 * kQ && 64 % kPer == 0, "the waves' rows fit into the stages");
-    float* out = reinterpret_cast<float*>(ops_smem) + wave * 32 * kRow;
-    const int c = lane % kPer * 8, j = j0 + wj * WJT + c, left_j = a.N - j, iw = i0 + wi * (BI / WI) + lane / kPer;
+    constexpr int WJT = 16 * FJ, kRow = WJT + 4, kPer = WJT / 8, kIt = 32 * kPer / 64, kRowsIt = 64 / kPer;
+    static_assert(NW * 32 * kRow * 4 <= (NW == 8 ? 160 : 80) * 1024 && 64 % kPer == 0, "the waves' rows fit into the stages");
+    float* out = smem + wave * 32 * kRow;
+    const int c = lane % kPer * 8, j = jw + c, left_j = a.N - j, iw = i_wave + lane / kPer;
     const bool res = !a.part && a.ep.residual && left_j > 0;
     float bias[8];
     if (!a.part && a.ep.bias && left_j > 0) load_row<T, 8>((const T*)a.ep.bias + j, left_j, bias);
@@ -316,6 +237,250 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
     }
 }
 
+template <typename T, bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_mfma_kernel(ProductArgs a) {
+    constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16, HW = BI / WI;
+    typedef Side<2, TRP, BI, HW, NW> SP;
+    typedef Side<2, TRQ, BJ, BJ / WJ, NW> SQ;
+    constexpr int kReq = SP::kReq;
+    static_assert(SP::kReq == SQ::kReq, "the waits below count as many requests of each operand");
+    extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
+    const Place at = place_of(blockIdx.x, a.tiles_i, a.tiles_j, a.splits);
+    const int i0 = at.i * BI, j0 = at.j * BJ, split = at.split;
+    const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
+    constexpr unsigned kP = SP::kChunk, kQ = SQ::kChunk, kQ0 = 2 * kP;      // LDS: P's two chunks, then Q's three
+    const unsigned lq = lds + kQ0;
+    SP sp;
+    SQ sq;
+    sp.init(a.P, i0, a.M, wave, lane, wi * HW, lds);
+    sq.init(a.Q, j0, a.N, wave, lane, wj * (BJ / WJ), lq);
+    const int first = split * a.depth, last = first + a.depth < a.K ? first + a.depth : a.K;
+    Cursor<2, TRP> cp = cursor<2, TRP>(a.P, i0, first, last);
+    Cursor<2, TRQ> cq = cursor<2, TRQ>(a.Q, j0, first, last);
+    u32x4 srd;
+    int left;
+    auto request_p = [&](int r, unsigned base) { sp.request(r, srd, left, lds + base + (r * NW + wave) * 1024); };
+    auto request_q = [&](int r, unsigned base) { sq.request(r, srd, left, lq + base + (r * NW + wave) * 1024); };
+
+    f32x4 acc[FI][FJ];
+#pragma unroll
+    for (int p = 0; p < FI; ++p)
+#pragma unroll
+        for (int q = 0; q < FJ; ++q) {
+            acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+            asm volatile("" : "+v"(acc[p][q]));            // (written here, far from the first product)
+        }
+    // Chunk c = steps 2c and 2c + 1.  The fragments of a step are read while the step before multiplies; one barrier a chunk, in front of step 2c + 1, behind
+    // which chunk c + 1 has landed (every wave has waited for all but its last four requests) and chunk c has been read.  Its place in P's ring is
+    // requested for chunk c + 2 in step 2c + 1, the one of chunk c - 1 in Q's ring for chunk c + 2 in step 2c.
+    s16x8 fp[2][FI], fq[2][FJ];
+    auto all_p = [&](unsigned base) {
+        srd = cp.next(&left);
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) request_p(r, base);
+    };
+    auto all_q = [&](unsigned base) {
+        srd = cq.next(&left);
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) request_q(r, base);
+    };
+    all_p(0);
+    all_q(0);
+    all_q(kQ);
+    all_p(kP);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * kReq) : "memory");
+#pragma unroll
+    for (int q = 0; q < FJ; ++q) fq[0][q] = sq.fragment(q, 0, 0);
+#pragma unroll
+    for (int p = 0; p < FI; ++p) fp[0][p] = sp.fragment(p, 0, 0);
+    unsigned bp = 0, bq = 0, free_q = 2 * kQ;              // the current chunk's places in the rings, Q's free one
+    constexpr int kReads = FI + FJ, kRows = FI == 8 ? 6 : FI;
+    for (int c = first; c < last; c += 64) {
+        srd = cq.next(&left);
+#pragma unroll
+        for (int p = 0; p < FI; ++p) {                     // fragments of the step's other half first, then requests, between rows of products
+#pragma unroll
+            for (int f = p * kReads / kRows; f < (p + 1) * kReads / kRows && f < kReads; ++f) {
+                if (f < FJ) fq[1][f] = sq.fragment(f, 1, bq);
+                else fp[1][f - FJ] = sp.fragment(f - FJ, 1, bp);
+            }
+#pragma unroll
+            for (int q = 0; q < FJ; ++q) Mfma<T>::tied(fq[0][q], fp[0][p], acc[p][q]);
+#pragma unroll
+            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request_q(r, free_q);
+            __builtin_amdgcn_sched_barrier(0);             // (left to itself the compiler begins the next step's products here and waits for their operands)
+        }
+        free_q = bq;
+        bq = bq == 2 * kQ ? 0 : bq + kQ;
+        bp ^= kP;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kReq) : "memory");
+        srd = cp.next(&left);
+#pragma unroll
+        for (int p = 0; p < FI; ++p) {
+#pragma unroll
+            for (int f = p * kReads / kRows; f < (p + 1) * kReads / kRows && f < kReads; ++f) {
+                if (f < FJ) fq[0][f] = sq.fragment(f, 0, bq);
+                else fp[0][f - FJ] = sp.fragment(f - FJ, 0, bp);
+            }
+#pragma unroll
+            for (int q = 0; q < FJ; ++q) Mfma<T>::tied(fq[1][q], fp[1][p], acc[p][q]);
+#pragma unroll
+            for (int r = p * kReq / FI; r < (p + 1) * kReq / FI; ++r) request_p(r, bp ^ kP);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    asm volatile("s_nop 15\n\ts_nop 15");                    // the last products' results are there (16 passes at most), for whatever reads them below
+#pragma unroll
+    for (int p = 0; p < FI; ++p)
+#pragma unroll
+        for (int q = 0; q < FJ; ++q) asm volatile("" : "+v"(acc[p][q]));
+    store_tile<T, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), split, acc);
+}
+
+// v as three bf16 values whose sum it is: the first eight bits cut off (so that no finite value becomes infinite), the rest rounded to nearest twice;
+// infinities and NaN make all of a product NaN
+__device__ __forceinline__ void three(float v, b16 (&p)[3]) {
+    const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r = v - h;
+    p[0] = __builtin_bit_cast(b16, (unsigned short)(__float_as_uint(v) >> 16));
+    p[1] = (b16)r;
+    p[2] = (b16)(r - (float)p[1]);
+}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+// the same for eight values, as three fragments: 44 instructions
+__device__ __forceinline__ void three8(const float (&v)[8], s16x8 (&p)[3]) {
+    unsigned o[3][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned a = __float_as_uint(v[2 * k]), b = __float_as_uint(v[2 * k + 1]);
+        o[0][k] = __builtin_amdgcn_perm(b, a, 0x07060302u);       // the upper halves of both
+        const f32x2 r{v[2 * k] - __uint_as_float(a & 0xffff0000u), v[2 * k + 1] - __uint_as_float(b & 0xffff0000u)};
+        o[1][k] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, b16x2));
+        const f32x2 s{r[0] - __uint_as_float(o[1][k] << 16), r[1] - __uint_as_float(o[1][k] & 0xffff0000u)};
+        o[2][k] = __builtin_bit_cast(unsigned, __builtin_convertvector(s, b16x2));
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) p[q] = __builtin_bit_cast(s16x8, u32x4{o[q][0], o[q][1], o[q][2], o[q][3]});
+}
+// The fp32 product: the same tiles, rings and requests with chunks of 32 k; a fragment's eight values are read as fp32 and split into three bf16
+// fragments in registers (5.5 instructions a value), and each pair of fragments is multiplied six times: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); what is
+// left out is below 2^-22 of each product, 2^-25 in the mean.  Bound by the matrix pipe: 192 instructions of 16 cycles a chunk and wave, beside 2100
+// cycles of splitting.  (Three bf16 planes in memory, made by a kernel in front and multiplied by the 16-bit kernel: 18 us a 44 MB operand, and three
+// times the requests: 21504 x 512 x 768 110 us.)
+// Q's fragments of a chunk stay in registers; P's come one row of products ahead.  The next chunk's Q is read and split in the last row, each fragment
+// behind its last product; the barrier stands in front of that row, when all of this chunk has been read.
+template <bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_f32_kernel(ProductArgs a) {
+    constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16, HW = BI / WI;
+    typedef Side<4, TRP, BI, HW, NW> SP;
+    typedef Side<4, TRQ, BJ, BJ / WJ, NW> SQ;
+    constexpr int kReq = SP::kReq;
+    static_assert(SP::kReq == SQ::kReq && kReq <= FI, "the waits below count as many requests of each operand");
+    extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
+    const Place at = place_of(blockIdx.x, a.tiles_i, a.tiles_j, a.splits);
+    const int i0 = at.i * BI, j0 = at.j * BJ;
+    const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
+    constexpr unsigned kP = SP::kChunk, kQ = SQ::kChunk;
+    const unsigned lq = lds + 2 * kP;
+    SP sp;
+    SQ sq;
+    sp.init(a.P, i0, a.M, wave, lane, wi * HW, lds);
+    sq.init(a.Q, j0, a.N, wave, lane, wj * (BJ / WJ), lq);
+    const int first = at.split * a.depth, last = first + a.depth < a.K ? first + a.depth : a.K;
+    Cursor<4, TRP> cp = cursor<4, TRP>(a.P, i0, first, last);
+    Cursor<4, TRQ> cq = cursor<4, TRQ>(a.Q, j0, first, last);
+    u32x4 srd;
+    int left;
+    auto request_p = [&](int r, unsigned base) { sp.request(r, srd, left, lds + base + (r * NW + wave) * 1024); };
+    auto request_q = [&](int r, unsigned base) { sq.request(r, srd, left, lq + base + (r * NW + wave) * 1024); };
+    auto all_p = [&](unsigned base) {
+        srd = cp.next(&left);
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) request_p(r, base);
+    };
+    auto all_q = [&](unsigned base) {
+        srd = cq.next(&left);
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) request_q(r, base);
+    };
+    f32x4 acc[FI][FJ];
+#pragma unroll
+    for (int p = 0; p < FI; ++p)
+#pragma unroll
+        for (int q = 0; q < FJ; ++q) acc[p][q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    all_p(0);
+    all_q(0);
+    all_q(kQ);
+    all_p(kP);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(2 * kReq) : "memory");
+    s16x8 fq[FJ][3], fp[2][3];
+    float raw[8], rq[2][8];
+#pragma unroll
+    for (int q = 0; q < FJ; ++q) {
+        sq.values(q, 0, raw);
+        three8(raw, fq[q]);
+    }
+    sp.values(0, 0, raw);
+    three8(raw, fp[0]);
+    sp.values(1, 0, raw);
+    unsigned bp = 0, bq = 0, free_q = 2 * kQ;              // the current chunk's places in the rings, Q's free one
+    auto products = [&](int p, int q0, int q1) {           // six products of row p with the fragments [q0, q1): neighbours in time are independent of each other
+        constexpr int kQ6[6] = {2, 0, 1, 1, 0, 0}, kP6[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int s = 0; s < 6; ++s)
+#pragma unroll
+            for (int q = q0; q < q1; ++q) acc[p][q] = Mfma<b16>::run(fq[q][kQ6[s]], fp[p & 1][kP6[s]], acc[p][q]);
+    };
+    // the order of a row: two vector instructions of the next fragment's splitting in the shadow of each matrix instruction.  (One behind the other, the two
+    // waves of a SIMD split and multiply at the same times, and the step takes the sum of both: 90 us at 21504 x 512 x 768.)
+    auto interleave = [&]() {
+#pragma unroll
+        for (int k = 0; k < 6 * FJ; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int c = first; c < last; c += 32) {
+        srd = cq.next(&left);
+#pragma unroll
+        for (int p = 0; p < FI - 1; ++p) {
+            three8(raw, fp[(p + 1) & 1]);
+            products(p, 0, FJ);
+            interleave();
+            if (p + 2 < FI) sp.values(p + 2, bp, raw);
+            if (p < kReq) request_q(p, free_q);
+        }
+        if (kReq == FI) request_q(kReq - 1, free_q);
+        free_q = bq;
+        bq = bq == 2 * kQ ? 0 : bq + kQ;
+        bp ^= kP;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kReq) : "memory");
+        srd = cp.next(&left);
+        sq.values(0, bq, rq[0]);
+        sq.values(1, bq, rq[1]);
+        sp.values(0, bp, raw);
+#pragma unroll
+        for (int q = 0; q < FJ; q += 2) {
+            products(FI - 1, q, q + 2);
+            three8(rq[0], fq[q]);
+            three8(rq[1], fq[q + 1]);
+            if (q + 2 < FJ) {
+                sq.values(q + 2, bq, rq[0]);
+                sq.values(q + 3, bq, rq[1]);
+            }
+        }
+        three8(raw, fp[0]);
+        sp.values(1, bp, raw);
+#pragma unroll
+        for (int r = 0; r < kReq; ++r) request_p(r, bp ^ kP);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    store_tile<float, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), at.split, acc);
+}
+
 // the splits' parts in order, and the epilogue; a lane takes four neighbours
 template <typename T>
 __global__ __launch_bounds__(256) void product_join_kernel(const float* part, int splits, long long M, int N, long long ld, Epilogue ep) {
@@ -334,48 +499,6 @@ __global__ __launch_bounds__(256) void product_join_kernel(const float* part, in
     }
 }
 
-// v as three bf16 values whose sum it is (each rounded to nearest; a finite value never becomes infinite; infinities and NaN make all of it NaN)
-__device__ __forceinline__ void three(float v, b16 (&p)[3]) {
-    p[0] = (b16)v;
-    if (fabsf(v) < INFINITY && !(fabsf((float)p[0]) < INFINITY)) p[0] = __builtin_bit_cast(b16, (unsigned short)(__float_as_uint(v) >> 16));
-    const float r = v - (float)p[0];
-    p[1] = (b16)r;
-    p[2] = (b16)(r - (float)p[1]);
-}
-template <typename T, int N> struct Planes;       // N values into the planes of a staged operand
-template <int N> struct Planes<float, N> {
-    static constexpr int n = 3;
-    static __device__ __forceinline__ void put(const float (&v)[N], void* out, long long plane, long long at) {
-        Vec<b16, N> o[3];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            b16 p[3];
-            three(v[k], p);
-            o[0].v[k] = p[0]; o[1].v[k] = p[1]; o[2].v[k] = p[2];
-        }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *(Vec<b16, N>*)((b16*)out + q * plane + at) = o[q];
-    }
-};
-template <int N> struct Planes<f16, N> {
-    static constexpr int n = 1;
-    static __device__ __forceinline__ void put(const float (&v)[N], void* out, long long, long long at) {
-        Vec<f16, N> o;
-#pragma unroll
-        for (int k = 0; k < N; ++k) o.v[k] = (f16)v[k];
-        *(Vec<f16, N>*)((f16*)out + at) = o;
-    }
-};
-template <int N> struct Planes<b16, N> {
-    static constexpr int n = 1;
-    static __device__ __forceinline__ void put(const float (&v)[N], void* out, long long, long long at) {
-        Vec<b16, N> o;
-#pragma unroll
-        for (int k = 0; k < N; ++k) o.v[k] = (b16)v[k];
-        *(Vec<b16, N>*)((b16*)out + at) = o;
-    }
-};
-
 // eight values of row r from column c on, zeros beyond the width
 template <typename T>
 __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int width, float (&v)[8]) {
@@ -392,27 +515,25 @@ __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int wi
     for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
 }
 
-// a kept matrix as planes of 16-bit elements with rows of whole 16-byte pieces (zeros behind the width).  ONE: one plane whatever the type (8-bit
-// codes, whose values bf16 holds exactly)
-template <typename T, bool ONE>
-__global__ __launch_bounds__(256) void stage_kernel(Saved s, long long rows, int width, void* out, long long ld, long long plane) {
+// a kept matrix as rows of whole 16-byte pieces in the call's type (zeros behind the width)
+template <typename T>
+__global__ __launch_bounds__(256) void stage_kernel(Saved s, long long rows, int width, T* out, long long ld) {
     const int n = (int)(ld / 8);
     for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < rows * n; x += (long long)gridDim.x * 256) {
         const long long r = x / n;
         const int c = (int)(x % n) * 8;
         float v[8];
         load8<T>(s, r, c, width, v);
-        typedef typename std::conditional<ONE && sizeof(T) == 4, b16, T>::type O;
-        Planes<O, 8>::put(v, out, plane, r * ld + c);
+        store_row<T, 8>(out + r * ld + c, 8, v);
     }
 }
 
-// d = dy act'(z) into planes (16-bit types: one, rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 256 columns: 32 lanes of eight
+// d = dy act'(z) in the call's type (16-bit types: rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 256 columns: 32 lanes of eight
 // columns, eight rows at a time, four rows of a lane in flight.
 // Rounding d: 16-bit products take 16-bit operands, and this rounding (half a step per factor, independent of each other) moves a gradient by
 // no more than the rounding of the gradient itself does.  The bias gradient takes d before it.
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, long long M, int N, void* d, long long ldd, long long plane, float* part) {
+__global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, long long M, int N, T* d, long long ldd, float* part) {
     constexpr bool fast = sizeof(T) == 2;
     __shared__ float sum[8][256];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * 256 + lane * 8;
@@ -436,7 +557,7 @@ __global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, 
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[q][k] = c + k < N ? v[q][k] * u[q][k] : 0.f;
             }
-            if (d) Planes<T, 8>::put(v[q], d, plane, (m0 + 8 * q) * ldd + c);
+            if (d) store_row<T, 8>(d + (m0 + 8 * q) * ldd + c, 8, v[q]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc[k] += v[q][k];
         }

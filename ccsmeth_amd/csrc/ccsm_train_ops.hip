@@ -122,6 +122,30 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
     f<<<(unsigned)(a.tiles_i * a.tiles_j * a.splits), B == 256 ? 512 : 256, lds, st>>>(a);
     return hipGetLastError();
 }
+// The tile and the number of parts of the contraction with the least estimated time.  The estimate: workgroups go in rounds, 256 of the large tile (one for
+// each CU), 512 of the small one (two for each CU, and a round of up to 256 has them to itself); a round takes its chunks' measured time; parts cost a
+// launch, their sums' way through memory, and a step of the join each.  Chunk times measured at 2048^3 and 4096 x 4096 x 1024 (us, 16 bits | fp32):
+// large tile 1.3 | 4.5, small tile alone 0.55 | 1.4, in pairs 0.8 | 2.6.  Measured against the rule before (large tiles from 200 on, parts up to
+// 512 workgroups), bf16 | fp32, us, before -> after: 4096 x 1024 x 1024 26.6 -> 14.1 | 61 -> 53; 2048^3 33 -> 23 | 101 -> 95; 30000 x 1800 x 600
+// 92 -> 91 | 470 -> 372; 1024 x 4096 x 1024 26.3 -> 22.5 | 59 -> 57.
+struct Shape { int tile, splits; };
+Shape shape_of(int64_t M, int64_t N, int64_t chunks, bool f32) {
+    const double large = f32 ? 4.5 : 1.3, alone = f32 ? 1.4 : 0.55, pair = f32 ? 2.6 : 0.8;
+    const double launch = 4, per_part = 0.08, sums = (double)M * (double)N * 8 / 6e6;     // (written and read at 6 TB/s)
+    const int64_t tiles_big = cdiv(M, 256) * cdiv(N, 256), tiles_small = cdiv(M, 128) * cdiv(N, 128);
+    Shape best{128, 1};
+    double least = 0;
+    for (int64_t s = 1; s <= 256 && (s == 1 || 2 * s <= chunks); s += s < 32 ? 1 : s / 8) {
+        const double depth = (double)cdiv(chunks, s), join = s == 1 ? 0 : launch + per_part * (double)s + sums * (double)s;
+        const int64_t big = tiles_big * s, small = tiles_small * s, rest = small % 512;
+        if (s > 1 && small > 2048) break;
+        const double in_big = (double)cdiv(big, 256) * large * depth + join;
+        const double in_small = ((double)(small / 512) * pair + (rest == 0 ? 0 : rest <= 256 ? alone : pair)) * depth + join;
+        if (s == 1 || in_small < least) { least = in_small; best = {128, (int)s}; }
+        if (in_big < least) { least = in_big; best = {256, (int)s}; }
+    }
+    return best;
+}
 // out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue
 template <typename T, bool TRP, bool TRQ>
 hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, bool count) {
@@ -131,14 +155,10 @@ hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, in
     a.ep = ep;
     constexpr int64_t chunk = 128 / (int64_t)sizeof(T);
     const int64_t chunks = cdiv(K, chunk);
-    const int64_t big = cdiv(M, 256) * cdiv(N, 256), small = cdiv(M, 128) * cdiv(N, 128);
-    const int B = big >= 200 ? 256 : 128;
+    const Shape shape = shape_of(M, N, chunks, sizeof(T) == 4);
+    const int B = shape.tile;
     a.tiles_i = (int)cdiv(M, B); a.tiles_j = (int)cdiv(N, B);
-    const int64_t tiles = B == 256 ? big : small, slots = B == 256 ? 256 : 512;
-    int64_t splits = tiles * 2 <= slots ? slots / tiles : 1;
-    const int64_t least = sizeof(T) == 4 ? 4 : 8;                 // chunks of a split
-    if (splits > cdiv(chunks, least)) splits = cdiv(chunks, least);
-    a.depth = (int)(cdiv(chunks, splits) * chunk);
+    a.depth = (int)(cdiv(chunks, shape.splits) * chunk);
     a.splits = (int)cdiv(K, a.depth);
     a.part_ld = (int64_t)up(N, 4);
     a.part = a.splits > 1 ? ws.take<float>((size_t)a.splits * M * a.part_ld) : nullptr;

@@ -245,6 +245,31 @@ def test_nan_stays_in_its_row():
             assert y[1].isnan().all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2:]).all()
 
 
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("m,k,n", [(20, 600, 300), (300, 500, 400)])
+def test_small_backward_rounds_only_its_results(t, m, k, n):
+    """products this small keep what the rounding of d to 16 bits leaves: what is left of the error is the results' own rounding, and a hundredth for the
+    sums, the slopes (2^-20 of dy) and the second piece's rounding (2^-11 of half a step in fp16, 2^-8 in bf16)"""
+    dy, x, w, z = normal(1, m, n, t=t, by=0.05), normal(2, m, k, t=t), normal(3, n, k, t=t, by=k ** -0.5), normal(4, m, n, t=t)
+    d = dy.double() * slope64(z.double(), "gelu")
+    dx, dw, _ = ops.linear_backward(dy, x, w, z, activation="gelu")
+    for out, ref in ((dx, mm(d, w.double())), (dw, mm(d.t(), x.double()))):
+        assert float((out.double() - ref).norm()) <= 1.01 * float((ref.to(t).double() - ref).norm())
+
+
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("m", [8, 600])
+def test_an_infinite_d_stays_infinite(t, m):
+    """of both ways: d past the type's range (fp16: 65504 x 1.1), and an infinite dy"""
+    dy, x, w = normal(1, m, 40, t=t, by=0.05), normal(2, m, 32, t=t), torch.full((40, 32), 0.5, dtype=t, device=DEV)
+    z = torch.full((m, 40), 1.5, dtype=t, device=DEV)             # (gelu's and silu's slope is more than 1 there)
+    dy[1, 3], dy[2, 5] = torch.finfo(t).max, float("inf")
+    for act in ("gelu", "relu"):
+        dx, _, _ = ops.linear_backward(dy, x, w, z, activation=act)
+        assert torch.isfinite(dx[0]).all() and torch.isfinite(dx[3:]).all()
+        assert bool((dx[2] == float("inf")).all()) and bool((dx[1] > 0).all())
+
+
 # ---- 8-bit checkpoints ----------------------------------------------------------------------------------------------
 def in8(x, code):
     """what the header says, in 64 bits: blocks of 32, the least power of two, nearest code with ties to even, the type's range kept"""

@@ -311,6 +311,29 @@ EmbedScratch embed_scratch(Scratch& ws, const SortPlan& s, int64_t tokens, int64
     e.part = ws.take<float>((size_t)2 * s.sums * e.part_ld);
     return e;
 }
+// Tables of few rows, for their own two kernels.  Eight tokens of a slice at least, and enough to be worth a table's way through memory; four workgroups
+// for each CU at most
+bool few_rows(int64_t rows, int width) { return rows <= kFewIds && rows * width <= kFewValues; }
+struct FewPlan { int lanes, slices, per; int64_t blocks, part_ld; unsigned columns; };
+FewPlan few_plan(int64_t tokens, int64_t rows, int width) {
+    FewPlan f;
+    const int64_t all = cdiv(width, 4);
+    f.columns = (unsigned)cdiv(all, 256);
+    f.lanes = (int)(all < 256 ? all : 256);
+    f.slices = 256 / f.lanes;
+    const int64_t most = f.columns < 1024 ? 1024 / f.columns : 1, even = cdiv(tokens, f.slices * most), worth = cdiv(4 * rows, f.slices);
+    f.per = (int)up((size_t)(even > worth ? even : worth), 8);
+    f.blocks = cdiv(tokens, (int64_t)f.slices * f.per);
+    f.part_ld = (int64_t)up(width, 4);
+    return f;
+}
+template <typename T>
+void few_sums(hipStream_t st, const FewPlan& f, const void* ids, int id_type, int64_t tokens, int rows, int width, const void* dy, int64_t lddy, float scale, void* dt,
+              int64_t ldt, float* part) {
+    few_sum_kernel<T><<<dim3((unsigned)f.blocks, f.columns), 256, (size_t)rows * 257 * 16, st>>>(ids, id_type, tokens, rows, f.per, Div::by((unsigned)f.lanes), f.slices, width,
+                                                                                        (const T*)dy, lddy, part, f.part_ld);
+    few_join_kernel<T><<<(unsigned)cdiv(rows * f.part_ld, 64), 256, 0, st>>>(part, f.part_ld, (int)f.blocks, rows, width, scale, (T*)dt, ldt);
+}
 ccsm_status check_embedding(int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int width) {
     REFUSE(!good_type(type), "embedding: unknown type");
     REFUSE(id_type < CCSM_ID_U8 || id_type > CCSM_ID_I64, "embedding: unknown type of ids");
@@ -394,7 +417,10 @@ ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int6
 size_t ccsm_train_embedding_backward_workspace(int type, int64_t tokens, int64_t rows, int32_t width) {
     if (!good_type(type) || tokens <= 0 || tokens > kMostRows || rows <= 0 || rows > kMostRows || width <= 0 || width > kMostCols) return 0;
     Scratch ws;
-    (void)embed_scratch(ws, sort_plan(type, tokens, rows, width), tokens, rows, width);
+    if (few_rows(rows, width)) {
+        const FewPlan f = few_plan(tokens, rows, width);
+        ws.take<float>((size_t)f.blocks * rows * f.part_ld);
+    } else (void)embed_scratch(ws, sort_plan(type, tokens, rows, width), tokens, rows, width);
     return ws.used;
 }
 ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
@@ -414,6 +440,13 @@ ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int
     }
     Scratch ws;
     ws.base = (char*)workspace;
+    if (few_rows(rows, width)) {
+        const FewPlan f = few_plan(tokens, rows, width);
+        float* part = ws.take<float>((size_t)f.blocks * rows * f.part_ld);
+        TYPED(type, few_sums<T>(st, f, ids, id_type, tokens, (int)rows, width, dy, lddy, scale, dtable, ldt, part));
+        LAUNCHED("embedding_backward");
+        return CCSM_OK;
+    }
     const SortPlan s = sort_plan(type, tokens, rows, width);
     const EmbedScratch b = embed_scratch(ws, s, tokens, rows, width);
     int k = 0;

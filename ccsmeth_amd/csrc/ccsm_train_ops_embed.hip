@@ -6,6 +6,8 @@
 // border goes to two partial rows of the workspace (its head, its tail), which a second kernel adds in a fixed order.  Rows of the table that no
 // token names are marked by the sort's last pass (a byte for each row) and cleared by further workgroups of the sums' launch, so the table
 // is written once.  No floating-point atomics: the order of a sum depends on the ids alone.
+//
+// Tables of a few rows (bases, strands, segments) are not sorted for: every lane adds its tokens up in its own copy of the table's columns.
 #include "ccsm_train_ops_common.h"
 
 namespace ccsm_ops {
@@ -369,6 +371,92 @@ __global__ __launch_bounds__(256) void join_kernel(const unsigned* keys, long lo
             store_row<T, 4>(dt + (long long)k * ldt + c, width - c, v);
         }
     }
+}
+
+// ---- tables of few rows ----------------------------------------------------------------------------------------------
+// A lane has four neighbouring columns of every row in LDS (rows x 16 bytes) and adds to them the tokens of its slice, `per` of them, each `slices`
+// behind the last, eight in flight.  Then the slices of the workgroup are added up, and few_join_kernel adds the workgroups' tables.  No atomics; the
+// order of a sum depends on the sizes and ids alone.  Two launches, where the sort's way has four at
+// least.  Measured (fp32, us a call with its host part, sort -> here): 5 x 8 21 -> 13.6 at 21504 tokens, 48 -> 19.5 at a million; 2 x 1024 60 -> 30 at 21504.
+// Larger tables leave too few waves on a CU (15 x 256 24 -> 19 at 21504 tokens, but 316 -> 442 at a million; 15 x 1024 37 -> 52).
+constexpr int kFewIds = 15, kFewValues = 2048;             // (62 KB of LDS at most)
+template <typename T>
+__global__ __launch_bounds__(256) void few_sum_kernel(const void* ids, int id_type, long long n, int rows, int per, Div lanes, int slices, int width, const T* dy,
+                                                      long long lddy, float* part, long long part_ld) {
+    typedef Vec<float, 4> V;
+    extern __shared__ __align__(16) char room[];
+    V* tab = (V*)room;                                     // [rows][257]
+    const int j = (int)lanes.of(threadIdx.x), lane = (int)threadIdx.x - j * (int)lanes.d, c = (int)blockIdx.y * 1024 + 4 * lane;
+    for (int r = 0; r < rows; ++r) tab[r * 257 + threadIdx.x] = V{};
+    const long long base = (long long)blockIdx.x * slices * per + j;
+    if (j < slices && c < width) {
+        for (int b = 0; b < per; b += 8) {
+            unsigned id[8];
+            Loose<T, 4> v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const long long t = base + (long long)(b + q) * slices;
+                id[q] = t < n ? id_at(ids, id_type, t, rows) : (unsigned)rows;
+                if (t < n) v[q] = raw_row<T, 4>(dy + t * lddy + c, width - c);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (id[q] < (unsigned)rows) {
+                    V o = tab[id[q] * 257 + threadIdx.x];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o.v[k] += (float)v[q].v[k];
+                    tab[id[q] * 257 + threadIdx.x] = o;
+                }
+        }
+    }
+    __syncthreads();
+    // `many` lanes for each four columns of a row: each adds slices g, g + many, ... into slice g, the first of them those
+    const int cells = rows * (int)lanes.d, many = cells >= 256 ? 1 : 256 / cells < slices ? 256 / cells : slices;
+    for (int pass = 0; pass < 2; ++pass) {
+        const int step = pass ? 1 : many, end = pass ? many : slices, use = pass ? cells : cells * many;
+        for (int e = threadIdx.x; e < use; e += 256) {
+            const int g = e / cells, cell = e - g * cells, r = (int)lanes.of(cell), l = cell - r * (int)lanes.d;
+            V o = tab[r * 257 + g * (int)lanes.d + l];
+            for (int w = g + step; w < end; w += step) {
+                const V a = tab[r * 257 + w * (int)lanes.d + l];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o.v[k] += a.v[k];
+            }
+            const int col = (int)blockIdx.y * 1024 + 4 * l;
+            if (pass == 0) tab[r * 257 + g * (int)lanes.d + l] = o;
+            else if (col < width) *(V*)(part + ((long long)blockIdx.x * rows + r) * part_ld + col) = o;
+        }
+        __syncthreads();
+    }
+}
+// a workgroup: 16 lanes of four columns of the table, 16 slices of the parts
+template <typename T>
+__global__ __launch_bounds__(256) void few_join_kernel(const float* part, long long part_ld, int parts, int rows, int width, float scale, T* dt, long long ldt) {
+    typedef Vec<float, 4> V;
+    __shared__ V sum[16][16];
+    const int lane = threadIdx.x & 15, slice = threadIdx.x >> 4;
+    const long long quarter = part_ld / 4, cell = (long long)blockIdx.x * 16 + lane, all = rows * quarter;
+    V o = {};
+    if (cell < all)
+#pragma unroll 4
+        for (int p = slice; p < parts; p += 16) {
+            const V a = *(const V*)(part + 4 * (p * all + cell));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o.v[k] += a.v[k];
+        }
+    sum[slice][lane] = o;
+    __syncthreads();
+    if (slice != 0 || cell >= all) return;
+    for (int w = 1; w < 16; ++w) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o.v[k] += sum[w][lane].v[k];
+    }
+    const long long r = cell / quarter;
+    const int c = 4 * (int)(cell - r * quarter);
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = o.v[k] == 0.f ? 0.f : o.v[k] * scale;
+    store_row<T, 4>(dt + r * ldt + c, width - c, v);
 }
 
 }  // namespace ccsm_ops

@@ -371,6 +371,24 @@ def test_embedding(t, tokens, rows, width):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens,rows,width", [(1, 15, 1), (7, 1, 2048), (300, 15, 4), (5000, 15, 136), (5000, 16, 128), (20000, 2, 1024), (20000, 3, 1024), (300, 15, 137), (40000, 15, 33), (200001, 5, 8)])
+def test_embedding_of_few_rows(t, tokens, rows, width):
+    """tables that are not sorted for, up to their largest and one more row; a gradient and a table with strides of their own"""
+    g = torch.Generator().manual_seed(rows)
+    ids = torch.randint(-1, rows + 1, (tokens,), generator=g)
+    if rows > 2:
+        ids[ids == 1] = 2                                             # a row that no token names
+    ids = ids.to(torch.int32).to(DEV)
+    table, dy = normal(1, rows, width + 3, t=t)[:, 1:1 + width], normal(2, tokens, width + 5, t=t, by=0.1)[:, 3:3 + width]
+    check_embedding(ids, table, dy, 0.5, ops.embedding(ids, table, 0.5), ops.embedding_backward(dy, ids, rows, 0.5), t)
+    nan = dy.clone()
+    nan[0] = float("nan")
+    got = ops.embedding_backward(nan, ids, rows, 0.5)
+    at = int(ids[0])
+    assert torch.isfinite(got[[r for r in range(rows) if r != at]].float()).all() and (not 0 <= at < rows or got[at].isnan().all())
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_embedding_extremes(t):
     """every token the same; every token another one; none; the last row only; ids beyond 32 bits; rows that no token names"""
     tokens, width = 9000, 24

@@ -93,14 +93,23 @@ bool whole_rows(const void* p, int64_t ld, int64_t width, int type) {
     const int64_t n = 16 / (int64_t)size_of(type);
     return !off_by(p, 16) && ld % n == 0 && width % n == 0 && ld < (1 << 21);      // (the kernels' 32-bit offsets span a tile's rows)
 }
-template <typename T>
-Plane staged(const Saved& s, int64_t rows, int64_t width, Scratch& ws, hipStream_t st, bool count) {
-    if (s.code == kCodeNone && whole_rows(s.data, s.ld, width, TypeOf<T>::v)) return Plane{s.data, s.ld};
-    const int64_t ld = (int64_t)up(width, 8);
-    T* out = ws.take<T>((size_t)rows * ld);
-    if (!count) stage_kernel<T><<<grid_of(cdiv(rows * ld / 8, 256), 1 << 16), 256, 0, st>>>(s, rows, (int)width, out, ld);
-    return Plane{out, ld};
-}
+// (both operands' copies in one launch: 3 us and a gap of 2 each)
+struct Staging {
+    StageJob jobs[2] = {};
+    int count = 0;
+    template <typename T> Plane of(const Saved& s, int64_t rows, int64_t width, Scratch& ws) {
+        if (s.code == kCodeNone && whole_rows(s.data, s.ld, width, TypeOf<T>::v)) return Plane{s.data, s.ld};
+        const int64_t ld = (int64_t)up(width, 8);
+        T* out = ws.take<T>((size_t)rows * ld);
+        jobs[count++] = StageJob{s, rows * ld / 8, (int)width, out, ld};
+        return Plane{out, ld};
+    }
+    template <typename T> hipError_t launch(hipStream_t st) const {
+        if (!count) return hipSuccess;
+        stage_kernel<T><<<grid_of(cdiv(jobs[0].items + jobs[1].items, 256), 1 << 16), 256, 0, st>>>(jobs[0], jobs[1]);
+        return hipGetLastError();
+    }
+};
 
 template <typename T, bool TRP, bool TRQ, int B>
 hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
@@ -200,7 +209,9 @@ ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bo
         TRY((direct<T, false, false>(st, plain(p->x, p->ldx), plain(p->x, p->ldx), CCSM_ACT_NONE, plain(p->w, p->ldw), p->rows, p->outer, p->inner, nullptr, ep)), "linear_forward");
         return CCSM_OK;
     }
-    const Plane x = staged<T>(plain(p->x, p->ldx), p->rows, p->inner, ws, st, count), w = staged<T>(plain(p->w, p->ldw), p->outer, p->inner, ws, st, count);
+    Staging stage;
+    const Plane x = stage.of<T>(plain(p->x, p->ldx), p->rows, p->inner, ws), w = stage.of<T>(plain(p->w, p->ldw), p->outer, p->inner, ws);
+    if (!count) TRY(stage.launch<T>(st), "linear_forward");
     TRY((product<T, false, false>(st, x, w, p->rows, p->outer, p->inner, ep, ws, count)), "linear_forward");
     return CCSM_OK;
 }
@@ -261,14 +272,11 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 8), 256, 0, st>>>(part, (int)parts, N, (T*)p->dbias);
         LAUNCHED("linear_backward");
     }
-    if (p->dx) {
-        const Plane w = staged<T>(plain(p->w, p->ldw), N, K, ws, st, count);
-        TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, count)), "linear_backward: dx");
-    }
-    if (p->dw) {
-        const Plane x = staged<T>(saved_of(p->x), M, K, ws, st, count);
-        TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, count)), "linear_backward: dw");
-    }
+    Staging stage;
+    const Plane w = p->dx ? stage.of<T>(plain(p->w, p->ldw), N, K, ws) : Plane{}, x = p->dw ? stage.of<T>(saved_of(p->x), M, K, ws) : Plane{};
+    if (!count) TRY(stage.launch<T>(st), "linear_backward");
+    if (p->dx) TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, count)), "linear_backward: dx");
+    if (p->dw) TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, count)), "linear_backward: dw");
     return CCSM_OK;
 }
 

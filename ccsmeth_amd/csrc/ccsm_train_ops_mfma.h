@@ -515,16 +515,20 @@ __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int wi
     for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
 }
 
-// a kept matrix as rows of whole 16-byte pieces in the call's type (zeros behind the width)
+// kept matrices as rows of whole 16-byte pieces in the call's type (zeros behind the width); an item is eight values
+struct StageJob { Saved from; long long items; int width; void* out; long long ld; };
 template <typename T>
-__global__ __launch_bounds__(256) void stage_kernel(Saved s, long long rows, int width, T* out, long long ld) {
-    const int n = (int)(ld / 8);
-    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < rows * n; x += (long long)gridDim.x * 256) {
-        const long long r = x / n;
-        const int c = (int)(x % n) * 8;
+__global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) {
+    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < a.items + b.items; x += (long long)gridDim.x * 256) {
+        const bool first = x < a.items;
+        const StageJob& job = first ? a : b;
+        const long long i = first ? x : x - a.items;
+        const int n = (int)(job.ld / 8);
+        const long long r = i >> 32 ? i / n : (unsigned)i / (unsigned)n;
+        const int c = (int)(i - r * n) * 8;
         float v[8];
-        load8<T>(s, r, c, width, v);
-        store_row<T, 8>(out + r * ld + c, 8, v);
+        load8<T>(job.from, r, c, job.width, v);
+        store_row<T, 8>((T*)job.out + r * job.ld + c, 8, v);
     }
 }
 

@@ -78,18 +78,20 @@ __device__ __forceinline__ float sigmoid_(float z) { return rcp_<FAST>(1.f + exp
 template <bool FAST>
 __device__ __forceinline__ float tanh_(float z) {
     if (!FAST) return tanhf(z);
-    // 1 - 2 / (1 + e^2|z|); below 2^-4 that loses bits, and z - z^3 / 3 + 2 z^5 / 15 is within 2^-20 z
-    const float a = fabsf(z), t = 1.f - 2.f * rcp_<true>(1.f + exp_<true>(2.f * a)), q = z * z;
-    return a < 0.0625f ? z * (1.f + q * (-0.33333333f + q * 0.13333333f)) : copysignf(t, z);
+    // 1 - 2 / (1 + e^2z); below 2^-6 that loses bits (2^-24 / |z|), and z - z^3 / 3 is within 2^-27 z
+    const float t = 1.f - 2.f * rcp_<true>(1.f + __builtin_amdgcn_exp2f(2.88539008f * z));
+    return fabsf(z) < 0.015625f ? z - z * z * z * 0.33333333f : t;
 }
 // the normal distribution's Phi(z), and e^(-z^2 / 2) (the library's erfc keeps its relative accuracy in the lower tail)
 template <bool FAST>
 __device__ __forceinline__ float phi_(float z, float* e) {
-    const float x = fabsf(z) * 0.70710678f;
-    *e = exp_<FAST>(-0.5f * z * z);
-    if (!FAST) return 0.5f * erfcf(-z * 0.70710678118654752f);
-    const float t = rcp_<true>(1.f + 0.3275911f * x);
-    const float q = 0.5f * *e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    if (!FAST) {
+        *e = expf(-0.5f * z * z);
+        return 0.5f * erfcf(-z * 0.70710678118654752f);
+    }
+    *e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+    const float t = rcp_<true>(1.f + 0.23164190f * fabsf(z));      // (the formula's 0.3275911 |z| / sqrt 2; its coefficients halved)
+    const float q = *e * t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
     return z >= 0.f ? 1.f - q : q;
 }
 template <bool FAST, int N>

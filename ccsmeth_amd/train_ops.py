@@ -46,7 +46,8 @@ class LinearGrad(C.Structure):
 # the two structures as bytes (the header's layout): one pack call is a third of what filling a ctypes structure costs per call
 _LINEAR = struct.Struct("@iiqiiPqPqPPqPqPq")
 _GRAD = struct.Struct("@iiqiiPqPqiPqPqPqiPqPqPqP")
-assert _LINEAR.size == C.sizeof(Linear) and _GRAD.size == C.sizeof(LinearGrad)
+_SAVED = struct.Struct("@PqiPq")
+assert _LINEAR.size == C.sizeof(Linear) and _GRAD.size == C.sizeof(LinearGrad) and _SAVED.size == C.sizeof(Saved)
 _NONE = (0, 0, 0, 0, 0)
 
 _ops = None
@@ -70,7 +71,7 @@ def load():
     lib.ccsm_train_embedding_backward_workspace.restype = cs
     lib.ccsm_train_embedding_backward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp, cs, vp]
     lib.ccsm_train_act8_pack.argtypes = [ci, ci, ci, cl, C.c_int32, vp, cl, vp, cl, vp, cl, vp]
-    lib.ccsm_train_act8_unpack.argtypes = [ci, ci, cl, C.c_int32, C.POINTER(Saved), vp, cl, vp]
+    lib.ccsm_train_act8_unpack.argtypes = [ci, ci, cl, C.c_int32, vp, vp, cl, vp]
     _ops = lib
     return lib
 
@@ -85,15 +86,15 @@ def _types():
     return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}, {torch.uint8: 0, torch.int32: 1, torch.int64: 2}
 
 
-_TYPE = _ID = _torch = None
+_TYPE = _ID = _torch = _Tensor = None
 
 
 def _init():
-    global _TYPE, _ID, _torch
+    global _TYPE, _ID, _torch, _Tensor
     if _torch is None:
         import torch
         _TYPE, _ID = _types()
-        _torch = torch
+        _torch, _Tensor = torch, torch.Tensor
     return _torch
 
 
@@ -117,10 +118,27 @@ def _on_gpu(t, name):
         raise ValueError("%s must be on a GPU: there is no CPU path" % name)
 
 
+# A call of one token is bound by the host (10 us, of which the launch is 3): the two checks below see in a few attributes that nothing is wrong, and
+# leave it to the ones above to say what is.
+def _lead(t, name):
+    """the type and the device's number of a call's first tensor"""
+    if type(t) is not _Tensor or t.dtype not in _TYPE or t.requires_grad or not t.is_cuda:
+        _tensor(t, name)
+        _on_gpu(t, name)
+    return t.dtype, t.get_device()
+
+
+def _same(t, name, dtype, at, lead):
+    """t, of the call's type and on its device"""
+    if type(t) is _Tensor and t.dtype is dtype and t.get_device() == at and not t.requires_grad:
+        return t
+    return _tensor(t, name, dtype, lead.device)
+
+
 def _rows(t):
-    """(2-D view or copy with contiguous rows, its row stride)"""
-    if t.dim() == 2 and t.is_contiguous():
-        return t, t.shape[1]
+    """(tensor whose rows are contiguous, its row stride): t as it is, or a copy"""
+    if t.is_contiguous() and t.dim():
+        return t, t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1]) if t.dim() else t.reshape(1, 1)
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
@@ -147,12 +165,12 @@ def _elsewhere(call, stream, device, given, *args, **kw):
     return out
 
 
-def _raw_stream(device):
-    return _torch._C._cuda_getCurrentRawStream(device.index)
+def _raw_stream(at):
+    return _torch._C._cuda_getCurrentRawStream(at)
 
 
-def _scratch(n, device):
-    return _torch.empty(n, dtype=_torch.uint8, device=device) if n else None
+def _scratch(n, lead):
+    return lead.new_empty(n, dtype=_torch.uint8) if n else None
 
 
 def _ptr(t):
@@ -163,6 +181,13 @@ def _activation(name):
     if name not in ACTIVATIONS:
         raise ValueError("activation must be one of %s, not %r" % (", ".join(ACTIVATIONS), name))
     return ACTIVATIONS[name]
+
+
+def _library():
+    if _ops is None or _torch is None:
+        _init()
+        load()
+    return _ops
 
 
 def _out(out, shape, dtype, device, name):
@@ -207,99 +232,99 @@ class Checkpoint8:
         return self.codes.numel() + self.scales.numel()
 
     def _saved(self):
-        return self.codes.data_ptr(), self.codes.shape[1], CODES[self.code], self.scales.data_ptr(), self.scales.shape[1]
+        blocks = (self.shape[-1] + 31) // 32
+        return self.codes.data_ptr(), 32 * blocks, CODES[self.code], self.scales.data_ptr(), blocks
 
     def values(self, dtype=None, *, out=None, stream=None):
         """The values that the codes stand for, as a tensor of `dtype` (default: the type it was made of, which holds them exactly)."""
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _TYPE:
             raise ValueError("dtype must be float32, float16 or bfloat16, not %s" % dtype)
-        lib = load()
-        _on_gpu(self.codes, "the checkpoint")
-        dev = self.device
+        lib = _library()
+        codes, shape = self.codes, self.shape
+        _on_gpu(codes, "the checkpoint")
         if stream is not None:
-            return _elsewhere(self.values, stream, dev, (self, out), dtype, out=out)
-        y = _torch.empty(self.shape, dtype=dtype, device=dev) if out is None else _out(out, self.shape, dtype, dev, "out")
-        y2, ldy = _rows(y)
-        s = Saved(*self._saved())
-        _check(lib.ccsm_train_act8_unpack(dev.index, _TYPE[dtype], y2.shape[0], y2.shape[1], C.byref(s), y2.data_ptr(), ldy, _raw_stream(dev)))
+            return _elsewhere(self.values, stream, self.device, (self, out), dtype, out=out)
+        if out is None:
+            y, width = codes.new_empty(shape, dtype=dtype), shape[-1]
+            ldy = width
+        else:
+            y, width = _out(out, shape, dtype, self.device, "out"), shape[-1]
+            ldy = _rows(y)[1]
+        at = codes.get_device()
+        _check(lib.ccsm_train_act8_unpack(at, _TYPE[dtype], codes.shape[0], width, _SAVED.pack(*self._saved()), y.data_ptr(), ldy, _raw_stream(at)))
         return y
 
 
 def checkpoint8(x, code="int8", *, stream=None):
     """x (..., width) -> Checkpoint8: blocks of 32 values of a row share a power of two; "int8" keeps 127 even steps either side of zero (bounded
     activations, normalised inputs), "e4m3" three bits behind the leading one (long-tailed ones)."""
-    torch = _init()
-    lib = load()
+    lib = _library()
     if code not in CODES:
         raise ValueError("code must be one of %s, not %r" % (", ".join(CODES), code))
-    _tensor(x, "x")
-    _on_gpu(x, "x")
-    if x.dim() == 0 or x.shape[-1] < 1:
+    t, at = _lead(x, "x")
+    shape = x.shape
+    if not shape or shape[-1] < 1:
         raise ValueError("x must have at least one column")
-    dev = x.device
     if stream is not None:
-        return _elsewhere(checkpoint8, stream, dev, (x,), x, code)
+        return _elsewhere(checkpoint8, stream, x.device, (x,), x, code)
     x2, ldx = _rows(x)
-    rows, width = x2.shape
-    blocks = -(-width // 32)
-    codes = torch.empty((rows, 32 * blocks), dtype=torch.uint8, device=dev)
-    scales = torch.empty((rows, blocks), dtype=torch.uint8, device=dev)
-    _check(lib.ccsm_train_act8_pack(dev.index, _TYPE[x.dtype], CODES[code], rows, width, x2.data_ptr(), ldx, codes.data_ptr(), 32 * blocks, scales.data_ptr(), blocks,
-                                    _raw_stream(dev)))
+    width = shape[-1]
+    rows, blocks, u8 = x.numel() // width, (width + 31) // 32, _torch.uint8
+    codes, scales = x.new_empty((rows, 32 * blocks), dtype=u8), x.new_empty((rows, blocks), dtype=u8)
+    _check(lib.ccsm_train_act8_pack(at, _TYPE[t], CODES[code], rows, width, x2.data_ptr(), ldx, codes.data_ptr(), 32 * blocks, scales.data_ptr(), blocks, _raw_stream(at)))
     c = Checkpoint8.__new__(Checkpoint8)                    # (what __init__ checks holds here)
-    c.codes, c.scales, c.shape, c.dtype, c.code = codes, scales, x.shape, x.dtype, code
+    c.codes, c.scales, c.shape, c.dtype, c.code = codes, scales, shape, t, code
     return c
 
 
 def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=False, *, out=None, stream=None):
     """y = act(x weight^T + bias) + residual; x (..., inner), weight (outer, inner), bias (outer), residual and y (..., outer).
     keep_preact: -> (y, z) with z = x weight^T + bias as linear_backward takes it.  out: where y goes (it may be the residual)."""
-    _init()
-    lib = load()
+    lib = _library()
     act = _activation(activation)
-    t, dev = _tensor(x, "x").dtype, x.device
-    _on_gpu(x, "x")
-    _tensor(weight, "weight", t, dev)
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError("x must be (..., inner) and weight (outer, inner): got %s and %s" % (tuple(x.shape), tuple(weight.shape)))
-    outer, inner = weight.shape
+    t, at = _lead(x, "x")
+    _same(weight, "weight", t, at, x)
+    given, both = x.shape, weight.shape
+    if len(both) != 2 or not given or given[-1] != both[1]:
+        raise ValueError("x must be (..., inner) and weight (outer, inner): got %s and %s" % (tuple(given), tuple(both)))
+    outer, inner = both
     if inner < 1 or outer < 1:
         raise ValueError("weight has no rows or no columns")
-    shape = x.shape[:-1] + (outer,)
-    if bias is not None and tuple(_tensor(bias, "bias", t, dev).shape) != (outer,):
+    shape = given[:-1] + (outer,)
+    if bias is not None and _same(bias, "bias", t, at, x).shape != (outer,):
         raise ValueError("bias must be (%d,)" % outer)
-    if residual is not None and _tensor(residual, "residual", t, dev).shape != shape:
+    if residual is not None and _same(residual, "residual", t, at, x).shape != shape:
         raise ValueError("residual must be %s" % (tuple(shape),))
     if stream is not None:
-        return _elsewhere(linear, stream, dev, (x, weight, bias, residual, out), x, weight, bias, residual, activation, keep_preact, out=out)
-    empty = _torch.empty
-    y = empty(shape, dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
-    z = empty(shape, dtype=t, device=dev) if keep_preact else None
+        return _elsewhere(linear, stream, x.device, (x, weight, bias, residual, out), x, weight, bias, residual, activation, keep_preact, out=out)
+    y, ldy = (x.new_empty(shape), outer) if out is None else _rows(_out(_tensor(out, "out"), shape, t, x.device, "out"))
+    z = x.new_empty(shape) if keep_preact else None
     x2, ldx = _rows(x)
     w2, ldw = _rows(weight)
     b1 = None if bias is None else bias.contiguous()
-    y2, ldy = _rows(y)
     r2, ldr = (None, 0) if residual is None else _rows(residual)
-    p = _LINEAR.pack(_TYPE[t], act, x2.shape[0], inner, outer, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b1), _ptr(r2), ldr, y2.data_ptr(), ldy, _ptr(z), outer)
+    p = _LINEAR.pack(_TYPE[t], act, x.numel() // inner, inner, outer, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b1), _ptr(r2), ldr, y.data_ptr(), ldy, _ptr(z), outer)
     need = lib.ccsm_train_linear_workspace(p)
-    ws = _scratch(need, dev)
-    _check(lib.ccsm_train_linear_forward(dev.index, p, _ptr(ws), need, _raw_stream(dev)))
+    ws = _scratch(need, x)
+    _check(lib.ccsm_train_linear_forward(at, p, _ptr(ws), need, _raw_stream(at)))
+    if out is not None:
+        y = out
     return (y, z) if keep_preact else y
 
 
 def linear_backward(dy, x, weight, preact=None, activation="none", *, need_dx=True, need_dw=True, need_db=True, stream=None):
     """The gradients of y = act(x weight^T + bias) (+ residual, whose gradient is dy itself): (dx, dw, db), None for what is not needed.
     dy (..., outer); x (..., inner) and preact (..., outer) are tensors or Checkpoint8s; preact only where there is an activation."""
-    _init()
-    lib = load()
+    lib = _library()
     act = _activation(activation)
-    t, dev = _tensor(dy, "dy").dtype, dy.device
-    _on_gpu(dy, "dy")
-    _tensor(weight, "weight", t, dev)
-    if weight.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != weight.shape[0]:
-        raise ValueError("dy must be (..., outer) and weight (outer, inner): got %s and %s" % (tuple(dy.shape), tuple(weight.shape)))
-    outer, inner = weight.shape
+    t, at = _lead(dy, "dy")
+    _same(weight, "weight", t, at, dy)
+    given, both = dy.shape, weight.shape
+    if len(both) != 2 or not given or given[-1] != both[0]:
+        raise ValueError("dy must be (..., outer) and weight (outer, inner): got %s and %s" % (tuple(given), tuple(both)))
+    outer, inner = both
+    lead = given[:-1]
     if inner < 1 or outer < 1:
         raise ValueError("weight has no rows or no columns")
     if act and preact is None:
@@ -308,86 +333,80 @@ def linear_backward(dy, x, weight, preact=None, activation="none", *, need_dx=Tr
     def saved(v, cols, name):
         if v is None:
             return _NONE, None
-        if tuple(v.shape) != tuple(dy.shape[:-1]) + (cols,):
-            raise ValueError("%s must be %s, not %s" % (name, tuple(dy.shape[:-1]) + (cols,), tuple(v.shape)))
+        if v.shape != lead + (cols,):
+            raise ValueError("%s must be %s, not %s" % (name, tuple(lead) + (cols,), tuple(v.shape)))
         if isinstance(v, Checkpoint8):
-            if v.device != dev:
-                raise ValueError("%s is on %s, not on %s" % (name, v.device, dev))
+            if v.codes.get_device() != at:
+                raise ValueError("%s is on %s, not on %s" % (name, v.device, dy.device))
             if v.dtype is not t:
                 raise ValueError("%s was made of %s, the call's type is %s" % (name, v.dtype, t))
             return v._saved(), None
-        v2, ld = _rows(_tensor(v, name, t, dev))
+        v2, ld = _rows(_same(v, name, t, at, dy))
         return (v2.data_ptr(), ld, 0, 0, 0), v2
 
     if need_dw and x is None:
         raise ValueError("x is needed for dw")
     if stream is not None:
-        return _elsewhere(linear_backward, stream, dev, (dy, x, weight, preact), dy, x, weight, preact, activation, need_dx=need_dx, need_dw=need_dw, need_db=need_db)
-    empty = _torch.empty
+        return _elsewhere(linear_backward, stream, dy.device, (dy, x, weight, preact), dy, x, weight, preact, activation, need_dx=need_dx, need_dw=need_dw, need_db=need_db)
     xs, _x = saved(x if need_dw else None, inner, "x")
     zs, _z = saved(preact if act else None, outer, "preact")
-    dx = empty(dy.shape[:-1] + (inner,), dtype=t, device=dev) if need_dx else None
-    dw = empty((outer, inner), dtype=t, device=dev) if need_dw else None
-    db = empty((outer,), dtype=t, device=dev) if need_db else None
+    dx = dy.new_empty(lead + (inner,)) if need_dx else None
+    dw = dy.new_empty((outer, inner)) if need_dw else None
+    db = dy.new_empty(outer) if need_db else None
     d2, ldd = _rows(dy)
     w2, ldw = _rows(weight)
-    p = _GRAD.pack(_TYPE[t], act, d2.shape[0], inner, outer, d2.data_ptr(), ldd, *xs, w2.data_ptr(), ldw, *zs, _ptr(dx), inner, _ptr(dw), inner, _ptr(db))
+    p = _GRAD.pack(_TYPE[t], act, dy.numel() // outer, inner, outer, d2.data_ptr(), ldd, *xs, w2.data_ptr(), ldw, *zs, _ptr(dx), inner, _ptr(dw), inner, _ptr(db))
     need = lib.ccsm_train_linear_backward_workspace(p)
-    ws = _scratch(need, dev)
-    _check(lib.ccsm_train_linear_backward(dev.index, p, _ptr(ws), need, _raw_stream(dev)))
+    ws = _scratch(need, dy)
+    _check(lib.ccsm_train_linear_backward(at, p, _ptr(ws), need, _raw_stream(at)))
     return dx, dw, db
 
 
-def _ids(ids, device):
-    torch = _torch
-    if not isinstance(ids, torch.Tensor) or ids.dtype not in _ID:
+def _ids(ids, at, lead):
+    if not isinstance(ids, _Tensor) or ids.dtype not in _ID:
         raise ValueError("ids must be a uint8, int32 or int64 tensor")
-    if ids.device != device:
-        raise ValueError("ids are on %s, not on %s" % (ids.device, device))
+    if ids.get_device() != at:
+        raise ValueError("ids are on %s, not on %s" % (ids.device, lead.device))
     return ids.contiguous()
 
 
 def embedding(ids, table, scale=1.0, *, out=None, stream=None):
     """y (*ids.shape, width) = scale * table[ids].  Ids outside [0, len(table)), padding of -1 for instance, give a row of zeros."""
-    _init()
-    lib = load()
-    t, dev = _tensor(table, "table").dtype, table.device
-    _on_gpu(table, "table")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+    lib = _library()
+    t, at = _lead(table, "table")
+    both = table.shape
+    if len(both) != 2 or both[0] < 1 or both[1] < 1:
         raise ValueError("table must be (rows, width)")
     if stream is not None:
-        return _elsewhere(embedding, stream, dev, (ids, table, out), ids, table, scale, out=out)
-    i = _ids(ids, dev)
-    shape = ids.shape + (table.shape[1],)
-    y = _torch.empty(shape, dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), shape, t, dev, "out")
+        return _elsewhere(embedding, stream, table.device, (ids, table, out), ids, table, scale, out=out)
+    i = _ids(ids, at, table)
+    rows, width = both
+    shape = ids.shape + (width,)
+    y, ldy = (table.new_empty(shape), width) if out is None else _rows(_out(_tensor(out, "out"), shape, t, table.device, "out"))
     t2, ldt = _rows(table)
-    y2, ldy = _rows(y)
-    _check(lib.ccsm_train_embedding_forward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), t2.shape[0], t2.shape[1], t2.data_ptr(), ldt, float(scale), y2.data_ptr(),
-                                            ldy, _raw_stream(dev)))
-    return y
+    _check(lib.ccsm_train_embedding_forward(at, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), rows, width, t2.data_ptr(), ldt, float(scale), y.data_ptr(), ldy, _raw_stream(at)))
+    return y if out is None else out
 
 
 def embedding_backward(dy, ids, rows, scale=1.0, *, out=None, stream=None):
     """The gradient of embedding()'s table, (rows, width) in dy's type: row v = scale * the sum of dy's rows whose id is v, zero where there is none.
     A row's sum has one order, that of its tokens: the same inputs give the same bits."""
-    _init()
-    lib = load()
-    t, dev = _tensor(dy, "dy").dtype, dy.device
-    _on_gpu(dy, "dy")
+    lib = _library()
+    t, at = _lead(dy, "dy")
     rows = int(rows)
     if rows < 1:
         raise ValueError("rows must be at least 1")
-    if dy.dim() < 1 or dy.shape[-1] < 1 or not hasattr(ids, "shape") or dy.shape[:-1] != ids.shape:
+    given = dy.shape
+    if not given or given[-1] < 1 or not hasattr(ids, "shape") or given[:-1] != ids.shape:
         raise ValueError("dy must be (*ids.shape, width)")
-    width = dy.shape[-1]
     if stream is not None:
-        return _elsewhere(embedding_backward, stream, dev, (dy, ids, out), dy, ids, rows, scale, out=out)
-    i = _ids(ids, dev)
-    dt = _torch.empty((rows, width), dtype=t, device=dev) if out is None else _out(_tensor(out, "out"), _torch.Size((rows, width)), t, dev, "out")
+        return _elsewhere(embedding_backward, stream, dy.device, (dy, ids, out), dy, ids, rows, scale, out=out)
+    width = given[-1]
+    i = _ids(ids, at, dy)
+    dt, ldt = (dy.new_empty((rows, width)), width) if out is None else _rows(_out(_tensor(out, "out"), _torch.Size((rows, width)), t, dy.device, "out"))
     d2, ldd = _rows(dy)
-    t2, ldt = _rows(dt)
-    need = lib.ccsm_train_embedding_backward_workspace(_TYPE[t], i.numel(), rows, width)
-    ws = _scratch(need, dev)
-    _check(lib.ccsm_train_embedding_backward(dev.index, _TYPE[t], _ID[i.dtype], i.numel(), i.data_ptr(), rows, width, d2.data_ptr(), ldd, float(scale), t2.data_ptr(), ldt,
-                                             _ptr(ws), need, _raw_stream(dev)))
-    return dt
+    kind, n = _TYPE[t], i.numel()
+    need = lib.ccsm_train_embedding_backward_workspace(kind, n, rows, width)
+    ws = _scratch(need, dy)
+    _check(lib.ccsm_train_embedding_backward(at, kind, _ID[i.dtype], n, i.data_ptr(), rows, width, d2.data_ptr(), ldd, float(scale), dt.data_ptr(), ldt, _ptr(ws), need, _raw_stream(at)))
+    return dt if out is None else out

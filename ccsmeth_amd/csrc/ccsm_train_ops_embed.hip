@@ -110,7 +110,7 @@ template <int Q>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const void* ids, int id_type, const unsigned* keys, const unsigned* at, long long n, long long rows, int shift,
                                                            int bins, const unsigned* starts, unsigned* keys_out, unsigned* at_out, uint8_t* marks) {
     __shared__ unsigned next[4][256];
-    __shared__ unsigned wave_sum[4];
+    __shared__ unsigned wave_sum[4], sums[2][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int d = threadIdx.x; d < 1024; d += 256) (&next[0][0])[d] = 0;
     __syncthreads();
@@ -128,12 +128,26 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const void* ids, int 
     unsigned start = 0;
     if (gridDim.x <= kFewBlocks) {
         unsigned all = 0;
-        if ((int)threadIdx.x < bins) {
-#pragma unroll 16
-            for (int b = 0; b < (int)gridDim.x; ++b) {
-                const unsigned t = starts[b * bins + threadIdx.x];
-                all += t;
-                start += b < (int)blockIdx.x ? t : 0;
+        const int groups = 256 / bins, d = threadIdx.x & (bins - 1);                  // (bins: a power of two, at most 256; every lane sums up)
+        for (int b0 = 0; b0 < (int)gridDim.x; b0 += 16 * groups) {                    // (uniform trips, loads without a condition: sixteen in flight)
+            unsigned t[16];
+            const int b = b0 + threadIdx.x / bins;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) t[q] = starts[min(b + q * groups, (int)gridDim.x - 1) * bins + d];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                all += b + q * groups < (int)gridDim.x ? t[q] : 0;
+                start += b + q * groups < (int)blockIdx.x ? t[q] : 0;
+            }
+        }
+        if (groups > 1) {
+            sums[0][threadIdx.x] = all;
+            sums[1][threadIdx.x] = start;
+            __syncthreads();
+            all = start = 0;
+            for (int q = 0; q < groups && (int)threadIdx.x < bins; ++q) {
+                all += sums[0][q * bins + threadIdx.x];
+                start += sums[1][q * bins + threadIdx.x];
             }
         }
         unsigned s = all;

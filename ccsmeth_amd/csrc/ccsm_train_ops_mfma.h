@@ -513,6 +513,10 @@ __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int wi
     else { decode4<kCodeE4m3>(u.x, k, a); decode4<kCodeE4m3>(u.y, k, b); }
 #pragma unroll
     for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+    if (width - c < 8) {                                   // (codes behind the width are whatever the caller left there, NaN's too)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = c + q < width ? v[q] : 0.f;
+    }
 }
 
 // kept matrices as rows of whole 16-byte pieces in the call's type (zeros behind the width); an item is eight values

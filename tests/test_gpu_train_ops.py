@@ -154,6 +154,20 @@ def test_backward_from_checkpoints(t, xc, zc, m, k, n):
     check_backward(dy, in8(x, xc) if xc else x, w, in8(z, zc) if zc else z, "silu", t, got)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", [(40, 20, 41), (1500, 43, 299)])
+def test_codes_behind_the_width_do_not_matter(t, m, k, n):
+    """a caller's own checkpoints, the codes behind whose width stand for NaN"""
+    dy, w = normal(1, m, n, t=t, by=0.05), normal(3, n, k, t=t, by=0.2)
+    x, z = (ops.checkpoint8(normal(4, m, c, t=t), code) for c, code in ((k, "int8"), (n, "e4m3")))
+    want = ops.linear_backward(dy, x, w, z, activation="silu")
+    for c, nan in ((x, 0x80), (z, 0x7f)):
+        c.codes[:, c.shape[-1]:] = nan
+    for a, b in zip(want, ops.linear_backward(dy, x, w, z, activation="silu")):
+        assert torch.equal(a, b) and torch.isfinite(a.float()).all()
+    assert torch.isfinite(x.values().float()).all()
+
+
 def test_backward_only_what_is_asked_for():
     dy, x, w, z = normal(1, 40, 24), normal(2, 40, 16), normal(3, 24, 16), normal(4, 40, 24)
     full = ops.linear_backward(dy, x, w, z, activation="tanh")

@@ -3,6 +3,7 @@
 // block of 32 exchange their largest magnitudes, and 16 codes leave as one aligned piece.  A power of two per block instead of any factor: the
 // division and the values are exact, so packing values that came from codes gives the same codes, and a product can take them as bf16
 // (or in the type that was packed) without a second rounding.
+// Measured (86016 x 512 bf16, int8): packing 21.8 us (133 MB at 6.1 TB/s, part of it still in the last-level cache), values 32 us (4.2 TB/s).
 #include "ccsm_train_ops_common.h"
 
 namespace ccsm_ops {

@@ -238,6 +238,7 @@ __global__ __launch_bounds__(256, 4) void piece_sum_kernel(const unsigned* keys,
             }
         };
         ahead(s);
+        const bool whole = width - c >= N;
         const unsigned before = s > 0 ? keys[s - 1] : ~0u, after = e < n ? keys[e] : ~0u;
         float acc[N];
 #pragma unroll
@@ -267,9 +268,15 @@ __global__ __launch_bounds__(256, 4) void piece_sum_kernel(const unsigned* keys,
             Loose<T, N> v[kAhead];
             unsigned now[kAhead];
 #pragma unroll
-            for (int q = 0; q < kAhead; ++q) {
-                now[q] = k[q];
-                if (now[q] < rows) v[q] = raw_row<T, N>(dy + (long long)from[q] * lddy + c, width - c);
+            for (int q = 0; q < kAhead; ++q) now[q] = k[q];
+            if (now[0] < rows) {                           // (sorted: tokens of no row are the last ones)
+                if (whole) {                               // eight loads without a condition between them
+#pragma unroll
+                    for (int q = 0; q < kAhead; ++q) v[q] = *reinterpret_cast<const Loose<T, N>*>(dy + (long long)from[q] * lddy + c);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < kAhead; ++q) v[q] = raw_row<T, N>(dy + (long long)from[q] * lddy + c, width - c);
+                }
             }
             if (kPiece > kAhead && b + kAhead < e) ahead(b + kAhead);
 #pragma unroll

@@ -33,16 +33,20 @@ __global__ __launch_bounds__(256) void lookup_kernel(const void* ids, int id_typ
         c[u] = (int)((i < items ? i : 0) - t[u] * pieces.d) * N;
         id[u] = id_at(ids, id_type, t[u], rows);
     }
-    float v[U][N];
+    Loose<T, N> r[U];                                      // (no token: the table's first row, not used; no condition between the loads)
+    if (width % N == 0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (id[u] < rows) load_row<T, N>(table + (long long)id[u] * ldt + c[u], width - c[u], v[u]);
+        for (int u = 0; u < U; ++u) r[u] = *reinterpret_cast<const Loose<T, N>*>(table + (long long)(id[u] < rows ? id[u] : 0) * ldt + c[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = raw_row<T, N>(table + (long long)(id[u] < rows ? id[u] : 0) * ldt + c[u], width - c[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+        float v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[u][k] = id[u] < rows ? v[u][k] * scale : 0.f;
-        if (first + 256u * u < items) store_row<T, N>(y + (long long)t[u] * ldy + c[u], width - c[u], v[u]);
+        for (int k = 0; k < N; ++k) v[k] = id[u] < rows ? (float)r[u].v[k] * scale : 0.f;
+        if (first + 256u * u < items) store_row<T, N>(y + (long long)t[u] * ldy + c[u], width - c[u], v);
     }
 }
 
@@ -205,7 +209,7 @@ constexpr int kLongPiece = 32, kShortPiece = 8;
 // Measured (65536 x 1024 bf16 over 50000 rows, 15.5 thousand of them met, from memory): 84 us, 236 MB at 2.8 TB/s, the sort in front 25, the join behind 11.
 // Clearing first, or between the sums, takes 5 and 25 us more; pieces of 8, 16, 64 tokens 7, 2, 25.
 template <typename T, int N, int kPiece>
-__global__ __launch_bounds__(256, 4) void piece_sum_kernel(const unsigned* keys, const unsigned* at, long long n, long long rows, unsigned sums, int groups, Div lanes, int width,
+__global__ __launch_bounds__(256, 3) void piece_sum_kernel(const unsigned* keys, const unsigned* at, long long n, long long rows, unsigned sums, int groups, Div lanes, int width,
                                                         const T* dy, long long lddy, float scale, T* dt, long long ldt, float* part, long long part_ld, const uint8_t* marks,
                                                         unsigned* list) {
     const int c0 = blockIdx.y * 256 * N;

@@ -199,10 +199,18 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, in
     if (!a.part && a.ep.bias && left_j > 0) load_row<T, 8>((const T*)a.ep.bias + j, left_j, bias);
     Loose<T, 8> r[2][kIt];
     auto residual = [&](int h, Loose<T, 8> (&o)[kIt]) {
+        const T* p[kIt];
 #pragma unroll
-        for (int q = 0; q < kIt; ++q) {
+        for (int q = 0; q < kIt; ++q) {                    // (rows behind the last one read that one: no condition between the loads)
             const int i = iw + 32 * h + q * kRowsIt;
-            if (i < a.M) o[q] = raw_row<T, 8>((const T*)a.ep.residual + (long long)i * a.ep.ldr + j, left_j);
+            p[q] = (const T*)a.ep.residual + (long long)(i < a.M ? i : a.M - 1) * a.ep.ldr + j;
+        }
+        if (left_j >= 8) {
+#pragma unroll
+            for (int q = 0; q < kIt; ++q) o[q] = *reinterpret_cast<const Loose<T, 8>*>(p[q]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < kIt; ++q) o[q] = raw_row<T, 8>(p[q], left_j);
         }
     };
     if (res) residual(0, r[0]);
@@ -519,6 +527,24 @@ __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int wi
     }
 }
 
+// the same of R rows, all of them requested before the first is used
+template <typename T, int R>
+__device__ __forceinline__ void load8s(const Saved& s, const long long (&r)[R], int c, int width, float (&v)[R][8]) {
+    if (s.code == kCodeNone && width - c >= 8) {
+        Loose<T, 8> t[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) t[q] = *reinterpret_cast<const Loose<T, 8>*>((const T*)s.data + r[q] * s.ld + c);
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[q][k] = (float)t[q].v[k];
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < R; ++q) load8<T>(s, r[q], c, width, v[q]);
+    }
+}
+
 // kept matrices as rows of whole 16-byte pieces in the call's type (zeros behind the width); an item is eight values
 struct StageJob { Saved from; long long items; int width; void* out; long long ld; };
 template <typename T>
@@ -551,14 +577,11 @@ __global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, 
     float acc[8] = {};
     if (c < N) {
         float v[4][8], u[4][8];
+        long long r[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (m0 + 8 * q < M) load8<T>(dy, m0 + 8 * q, c, N, v[q]);
-        if (act != kActNone) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (m0 + 8 * q < M) load8<T>(z, m0 + 8 * q, c, N, u[q]);
-        }
+        for (int q = 0; q < 4; ++q) r[q] = m0 + 8 * q < M ? m0 + 8 * q : M - 1;      // (no condition between the loads)
+        load8s<T, 4>(dy, r, c, N, v);
+        if (act != kActNone) load8s<T, 4>(z, r, c, N, u);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (m0 + 8 * q >= M) break;

@@ -223,20 +223,28 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, in
             for (int q = 0; q < FJ; ++q) *(f32x4*)(out + (16 * (p & 1) + (lane & 15)) * kRow + 16 * q + 4 * (lane >> 4)) = acc[p][q];
         }
         if (res && h + 1 < FI / 2) residual(h + 1, r[1]);
-        if (left_j > 0) {
+        static_assert(kIt % 2 == 0, "two pieces at a time");
 #pragma unroll
-            for (int q = 0; q < kIt; ++q) {
-                const int i = iw + 32 * h + q * kRowsIt;
-                const float* o = out + (lane / kPer + q * kRowsIt) * kRow + c;
-                const f32x4 u = *(const f32x4*)o, v = *(const f32x4*)(o + 4);
+        for (int q0 = 0; q0 < kIt; q0 += 2) {              // (two pieces read at a time; all four at once do not fit into the registers)
+            f32x4 u[2], v[2];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const float* o = out + (lane / kPer + (q0 + d) * kRowsIt) * kRow + c;
+                u[d] = *(const f32x4*)o;
+                v[d] = *(const f32x4*)(o + 4);
+            }
+            if (left_j <= 0) continue;
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const int i = iw + 32 * h + (q0 + d) * kRowsIt;
                 if (i >= a.M) continue;
                 if (a.part) {
                     float* g = a.part + ((long long)split * a.M + i) * a.part_ld + j;
-                    *(f32x4*)g = u;
-                    if (left_j > 4) *(f32x4*)(g + 4) = v;
+                    *(f32x4*)g = u[d];
+                    if (left_j > 4) *(f32x4*)(g + 4) = v[d];
                 } else {
-                    float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-                    finish<T, 8>(a.ep, i, j, left_j, z, bias, r[0][q]);
+                    float z[8] = {u[d][0], u[d][1], u[d][2], u[d][3], v[d][0], v[d][1], v[d][2], v[d][3]};
+                    finish<T, 8>(a.ep, i, j, left_j, z, bias, r[0][q0 + d]);
                 }
             }
         }
@@ -507,6 +515,19 @@ __global__ __launch_bounds__(256) void product_join_kernel(const float* part, in
     }
 }
 
+// the values of eight codes; those behind the width are whatever the caller left there, NaN's too: zeros
+__device__ __forceinline__ void decode8(int code, uint2 u, uint8_t scale, int left, float (&v)[8]) {
+    const float k = pow2_of_byte(scale);
+    float a[4], b[4];
+    if (code == kCodeInt8) { decode4<kCodeInt8>(u.x, k, a); decode4<kCodeInt8>(u.y, k, b); }
+    else { decode4<kCodeE4m3>(u.x, k, a); decode4<kCodeE4m3>(u.y, k, b); }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
+    if (left < 8) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < left ? v[q] : 0.f;
+    }
+}
 // eight values of row r from column c on, zeros beyond the width
 template <typename T>
 __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int width, float (&v)[8]) {
@@ -514,19 +535,8 @@ __device__ __forceinline__ void load8(const Saved& s, long long r, int c, int wi
         load_row<T, 8>((const T*)s.data + r * s.ld + c, width - c, v);
         return;
     }
-    const uint2 u = *(const uint2*)((const uint8_t*)s.data + r * s.ld + c);      // (a code row covers whole blocks of 32, 16-byte aligned)
-    const float k = pow2_of_byte(s.scales[r * s.lds + (c >> 5)]);
-    float a[4], b[4];
-    if (s.code == kCodeInt8) { decode4<kCodeInt8>(u.x, k, a); decode4<kCodeInt8>(u.y, k, b); }
-    else { decode4<kCodeE4m3>(u.x, k, a); decode4<kCodeE4m3>(u.y, k, b); }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) { v[q] = a[q]; v[4 + q] = b[q]; }
-    if (width - c < 8) {                                   // (codes behind the width are whatever the caller left there, NaN's too)
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = c + q < width ? v[q] : 0.f;
-    }
+    decode8(s.code, *(const uint2*)((const uint8_t*)s.data + r * s.ld + c), s.scales[r * s.lds + (c >> 5)], width - c, v);      // (a code row covers whole blocks of 32)
 }
-
 // the same of R rows, all of them requested before the first is used
 template <typename T, int R>
 __device__ __forceinline__ void load8s(const Saved& s, const long long (&r)[R], int c, int width, float (&v)[R][8]) {
@@ -539,6 +549,16 @@ __device__ __forceinline__ void load8s(const Saved& s, const long long (&r)[R], 
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[q][k] = (float)t[q].v[k];
         }
+    } else if (s.code != kCodeNone) {
+        uint2 t[R];
+        uint8_t k[R];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+            t[q] = *(const uint2*)((const uint8_t*)s.data + r[q] * s.ld + c);
+            k[q] = s.scales[r[q] * s.lds + (c >> 5)];
+        }
+#pragma unroll
+        for (int q = 0; q < R; ++q) decode8(s.code, t[q], k[q], width - c, v[q]);
     } else {
 #pragma unroll
         for (int q = 0; q < R; ++q) load8<T>(s, r[q], c, width, v[q]);

@@ -40,11 +40,12 @@ struct OnDevice {
     if (on_device_.err != hipSuccess) return hip_fail(on_device_.err, "hipSetDevice")
 
 // Where direct_kernel takes a product: forward ones of at most 64 rows, and products of at most 2^27 multiplications whose contraction is short, since
-// its steps follow each other without a tile's prefetch.  Measured (bf16 | fp32, us a call, tile way -> direct): 512^3 forward 12.8 -> 11.0 |
-// 24.6 -> 11.5, gradients 40 -> 30 | 66 -> 54; 255^3 forward 19 -> 13 | 22 -> 12, gradients 50 -> 33 | 90 -> 53; beyond: 1024^3 forward
-// 17.7 -> 25.6 | 38 -> 63; 128 x 128 with a contraction of 4096 forward 15.7 -> 21.8, as a gradient 22 -> 75; results of 13377 x 768 (stored in
-// pieces of 16 columns) 26 -> 51.
+// its steps follow each other without a tile's prefetch.  Measured (bf16 | fp32, us on the GPU, tile way -> direct): 512^3 forward 10.4 -> 6.0 |
+// 16.2 -> 8.9, gradients 25 -> 23 | 41 -> 33; 300 x 700 x 300 forward 15.9 -> 6.2 | 12.8 -> 9.3, gradients 29.5 -> 22 | 36 -> 32; beyond: 1024^3 forward
+// 13.8 -> 24 | 30 -> 53; a contraction of 4096 (128 x 128 results) 11 -> 20.5 | 14.5 -> 39; gradients of 2000 x 64 x 1000 32 -> 65 | 44 -> 87;
+// results of 13377 x 768 (stored in pieces of 16 columns) 26 -> 51.
 constexpr int64_t kFewRows = 64, kSmallProduct = 1 << 27, kSmallResult = 1 << 21, kShortForward = 1024, kShortBackward = 512;
+constexpr int64_t kNarrow = 1 << 21;                              // row strides that the kernels' 32-bit offsets span
 constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
 
 size_t size_of(int type) { return type == CCSM_TYPE_F32 ? 4 : 2; }
@@ -91,7 +92,7 @@ Saved plain(const void* p, int64_t ld) { return Saved{p, ld, kCodeNone, nullptr,
 // scratch (8-bit codes too: the values that they stand for)
 bool whole_rows(const void* p, int64_t ld, int64_t width, int type) {
     const int64_t n = 16 / (int64_t)size_of(type);
-    return !off_by(p, 16) && ld % n == 0 && width % n == 0 && ld < (1 << 21);      // (the kernels' 32-bit offsets span a tile's rows)
+    return !off_by(p, 16) && ld % n == 0 && width % n == 0 && ld < kNarrow;
 }
 // (both operands' copies in one launch: 3 us and a gap of 2 each)
 struct Staging {
@@ -181,7 +182,7 @@ hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, in
 
 bool small_product(int64_t M, int64_t N, int64_t K) { return M * N <= kSmallResult && M * N * K <= kSmallProduct; }
 template <typename T, bool TRP, bool TRQ>
-hipError_t direct(hipStream_t st, const Saved& p, const Saved& z, int act, const Saved& q, int64_t M, int64_t N, int64_t K, void* sums, const Epilogue& ep) {
+hipError_t direct(hipStream_t st, const Plane& p, const Plane& z, int act, const Plane& q, int64_t M, int64_t N, int64_t K, void* sums, const Epilogue& ep) {
     DirectArgs a{p, z, q, act, M, N, K, 1, sums, ep};
     while (a.kw < 8 && 32 * 2 * a.kw <= K) a.kw *= 2;             // (a wave has a whole step of 32 at least)
     const int mt = M <= 16 ? 1 : 4;
@@ -206,7 +207,7 @@ ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bo
     const Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
     if (p->rows <= kFewRows || (p->inner <= kShortForward && small_product(p->rows, p->outer, p->inner))) {
         if (count) return CCSM_OK;
-        TRY((direct<T, false, false>(st, plain(p->x, p->ldx), plain(p->x, p->ldx), CCSM_ACT_NONE, plain(p->w, p->ldw), p->rows, p->outer, p->inner, nullptr, ep)), "linear_forward");
+        TRY((direct<T, false, false>(st, Plane{p->x, p->ldx}, Plane{p->x, p->ldx}, CCSM_ACT_NONE, Plane{p->w, p->ldw}, p->rows, p->outer, p->inner, nullptr, ep)), "linear_forward");
         return CCSM_OK;
     }
     Staging stage;
@@ -251,12 +252,18 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         return CCSM_OK;
     }
     const Epilogue to_dx{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, to_dw{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone};
-    if (M <= kShortBackward && N <= kShortBackward && small_product(M, N, K)) {
+    const bool narrow = p->lddy < kNarrow && (!p->dx || p->ldw < kNarrow) && (p->activation == CCSM_ACT_NONE || p->preact.ld < kNarrow) && (!p->dw || p->x.ld < kNarrow);
+    if (narrow && M <= kShortBackward && N <= kShortBackward && small_product(M, N, K)) {
+        // checkpoints are made values in a launch of their own: a lane would read them code by code along the rows (bf16, both operands in 8 bits, us a
+        // backward pass: 512^3 52 -> 28, 64 x 512 x 512 43 -> 23)
+        Staging stage;
+        auto values = [&](const ccsm_saved& v, int width) { return v.code == kCodeNone ? Plane{v.data, v.ld} : stage.of<T>(saved_of(v), M, width, ws); };
+        const Plane dy{p->dy, p->lddy}, z = p->activation == CCSM_ACT_NONE ? dy : values(p->preact, N), x = p->dw ? values(p->x, K) : dy;
         if (count) return CCSM_OK;
-        const Saved dy = plain(p->dy, p->lddy), z = p->activation == CCSM_ACT_NONE ? dy : saved_of(p->preact);
-        if (p->dx) TRY((direct<T, false, true>(st, dy, z, p->activation, plain(p->w, p->ldw), M, K, N, nullptr, to_dx)), "linear_backward: dx");
+        TRY(stage.launch<T>(st), "linear_backward");
+        if (p->dx) TRY((direct<T, false, true>(st, dy, z, p->activation, Plane{p->w, p->ldw}, M, K, N, nullptr, to_dx)), "linear_backward: dx");
         if (p->dw || p->dbias)                                     // (the bias gradient comes with dw's product, or by the same sums without it)
-            TRY((direct<T, true, true>(st, dy, z, p->activation, p->dw ? saved_of(p->x) : dy, N, p->dw ? K : 1, M, p->dbias, to_dw)), "linear_backward: dw");
+            TRY((direct<T, true, true>(st, dy, z, p->activation, x, N, p->dw ? K : 1, M, p->dbias, to_dw)), "linear_backward: dw");
         return CCSM_OK;
     }
     // d as the products take it: dy itself where there is no activation and its rows are whole pieces

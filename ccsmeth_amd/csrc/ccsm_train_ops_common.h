@@ -217,20 +217,9 @@ __device__ __forceinline__ void decode4(unsigned u, float scale, float (&v)[4]) 
         v[j] = q == -128 ? __builtin_nanf("") : (float)q * scale;
     }
 }
-__device__ __forceinline__ float decode1(int code, unsigned byte, float scale) {
-    if (code == kCodeE4m3) return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0) * scale;
-    const int q = (int)(signed char)byte;
-    return q == -128 ? __builtin_nanf("") : (float)q * scale;
-}
-
-// element (row, col) of a kept matrix in type T, or of its codes
+// a matrix that a forward pass has kept, in the call's type or as codes
 struct Saved {
     const void* data; long long ld; int code; const uint8_t* scales; long long lds;
 };
-template <typename T>
-__device__ __forceinline__ float saved_at(const Saved& s, long long row, long long col) {
-    if (s.code == kCodeNone) return (float)((const T*)s.data)[row * s.ld + col];
-    return decode1(s.code, ((const uint8_t*)s.data)[row * s.ld + col], pow2_of_byte(s.scales[row * s.lds + (col >> 5)]));
-}
 
 }  // namespace ccsm_ops

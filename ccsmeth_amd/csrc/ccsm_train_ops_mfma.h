@@ -629,13 +629,13 @@ __global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, 
 
 // ---- small products and few rows ------------------------------------------------------------------------------------
 // The same products straight from memory into the matrix instructions' operands, without staging, LDS or a kernel in front: any type, alignment and
-// storage form, checkpoints and an activation's slope included.  A wave owns 16 j x 16 MT i; a workgroup's eight waves share the contraction (kw of
+// storage form, an activation's slope included.  A wave owns 16 j x 16 MT i; a workgroup's eight waves share the contraction (kw of
 // them) and the i between them; their sums are added in order through LDS.  fp32: the three bf16 parts of each operand are made in
 // registers.
-// For up to 64 rows it is bound by reading w once (1 x 512 x 768 bf16: 3.8 us; the tile kernel 9.8, four steps through LDS by six of 256 CUs); for
+// For up to 64 rows it is bound by reading w once (1 x 512 x 768 bf16: 3.6 us; the tile kernel 9.8, four steps through LDS by six of 256 CUs); for
 // small products by its one launch (the tile kernel's way takes up to three for a product and eight for a backward pass).
 struct DirectArgs {
-    Saved P, Z, Q;                // Z, act: P's elements are multiplied by act'(Z)
+    Plane P, Z, Q;                // Z, act: P's elements are multiplied by act'(Z)
     int act;
     long long M, N, K;
     int kw;                       // waves along k: 1, 2, 4 or 8
@@ -671,25 +671,22 @@ __global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
             }
         }
     };
-    // eight neighbours along k of one row (TR: column) of a kept matrix, zeros behind its end
-    auto eight = [&](const Saved& s, bool tr, long long r, long long k) -> Loose<T, 8> {
+    // eight neighbours along k of one row (TR: column) of a matrix, zeros behind its end.  TR: one address for all lanes and k, 32 bits for a lane's own
+    // part (addresses of 64 bits for each of 72 loads do not fit into the registers); strides are below 2^21
+    auto eight = [&](const Plane& s, bool tr, long long r, long long k0, unsigned kl) -> Loose<T, 8> {
+        const long long k = k0 + kl;
         const int left = (int)(a.K - k < 8 ? a.K - k : 8);
-        if (s.code == kCodeNone) {
-            if (!tr) return raw_row<T, 8>((const T*)s.data + r * s.ld + k, left);
-            Loose<T, 8> o;
-            const T* p = (const T*)s.data + k * s.ld + r;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) o.v[q] = q < left ? p[q * s.ld] : (T)0.f;
-            return o;
-        }
+        if (!tr) return raw_row<T, 8>((const T*)s.base + r * s.ld + k, left);
         Loose<T, 8> o;
+        const char* p = (const char*)s.base + k0 * s.ld * (long long)sizeof(T);
+        const unsigned own = (kl * (unsigned)s.ld + (unsigned)r) * (unsigned)sizeof(T);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) o.v[q] = q < left ? (T)saved_at<T>(s, tr ? k + q : r, tr ? r : k + q) : (T)0.f;
+        for (int q = 0; q < 8; ++q) o.v[q] = q < left ? *(const T*)(p + q * s.ld * (long long)sizeof(T) + own) : (T)0.f;
         return o;
     };
     // v becomes v act'(z), rounded, and `low` what the rounding leaves: both are multiplied, so that a 16-bit product here is as exact as one of the
     // unrounded v act'(z) (the tile kernels' is rounded once: an error of 0.21e-3 of the values in fp16, beside the result's own of as
-    // much).  The second piece costs 1 us of 25 (512 x 256 -> 128, a backward pass in fp16)
+    // much).  The second piece costs 1 us of 25
     auto sloped = [&](Loose<T, 8>& v, const Loose<T, 8>& z, Loose<T, 8>& low, float& t) {
         float u[8];
 #pragma unroll
@@ -706,57 +703,73 @@ __global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
             }
         }
     };
-    auto multiply = [&](const Loose<T, 8>& qv, const Loose<T, 8> (&pv)[MT]) {
-        s16x8 x[NP], y[NP];
-        pieces(qv, x);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            pieces(pv[t], y);
-            if constexpr (NP == 3) {
-                acc[t] = Mfma<E>::run(x[2], y[0], acc[t]);
-                acc[t] = Mfma<E>::run(x[0], y[2], acc[t]);
-                acc[t] = Mfma<E>::run(x[1], y[1], acc[t]);
-                acc[t] = Mfma<E>::run(x[1], y[0], acc[t]);
-                acc[t] = Mfma<E>::run(x[0], y[1], acc[t]);
-            }
-            acc[t] = Mfma<E>::run(x[0], y[0], acc[t]);
+    auto multiply = [&](const s16x8 (&x)[NP], const Loose<T, 8>& p, f32x4& c) {
+        s16x8 y[NP];
+        pieces(p, y);
+        if constexpr (NP == 3) {
+            c = Mfma<E>::run(x[2], y[0], c);
+            c = Mfma<E>::run(x[0], y[2], c);
+            c = Mfma<E>::run(x[1], y[1], c);
+            c = Mfma<E>::run(x[1], y[0], c);
+            c = Mfma<E>::run(x[0], y[1], c);
         }
+        c = Mfma<E>::run(x[0], y[0], c);
     };
     const bool slope = a.act != kActNone, want = a.sums != nullptr && blockIdx.x == 0;
     const int step = 32 * a.kw;
-    long long k0 = 0, k = wk * 32 + 8 * (lane >> 4);
-    if (!TRP && !TRQ && !slope && a.P.code == kCodeNone && a.Q.code == kCodeNone) {       // four steps of whole pieces in flight
-        for (; k0 + step * U <= a.K; k0 += step * U, k += step * U) {
+    long long k0 = 0;
+    const unsigned kl = wk * 32 + 8 * (lane >> 4);
+    if (!TRP && !TRQ && !slope) {       // four steps of whole pieces in flight
+        for (; k0 + step * U <= a.K; k0 += step * U) {
+            const long long k = k0 + kl;
             Loose<T, 8> qv[U], pv[U][MT];
 #pragma unroll
-            for (int u = 0; u < U; ++u) qv[u] = *reinterpret_cast<const Loose<T, 8>*>((const T*)a.Q.data + j * a.Q.ld + k + step * u);
+            for (int u = 0; u < U; ++u) qv[u] = *reinterpret_cast<const Loose<T, 8>*>((const T*)a.Q.base + j * a.Q.ld + k + step * u);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) pv[u][t] = *reinterpret_cast<const Loose<T, 8>*>((const T*)a.P.data + i[t] * a.P.ld + k + step * u);
+                for (int t = 0; t < MT; ++t) pv[u][t] = *reinterpret_cast<const Loose<T, 8>*>((const T*)a.P.base + i[t] * a.P.ld + k + step * u);
 #pragma unroll
-            for (int u = 0; u < U; ++u) multiply(qv[u], pv[u]);
+            for (int u = 0; u < U; ++u) {
+                s16x8 x[NP];
+                pieces(qv[u], x);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) multiply(x, pv[u][t], acc[t]);
+            }
         }
     }
-    for (; k0 < a.K; k0 += step, k += step) {
-        Loose<T, 8> pv[MT], zv[MT], low[MT];
+    for (; k0 < a.K; k0 += step) {
         Loose<T, 8> qv = {};
-        if (a.ep.y) qv = eight(a.Q, TRQ, j, k);
+        s16x8 x[NP];
+        if (a.ep.y) qv = eight(a.Q, TRQ, j, k0, kl);
+        constexpr int G = TRP && MT > 2 ? 2 : MT;          // (rows in flight: four columns of each of P and Z, element by element, spill)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) pv[t] = eight(a.P, TRP, i[t], k);
-        if (slope) {
+        for (int t0 = 0; t0 < MT; t0 += G) {
+            Loose<T, 8> pv[G], zv[G];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) zv[t] = eight(a.Z, TRP, i[t], k);
+            for (int t = 0; t < G; ++t) pv[t] = eight(a.P, TRP, i[t0 + t], k0, kl);
+            if (slope) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) sloped(pv[t], zv[t], low[t], tot[t]);
-            if constexpr (sizeof(T) == 2) multiply(qv, low);
-        } else if (want) {
+                for (int t = 0; t < G; ++t) zv[t] = eight(a.Z, TRP, i[t0 + t], k0, kl);
+            }
+            if (t0 == 0) pieces(qv, x);
+            if (slope) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+                for (int t = 0; t < G; ++t) {
+                    Loose<T, 8> low;
+                    sloped(pv[t], zv[t], low, tot[t0 + t]);
+                    if constexpr (sizeof(T) == 2) multiply(x, low, acc[t0 + t]);
+                }
+            } else if (want) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) tot[t] += (float)pv[t].v[q];
+                for (int t = 0; t < G; ++t)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) tot[t0 + t] += (float)pv[t].v[q];
+            }
+#pragma unroll
+            for (int t = 0; t < G; ++t) multiply(x, pv[t], acc[t0 + t]);
+            if (G < MT) __builtin_amdgcn_sched_barrier(0);
         }
-        multiply(qv, pv);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) sum[wave][t][lane] = acc[t];

@@ -222,6 +222,20 @@ def test_strides_and_alignment(t, m, k, n):
         assert torch.equal(a, c)
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("which", ["dy", "x", "w", "z"])
+def test_rows_far_apart(t, which):
+    """row strides past the kernels' 32-bit offsets"""
+    m, k, n = 20, 24, 40
+    dy, x, w, z = normal(1, m, n, t=t, by=0.05), normal(2, m, k, t=t), normal(3, n, k, t=t, by=0.2), normal(4, m, n, t=t)
+    given = {"dy": dy, "x": x, "w": w, "z": z}
+    far = torch.zeros(given[which].shape[0], (1 << 21) + 8, dtype=t, device=DEV)[:, :given[which].shape[1]]
+    far.copy_(given[which])
+    given[which] = far
+    check_linear(given["x"], given["w"], None, None, "gelu", t, ops.linear(given["x"], given["w"], activation="gelu"))
+    check_backward(dy, x, w, z, "silu", t, ops.linear_backward(given["dy"], given["x"], given["w"], given["z"], activation="silu"))
+
+
 def test_residual_may_be_the_output():
     for t in TYPES:
         for m in (2, 200):

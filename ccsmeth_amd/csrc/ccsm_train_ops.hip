@@ -105,9 +105,10 @@ struct Staging {
         jobs[count++] = StageJob{s, rows * ld / 8, (int)width, out, ld};
         return Plane{out, ld};
     }
+    unsigned blocks() const { return grid_of(cdiv(jobs[0].items + jobs[1].items, 256), 1 << 16); }
     template <typename T> hipError_t launch(hipStream_t st) const {
         if (!count) return hipSuccess;
-        stage_kernel<T><<<grid_of(cdiv(jobs[0].items + jobs[1].items, 256), 1 << 16), 256, 0, st>>>(jobs[0], jobs[1]);
+        stage_kernel<T><<<blocks(), 256, 0, st>>>(jobs[0], jobs[1]);
         return hipGetLastError();
     }
 };
@@ -156,9 +157,9 @@ Shape shape_of(int64_t M, int64_t N, int64_t chunks, bool f32) {
     }
     return best;
 }
-// out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue
+// out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue; with parts, what is left to add up goes to *join
 template <typename T, bool TRP, bool TRQ>
-hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, bool count) {
+hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, JoinJob* join, bool count) {
     ProductArgs a;
     a.P = p; a.Q = q;
     a.M = (int)M; a.N = (int)N; a.K = (int)K;
@@ -173,9 +174,14 @@ hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, in
     a.part_ld = (int64_t)up(N, 4);
     a.part = a.splits > 1 ? ws.take<float>((size_t)a.splits * M * a.part_ld) : nullptr;
     if (count) return hipSuccess;
-    hipError_t e = B == 256 ? launch_product<T, TRP, TRQ, 256>(a, st) : launch_product<T, TRP, TRQ, 128>(a, st);
-    if (e != hipSuccess || a.splits == 1) return e;
-    product_join_kernel<T><<<grid_of(cdiv(M * cdiv(N, 4), 256), 1 << 16), 256, 0, st>>>(a.part, a.splits, M, (int)N, a.part_ld, ep);
+    if (a.splits > 1) *join = JoinJob{a.part, a.splits, M, (int)N, a.part_ld, ep, grid_of(cdiv(M * cdiv(N, 4), 256), 1 << 16)};
+    return B == 256 ? launch_product<T, TRP, TRQ, 256>(a, st) : launch_product<T, TRP, TRQ, 128>(a, st);
+}
+template <typename T>
+hipError_t joins(hipStream_t st, const ColumnJob& c, const JoinJob& a, const JoinJob& b) {
+    const unsigned blocks = c.blocks + a.blocks + b.blocks;
+    if (!blocks) return hipSuccess;
+    joins_kernel<T><<<blocks, 256, 0, st>>>(c, a, b);
     return hipGetLastError();
 }
 #define TRY(x, what) do { hipError_t e_ = (x); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
@@ -213,7 +219,9 @@ ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bo
     Staging stage;
     const Plane x = stage.of<T>(plain(p->x, p->ldx), p->rows, p->inner, ws), w = stage.of<T>(plain(p->w, p->ldw), p->outer, p->inner, ws);
     if (!count) TRY(stage.launch<T>(st), "linear_forward");
-    TRY((product<T, false, false>(st, x, w, p->rows, p->outer, p->inner, ep, ws, count)), "linear_forward");
+    JoinJob join = {};
+    TRY((product<T, false, false>(st, x, w, p->rows, p->outer, p->inner, ep, ws, &join, count)), "linear_forward");
+    if (!count) TRY(joins<T>(st, ColumnJob{}, join, JoinJob{}), "linear_forward");
     return CCSM_OK;
 }
 
@@ -274,16 +282,17 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
     T* made = make ? ws.take<T>((size_t)M * ldd) : nullptr;
     const Plane d = make ? Plane{made, ldd} : Plane{p->dy, p->lddy};
     float* part = p->dbias ? ws.take<float>((size_t)parts * N) : nullptr;
-    if (!count && (part || make)) {
-        slope_kernel<T><<<dim3((unsigned)parts, (unsigned)cdiv(N, 256)), 256, 0, st>>>(dy, none ? dy : saved_of(p->preact), p->activation, M, N, made, ldd, part);
-        if (part) column_join_kernel<T><<<(unsigned)cdiv(N, 8), 256, 0, st>>>(part, (int)parts, N, (T*)p->dbias);
-        LAUNCHED("linear_backward");
-    }
     Staging stage;
     const Plane w = p->dx ? stage.of<T>(plain(p->w, p->ldw), N, K, ws) : Plane{}, x = p->dw ? stage.of<T>(saved_of(p->x), M, K, ws) : Plane{};
-    if (!count) TRY(stage.launch<T>(st), "linear_backward");
-    if (p->dx) TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, count)), "linear_backward: dx");
-    if (p->dw) TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, count)), "linear_backward: dw");
+    if (!count && (part || make)) {
+        const SlopeJob job{dy, none ? dy : saved_of(p->preact), p->activation, M, N, made, ldd, part, (unsigned)parts, (unsigned)(parts * cdiv(N, 256))};
+        slope_kernel<T><<<job.blocks + (stage.count ? stage.blocks() : 0), 256, 0, st>>>(job, stage.jobs[0], stage.jobs[1]);
+        LAUNCHED("linear_backward");
+    } else if (!count) TRY(stage.launch<T>(st), "linear_backward");
+    JoinJob join_x = {}, join_w = {};
+    if (p->dx) TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, &join_x, count)), "linear_backward: dx");
+    if (p->dw) TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, &join_w, count)), "linear_backward: dw");
+    if (!count) TRY(joins<T>(st, part ? ColumnJob{part, (int)parts, N, p->dbias, (unsigned)cdiv(N, 8)} : ColumnJob{}, join_x, join_w), "linear_backward");
     return CCSM_OK;
 }
 

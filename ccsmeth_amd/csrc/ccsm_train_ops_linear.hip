@@ -7,21 +7,31 @@
 namespace ccsm_ops {
 
 // the parts of a bias gradient in a fixed order: a workgroup takes eight columns, each lane every 32nd part; the 32 sums are added in order
+struct ColumnJob { const float* part; int parts; int N; void* out; unsigned blocks; };
 template <typename T>
-__global__ __launch_bounds__(256) void column_join_kernel(const float* part, int parts, int N, T* out) {
+__device__ __forceinline__ void column_join(const ColumnJob& job, unsigned block) {
     __shared__ float s[32][9];
-    const int c = threadIdx.x & 7, q = threadIdx.x >> 3, n = blockIdx.x * 8 + c;
+    const int c = threadIdx.x & 7, q = threadIdx.x >> 3, n = (int)block * 8 + c;
     float a = 0.f;
-    if (n < N) {
+    if (n < job.N) {
 #pragma unroll 8
-        for (int p = q; p < parts; p += 32) a += part[(long long)p * N + n];
+        for (int p = q; p < job.parts; p += 32) a += job.part[(long long)p * job.N + n];
     }
     s[q][c] = a;
     __syncthreads();
-    if (q == 0 && n < N) {
+    if (q == 0 && n < job.N) {
         for (int k = 1; k < 32; ++k) a += s[k][c];
-        out[n] = (T)a;
+        ((T*)job.out)[n] = (T)a;
     }
+}
+// what is left to add up behind the products of a call, in one launch
+template <typename T>
+__global__ __launch_bounds__(256) void joins_kernel(ColumnJob c, JoinJob a, JoinJob b) {
+    unsigned block = blockIdx.x;
+    if (block < c.blocks) { column_join<T>(c, block); return; }
+    block -= c.blocks;
+    if (block < a.blocks) product_join<T>(a, block);
+    else product_join<T>(b, block - a.blocks);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void fill_zero_kernel(T* p, long long ld, long long rows, int cols) {

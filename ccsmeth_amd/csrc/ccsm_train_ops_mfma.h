@@ -497,16 +497,19 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
     store_tile<float, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), at.split, acc);
 }
 
-// the splits' parts in order, and the epilogue; a lane takes four neighbours
+// the splits' parts in order, and the epilogue; a lane takes four neighbours; workgroup `block` of `job.blocks`
+struct JoinJob { const float* part; int splits; long long M; int N; long long ld; Epilogue ep; unsigned blocks; };
 template <typename T>
-__global__ __launch_bounds__(256) void product_join_kernel(const float* part, int splits, long long M, int N, long long ld, Epilogue ep) {
-    const int nj = (N + 3) / 4;
-    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < M * nj; x += (long long)gridDim.x * 256) {
+__device__ __forceinline__ void product_join(const JoinJob& job, unsigned block) {
+    const Epilogue& ep = job.ep;
+    const long long M = job.M, ld = job.ld;
+    const int N = job.N, nj = (N + 3) / 4;
+    for (long long x = (long long)block * 256 + threadIdx.x; x < M * nj; x += (long long)job.blocks * 256) {
         const long long i = x / nj;
         const int j = (int)(x % nj) * 4;
-        f32x4 v = *(const f32x4*)(part + i * ld + j);
+        f32x4 v = *(const f32x4*)(job.part + i * ld + j);
 #pragma unroll 8
-        for (int s = 1; s < splits; ++s) v += *(const f32x4*)(part + ((long long)s * M + i) * ld + j);
+        for (int s = 1; s < job.splits; ++s) v += *(const f32x4*)(job.part + ((long long)s * M + i) * ld + j);
         float z[4] = {v[0], v[1], v[2], v[3]}, bias[4];
         Loose<T, 4> r;
         if (ep.bias) load_row<T, 4>((const T*)ep.bias + j, N - j, bias);
@@ -568,8 +571,8 @@ __device__ __forceinline__ void load8s(const Saved& s, const long long (&r)[R], 
 // kept matrices as rows of whole 16-byte pieces in the call's type (zeros behind the width); an item is eight values
 struct StageJob { Saved from; long long items; int width; void* out; long long ld; };
 template <typename T>
-__global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) {
-    for (long long x = (long long)blockIdx.x * 256 + threadIdx.x; x < a.items + b.items; x += (long long)gridDim.x * 256) {
+__device__ __forceinline__ void stage_items(const StageJob& a, const StageJob& b, unsigned block, unsigned blocks) {
+    for (long long x = (long long)block * 256 + threadIdx.x; x < a.items + b.items; x += (long long)blocks * 256) {
         const bool first = x < a.items;
         const StageJob& job = first ? a : b;
         const long long i = first ? x : x - a.items;
@@ -581,6 +584,8 @@ __global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) {
         store_row<T, 8>((T*)job.out + r * job.ld + c, 8, v);
     }
 }
+template <typename T>
+__global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) { stage_items<T>(a, b, blockIdx.x, gridDim.x); }
 
 // d = dy act'(z) in the call's type (16-bit types: rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 256 columns: 32 lanes of eight
 // columns, eight rows at a time, four rows of a lane in flight.
@@ -588,12 +593,24 @@ __global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) {
 // no more than the rounding of the gradient itself does.  The bias gradient takes d before it.
 // Bound by memory, and behind it by the slopes' instructions: 16384 x 4096 bf16 (gelu) 99 us, 400 MB at 4.1 TB/s; 43008 x 768 with z in e4m3 (silu)
 // 44 us, 165 MB at 3.8.
+// The workgroups behind the slopes' stage the products' other operands: one launch in front of both products.
+struct SlopeJob { Saved dy, z; int act; long long M; int N; void* d; long long ldd; float* part; unsigned parts, blocks; };
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, long long M, int N, T* d, long long ldd, float* part) {
+__global__ __launch_bounds__(256) void slope_kernel(SlopeJob job, StageJob sa, StageJob sb) {
+    if (blockIdx.x >= job.blocks) {
+        stage_items<T>(sa, sb, blockIdx.x - job.blocks, gridDim.x - job.blocks);
+        return;
+    }
+    const Saved &dy = job.dy, &z = job.z;
+    const int act = job.act, N = job.N;
+    const long long M = job.M, ldd = job.ldd;
+    T* d = (T*)job.d;
+    float* part = job.part;
+    const unsigned by = blockIdx.x / job.parts, bx = blockIdx.x - by * job.parts;
     constexpr bool fast = sizeof(T) == 2;
     __shared__ float sum[8][256];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.y * 256 + lane * 8;
-    const long long m0 = (long long)blockIdx.x * 32 + w;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (int)by * 256 + lane * 8;
+    const long long m0 = (long long)bx * 32 + w;
     float acc[8] = {};
     if (c < N) {
         float v[4][8], u[4][8];
@@ -619,12 +636,12 @@ __global__ __launch_bounds__(256) void slope_kernel(Saved dy, Saved z, int act, 
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[w][lane * 8 + k] = acc[k];
     __syncthreads();
-    const int n = blockIdx.y * 256 + threadIdx.x;
+    const int n = (int)(by * 256 + threadIdx.x);
     if (n >= N) return;
     float a = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) a += sum[k][threadIdx.x];
-    part[(long long)blockIdx.x * N + n] = a;
+    part[(long long)bx * N + n] = a;
 }
 
 // ---- small products and few rows ------------------------------------------------------------------------------------

@@ -113,14 +113,10 @@ struct Staging {
     }
 };
 
-template <typename T, bool TRP, bool TRQ, int B>
-hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
+template <int B, typename F, typename... A>
+hipError_t launch_tiles(F* f, std::atomic<uint64_t>& known, int64_t blocks, hipStream_t st, const A&... args) {
     constexpr int lds = 5 * B * 128;                    // two chunks of P, three of Q
-    void (*f)(ProductArgs);
-    if constexpr (sizeof(T) == 4) f = &product_f32_kernel<TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
-    else f = &product_mfma_kernel<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>;
     // an attribute of the function on each device: set once for each (setting it twice, from two threads, does no harm)
-    static std::atomic<uint64_t> known{0};
     int device = 0;
     hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return e;
@@ -130,8 +126,19 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
         if (e != hipSuccess) return e;
         known.fetch_or(bit, std::memory_order_relaxed);
     }
-    f<<<(unsigned)(a.tiles_i * a.tiles_j * a.splits), B == 256 ? 512 : 256, lds, st>>>(a);
+    f<<<(unsigned)blocks, B == 256 ? 512 : 256, lds, st>>>(args...);
     return hipGetLastError();
+}
+int64_t blocks_of(const ProductArgs& a) { return (int64_t)a.tiles_i * a.tiles_j * a.splits; }
+template <typename T, bool TRP, bool TRQ, int B>
+hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
+    static std::atomic<uint64_t> known{0};
+    return launch_tiles<B>(&product_kernel<T, TRP, TRQ, B>, known, blocks_of(a), st, a);
+}
+template <typename T, int B>
+hipError_t launch_pair(const ProductArgs& x, const ProductArgs& w, hipStream_t st) {
+    static std::atomic<uint64_t> known{0};
+    return launch_tiles<B>(&product_pair_kernel<T, B>, known, blocks_of(x) + blocks_of(w), st, x, w, (int)blocks_of(x));
 }
 // The tile and the number of parts of the contraction with the least estimated time.  The estimate: workgroups go in rounds, 256 of the large tile (one for
 // each CU), 512 of the small one (two for each CU, and a round of up to 256 has them to itself); a round takes its chunks' measured time; parts cost a
@@ -140,9 +147,11 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
 // 512 workgroups), bf16 | fp32, us, before -> after: 4096 x 1024 x 1024 26.6 -> 14.1 | 61 -> 53; 2048^3 33 -> 23 | 101 -> 95; 30000 x 1800 x 600
 // 92 -> 91 | 470 -> 372; 1024 x 4096 x 1024 26.3 -> 22.5 | 59 -> 57.
 struct Shape { int tile, splits; };
+struct Costs { double large, alone, pair, launch = 4, per_part = 0.08; };
+Costs costs(bool f32) { return f32 ? Costs{4.5, 1.4, 2.6} : Costs{1.3, 0.55, 0.8}; }
 Shape shape_of(int64_t M, int64_t N, int64_t chunks, bool f32) {
-    const double large = f32 ? 4.5 : 1.3, alone = f32 ? 1.4 : 0.55, pair = f32 ? 2.6 : 0.8;
-    const double launch = 4, per_part = 0.08, sums = (double)M * (double)N * 8 / 6e6;     // (written and read at 6 TB/s)
+    const auto [large, alone, pair, launch, per_part] = costs(f32);
+    const double sums = (double)M * (double)N * 8 / 6e6;     // (written and read at 6 TB/s)
     const int64_t tiles_big = cdiv(M, 256) * cdiv(N, 256), tiles_small = cdiv(M, 128) * cdiv(N, 128);
     Shape best{128, 1};
     double least = 0;
@@ -157,25 +166,52 @@ Shape shape_of(int64_t M, int64_t N, int64_t chunks, bool f32) {
     }
     return best;
 }
-// out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue; with parts, what is left to add up goes to *join
-template <typename T, bool TRP, bool TRQ>
-hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, JoinJob* join, bool count) {
+// the same of two products in one launch (M x N results over `chunks` each), whose workgroups share the CUs: the chunks of all of them, or the longest one
+struct Pair { int tile, splits[2]; };
+Pair pair_of(const int64_t (&M)[2], const int64_t (&N)[2], const int64_t (&chunks)[2], bool f32) {
+    const auto [large, alone, pair, launch, per_part] = costs(f32);
+    Pair best{128, {1, 1}};
+    double least = -1;
+    for (int tile = 128; tile <= 256; tile += 128) {
+        int64_t tiles[2];
+        for (int k = 0; k < 2; ++k) tiles[k] = cdiv(M[k], tile) * cdiv(N[k], tile);
+        for (int64_t sx = 1; sx == 1 || (2 * sx <= chunks[0] && tiles[0] * sx <= 2048 && sx <= 64); sx += sx < 4 ? 1 : sx / 2)
+            for (int64_t sw = 1; sw == 1 || (2 * sw <= chunks[1] && tiles[1] * sw <= 2048 && sw <= 256); sw += sw < 4 ? 1 : sw / 4 + 1) {
+                const int64_t dx = cdiv(chunks[0], sx), dw = cdiv(chunks[1], sw), longest = dx > dw ? dx : dw, groups = tiles[0] * sx + tiles[1] * sw;
+                const double all = (double)(tiles[0] * sx * dx + tiles[1] * sw * dw), alike = (double)longest * (tile == 256 ? large : groups <= 256 ? alone : pair);
+                double t = tile == 256 ? all / 256 * large : all / 512 * pair;
+                if (groups > (tile == 256 ? 256 : 512)) t += 0.5 * alike;               // (a last round that is half empty)
+                if (t < alike) t = alike;
+                if (sx > 1 || sw > 1) t += launch + per_part * (double)(sx > sw ? sx : sw);
+                if (sx > 1) t += (double)M[0] * (double)N[0] * 8 * (double)sx / 6e6;
+                if (sw > 1) t += (double)M[1] * (double)N[1] * 8 * (double)sw / 6e6;
+                if (least < 0 || t < least) { least = t; best = {tile, {(int)sx, (int)sw}}; }
+            }
+    }
+    return best;
+}
+// out(i, j) = sum over k P(i, k) Q(j, k) and the epilogue, in tiles and parts of that shape; with parts, what is left to add up goes to *join
+template <typename T>
+ProductArgs product_args(const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, int64_t chunks, Shape shape, const Epilogue& ep, Scratch& ws, JoinJob* join) {
     ProductArgs a;
     a.P = p; a.Q = q;
     a.M = (int)M; a.N = (int)N; a.K = (int)K;
     a.ep = ep;
-    constexpr int64_t chunk = 128 / (int64_t)sizeof(T);
-    const int64_t chunks = cdiv(K, chunk);
-    const Shape shape = shape_of(M, N, chunks, sizeof(T) == 4);
-    const int B = shape.tile;
-    a.tiles_i = (int)cdiv(M, B); a.tiles_j = (int)cdiv(N, B);
-    a.depth = (int)(cdiv(chunks, shape.splits) * chunk);
+    a.tiles_i = (int)cdiv(M, shape.tile); a.tiles_j = (int)cdiv(N, shape.tile);
+    a.depth = (int)(cdiv(chunks, shape.splits) * (128 / (int64_t)sizeof(T)));
     a.splits = (int)cdiv(K, a.depth);
     a.part_ld = (int64_t)up(N, 4);
     a.part = a.splits > 1 ? ws.take<float>((size_t)a.splits * M * a.part_ld) : nullptr;
-    if (count) return hipSuccess;
     if (a.splits > 1) *join = JoinJob{a.part, a.splits, M, (int)N, a.part_ld, ep, grid_of(cdiv(M * cdiv(N, 4), 256), 1 << 16)};
-    return B == 256 ? launch_product<T, TRP, TRQ, 256>(a, st) : launch_product<T, TRP, TRQ, 128>(a, st);
+    return a;
+}
+template <typename T> int64_t chunks_of(int64_t K) { return cdiv(K, 128 / (int64_t)sizeof(T)); }
+template <typename T, bool TRP, bool TRQ>
+hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, JoinJob* join, bool count) {
+    const Shape shape = shape_of(M, N, chunks_of<T>(K), sizeof(T) == 4);
+    const ProductArgs a = product_args<T>(p, q, M, N, K, chunks_of<T>(K), shape, ep, ws, join);
+    if (count) return hipSuccess;
+    return shape.tile == 256 ? launch_product<T, TRP, TRQ, 256>(a, st) : launch_product<T, TRP, TRQ, 128>(a, st);
 }
 template <typename T>
 hipError_t joins(hipStream_t st, const ColumnJob& c, const JoinJob& a, const JoinJob& b) {
@@ -290,8 +326,14 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         LAUNCHED("linear_backward");
     } else if (!count) TRY(stage.launch<T>(st), "linear_backward");
     JoinJob join_x = {}, join_w = {};
-    if (p->dx) TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, &join_x, count)), "linear_backward: dx");
-    if (p->dw) TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, &join_w, count)), "linear_backward: dw");
+    if (p->dx && p->dw) {
+        const int64_t chunks[2] = {chunks_of<T>(N), chunks_of<T>(M)};
+        const Pair both = pair_of({M, (int64_t)N}, {(int64_t)K, (int64_t)K}, chunks, sizeof(T) == 4);
+        const ProductArgs ax = product_args<T>(d, w, M, K, N, chunks[0], Shape{both.tile, both.splits[0]}, to_dx, ws, &join_x);
+        const ProductArgs aw = product_args<T>(d, x, N, K, M, chunks[1], Shape{both.tile, both.splits[1]}, to_dw, ws, &join_w);
+        if (!count) TRY((both.tile == 256 ? launch_pair<T, 256>(ax, aw, st) : launch_pair<T, 128>(ax, aw, st)), "linear_backward: dx and dw");
+    } else if (p->dx) TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, &join_x, count)), "linear_backward: dx");
+    else if (p->dw) TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, &join_w, count)), "linear_backward: dw");
     if (!count) TRY(joins<T>(st, part ? ColumnJob{part, (int)parts, N, p->dbias, (unsigned)cdiv(N, 8)} : ColumnJob{}, join_x, join_w), "linear_backward");
     return CCSM_OK;
 }

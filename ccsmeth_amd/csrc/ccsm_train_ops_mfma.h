@@ -254,7 +254,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, in
 }
 
 template <typename T, bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_mfma_kernel(ProductArgs a) {
+__device__ __forceinline__ void product_mfma(const ProductArgs& a, int block) {
     constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16, HW = BI / WI;
     typedef Side<2, TRP, BI, HW, NW> SP;
     typedef Side<2, TRQ, BJ, BJ / WJ, NW> SQ;
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
     static_assert(SP::kReq == SQ::kReq, "the waits below count as many requests of each operand");
     extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
-    const Place at = place_of(blockIdx.x, a.tiles_i, a.tiles_j, a.splits);
+    const Place at = place_of(block, a.tiles_i, a.tiles_j, a.splits);
     const int i0 = at.i * BI, j0 = at.j * BJ, split = at.split;
     const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
     constexpr unsigned kP = SP::kChunk, kQ = SQ::kChunk, kQ0 = 2 * kP;      // LDS: P's two chunks, then Q's three
@@ -387,7 +387,7 @@ __device__ __forceinline__ void three8(const float (&v)[8], s16x8 (&p)[3]) {
 // Q's fragments of a chunk stay in registers; P's come one row of products ahead.  The next chunk's Q is read and split in the last row, each fragment
 // behind its last product; the barrier stands in front of that row, when all of this chunk has been read.
 template <bool TRP, bool TRQ, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void product_f32_kernel(ProductArgs a) {
+__device__ __forceinline__ void product_f32(const ProductArgs& a, int block) {
     constexpr int NW = WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16, HW = BI / WI;
     typedef Side<4, TRP, BI, HW, NW> SP;
     typedef Side<4, TRQ, BJ, BJ / WJ, NW> SQ;
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
     static_assert(SP::kReq == SQ::kReq && kReq <= FI, "the waits below count as many requests of each operand");
     extern __shared__ __attribute__((aligned(1024))) char ops_smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WJ, wj = wave % WJ;
-    const Place at = place_of(blockIdx.x, a.tiles_i, a.tiles_j, a.splits);
+    const Place at = place_of(block, a.tiles_i, a.tiles_j, a.splits);
     const int i0 = at.i * BI, j0 = at.j * BJ;
     const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ops_smem;
     constexpr unsigned kP = SP::kChunk, kQ = SQ::kChunk;
@@ -495,6 +495,20 @@ __global__ __launch_bounds__(64 * WI * WJ, BI * BJ > 128 * 128 ? 1 : 2) void pro
         __builtin_amdgcn_sched_barrier(0);
     }
     store_tile<float, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), at.split, acc);
+}
+
+template <typename T, bool TRP, bool TRQ, int B>
+__device__ __forceinline__ void product_of(const ProductArgs& a, int block) {
+    if constexpr (sizeof(T) == 4) product_f32<TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>(a, block);
+    else product_mfma<T, TRP, TRQ, B, B, 2, B == 256 ? 4 : 2>(a, block);
+}
+template <typename T, bool TRP, bool TRQ, int B>
+__global__ __launch_bounds__(B == 256 ? 512 : 256, B == 256 ? 1 : 2) void product_kernel(ProductArgs a) { product_of<T, TRP, TRQ, B>(a, blockIdx.x); }
+// both products of a backward pass: the workgroups of the first (dx = d w), then those of the second (dw = d^T x), which fill the CUs that it leaves
+template <typename T, int B>
+__global__ __launch_bounds__(B == 256 ? 512 : 256, B == 256 ? 1 : 2) void product_pair_kernel(ProductArgs x, ProductArgs w, int first) {
+    if ((int)blockIdx.x < first) product_of<T, false, true, B>(x, blockIdx.x);
+    else product_of<T, true, true, B>(w, blockIdx.x - first);
 }
 
 // the splits' parts in order, and the epilogue; a lane takes four neighbours; workgroup `block` of `job.blocks`

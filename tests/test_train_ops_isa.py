@@ -37,7 +37,7 @@ def kernels(tmp_path_factory):
         for entry in notes.split("  - .agpr_count")[1:]:
             f = dict(re.findall(r"^    \.(\w+):\s+(\S+)", entry, re.M))
             meta[f["name"]] = (int(f["private_segment_fixed_size"]), int(f["vgpr_spill_count"]))
-        names = [n for n in meta if "product_mfma_kernel" in n]
+        names = [n for n in meta if re.search(r"product_(pair_)?kernelIDF16", n)]                       # of 16-bit types
         if not names:
             continue
         text = subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", "--no-show-raw-insn", "--disassemble-symbols=" + ",".join(names), co], check=True, capture_output=True,
@@ -71,12 +71,12 @@ def findings(ins, where, goes, report):
 
 
 def test_product_kernels(kernels):
-    assert len(kernels) == 12, sorted(kernels)                     # two types, three forms of the operands, two tiles
+    assert len(kernels) == 16, sorted(kernels)                     # two types, two tiles, three forms of the operands and the pair of two
     for name, (ins, where, goes, scratch, spilled) in kernels.items():
         said = []
         bad, products, tied, loops = findings(ins, where, goes, said.append)
         assert bad == 0, "\n".join(said)
-        assert products and tied == products and loops >= 1, (name, products, tied, loops)
+        assert products and tied == products and loops >= (2 if "pair" in name else 1), (name, products, tied, loops)
         assert scratch == 0 and spilled == 0, (name, scratch, spilled)
 
 

@@ -223,13 +223,24 @@ hipError_t joins(hipStream_t st, const ColumnJob& c, const JoinJob& a, const Joi
 #define TRY(x, what) do { hipError_t e_ = (x); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
 
 bool small_product(int64_t M, int64_t N, int64_t K) { return M * N <= kSmallResult && M * N * K <= kSmallProduct; }
-template <typename T, bool TRP, bool TRQ>
-hipError_t direct(hipStream_t st, const Plane& p, const Plane& z, int act, const Plane& q, int64_t M, int64_t N, int64_t K, void* sums, const Epilogue& ep) {
+DirectArgs direct_args(const Plane& p, const Plane& z, int act, const Plane& q, int64_t M, int64_t N, int64_t K, void* sums, const Epilogue& ep) {
     DirectArgs a{p, z, q, act, M, N, K, 1, sums, ep};
     while (a.kw < 8 && 32 * 2 * a.kw <= K) a.kw *= 2;             // (a wave has a whole step of 32 at least)
-    const int mt = M <= 16 ? 1 : 4;
+    return a;
+}
+unsigned rows_of(const DirectArgs& a, int mt) { return (unsigned)cdiv(a.M, 16 * mt * (8 / a.kw)); }
+template <typename T, bool TRP, bool TRQ>
+hipError_t direct(hipStream_t st, const DirectArgs& a) {
+    const int mt = a.M <= 16 ? 1 : 4;
     auto* f = mt == 1 ? &direct_kernel<T, TRP, TRQ, 1> : &direct_kernel<T, TRP, TRQ, 4>;
-    f<<<dim3((unsigned)cdiv(N, 16), (unsigned)cdiv(M, 16 * mt * (8 / a.kw))), 512, 0, st>>>(a);
+    f<<<dim3((unsigned)cdiv(a.N, 16), rows_of(a, mt)), 512, 0, st>>>(a);
+    return hipGetLastError();
+}
+template <typename T>
+hipError_t direct_pair(hipStream_t st, const DirectArgs& x, const DirectArgs& w) {      // (as many columns each)
+    const int mt = x.M <= 16 && w.M <= 16 ? 1 : 4;
+    auto* f = mt == 1 ? &direct_pair_kernel<T, 1> : &direct_pair_kernel<T, 4>;
+    f<<<dim3((unsigned)cdiv(x.N, 16), rows_of(x, mt) + rows_of(w, mt)), 512, 0, st>>>(x, w, rows_of(x, mt));
     return hipGetLastError();
 }
 
@@ -249,7 +260,7 @@ ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bo
     const Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
     if (p->rows <= kFewRows || (p->inner <= kShortForward && small_product(p->rows, p->outer, p->inner))) {
         if (count) return CCSM_OK;
-        TRY((direct<T, false, false>(st, Plane{p->x, p->ldx}, Plane{p->x, p->ldx}, CCSM_ACT_NONE, Plane{p->w, p->ldw}, p->rows, p->outer, p->inner, nullptr, ep)), "linear_forward");
+        TRY((direct<T, false, false>(st, direct_args(Plane{p->x, p->ldx}, Plane{p->x, p->ldx}, CCSM_ACT_NONE, Plane{p->w, p->ldw}, p->rows, p->outer, p->inner, nullptr, ep))), "linear_forward");
         return CCSM_OK;
     }
     Staging stage;
@@ -305,9 +316,12 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         const Plane dy{p->dy, p->lddy}, z = p->activation == CCSM_ACT_NONE ? dy : values(p->preact, N), x = p->dw ? values(p->x, K) : dy;
         if (count) return CCSM_OK;
         TRY(stage.launch<T>(st), "linear_backward");
-        if (p->dx) TRY((direct<T, false, true>(st, dy, z, p->activation, Plane{p->w, p->ldw}, M, K, N, nullptr, to_dx)), "linear_backward: dx");
-        if (p->dw || p->dbias)                                     // (the bias gradient comes with dw's product, or by the same sums without it)
-            TRY((direct<T, true, true>(st, dy, z, p->activation, x, N, p->dw ? K : 1, M, p->dbias, to_dw)), "linear_backward: dw");
+        const DirectArgs ax = direct_args(dy, z, p->activation, Plane{p->w, p->ldw}, M, K, N, nullptr, to_dx);
+        const DirectArgs aw = direct_args(dy, z, p->activation, x, N, p->dw ? K : 1, M, p->dbias, to_dw);
+        if (p->dx && p->dw) TRY(direct_pair<T>(st, ax, aw), "linear_backward: dx and dw");
+        else if (p->dx) TRY((direct<T, false, true>(st, ax)), "linear_backward: dx");
+        if (!(p->dx && p->dw) && (p->dw || p->dbias))              // (the bias gradient comes with dw's product, or by the same sums without it)
+            TRY((direct<T, true, true>(st, aw)), "linear_backward: dw");
         return CCSM_OK;
     }
     // d as the products take it: dy itself where there is no activation and its rows are whole pieces

@@ -673,15 +673,17 @@ struct DirectArgs {
     void* sums;                   // NULL, or (M): the sum over k of P(i, k), before its rounding
     Epilogue ep;                  // y NULL: the sums alone
 };
+template <typename T, int MT>
+struct DirectRoom { f32x4 sum[8][MT][64]; float total[8][MT][16]; };
 template <typename T, bool TRP, bool TRQ, int MT>
-__global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
+__device__ __forceinline__ void direct_product(const DirectArgs& a, DirectRoom<T, MT>& room, unsigned by) {
     typedef typename std::conditional<sizeof(T) == 4, b16, T>::type E;
     constexpr int NP = sizeof(T) == 4 ? 3 : 1, U = 4;
     constexpr bool fast = sizeof(T) == 2;
-    __shared__ f32x4 sum[8][MT][64];
-    __shared__ float total[8][MT][16];
+    auto& sum = room.sum;
+    auto& total = room.total;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave & (a.kw - 1), wm = wave / a.kw, mw = 8 / a.kw;
-    const long long j0 = (long long)blockIdx.x * 16, i0 = ((long long)blockIdx.y * mw + wm) * (16 * MT);
+    const long long j0 = (long long)blockIdx.x * 16, i0 = ((long long)by * mw + wm) * (16 * MT);
     const long long j = j0 + (lane & 15) < a.N ? j0 + (lane & 15) : a.N - 1;
     long long i[MT];
 #pragma unroll
@@ -815,7 +817,7 @@ __global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
     __syncthreads();
     for (int e = threadIdx.x; e < mw * MT * 64; e += 512) {
         const int l = e & 63, t = (e >> 6) % MT, w = (e >> 6) / MT;
-        const long long m = ((long long)blockIdx.y * mw + w) * (16 * MT) + 16 * t + (l & 15), n = j0 + 4 * (l >> 4);
+        const long long m = ((long long)by * mw + w) * (16 * MT) + 16 * t + (l & 15), n = j0 + 4 * (l >> 4);
         if (m >= a.M || n >= a.N || !a.ep.y) continue;
         const int left = (int)(a.N - n < 4 ? a.N - n : 4);
         f32x4 v = sum[w * a.kw][t][l];
@@ -829,12 +831,24 @@ __global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
     if (want)
         for (int e = threadIdx.x; e < mw * MT * 16; e += 512) {
             const int l = e & 15, t = (e >> 4) % MT, w = (e >> 4) / MT;
-            const long long m = ((long long)blockIdx.y * mw + w) * (16 * MT) + 16 * t + l;
+            const long long m = ((long long)by * mw + w) * (16 * MT) + 16 * t + l;
             if (m >= a.M) continue;
             float v = total[w * a.kw][t][l];
             for (int q = 1; q < a.kw; ++q) v += total[w * a.kw + q][t][l];
             ((T*)a.sums)[m] = (T)v;
         }
+}
+template <typename T, bool TRP, bool TRQ, int MT>
+__global__ __launch_bounds__(512) void direct_kernel(DirectArgs a) {
+    __shared__ DirectRoom<T, MT> room;
+    direct_product<T, TRP, TRQ, MT>(a, room, blockIdx.y);
+}
+// both products of a small backward pass: the rows of workgroups of the first (dx = d w), then those of the second (dw = d^T x)
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void direct_pair_kernel(DirectArgs x, DirectArgs w, unsigned first) {
+    __shared__ DirectRoom<T, MT> room;
+    if (blockIdx.y < first) direct_product<T, false, true, MT>(x, room, blockIdx.y);
+    else direct_product<T, true, true, MT>(w, room, blockIdx.y - first);
 }
 
 }  // namespace ccsm_ops

@@ -39,12 +39,13 @@ struct OnDevice {
     OnDevice on_device_(device);               \
     if (on_device_.err != hipSuccess) return hip_fail(on_device_.err, "hipSetDevice")
 
-// Where direct_kernel takes a product: forward ones of at most 64 rows, and products of at most 2^27 multiplications whose contraction is short, since
-// its steps follow each other without a tile's prefetch.  Measured (bf16 | fp32, us on the GPU, tile way -> direct): 512^3 forward 10.4 -> 6.0 |
-// 16.2 -> 8.9, gradients 25 -> 23 | 41 -> 33; 300 x 700 x 300 forward 15.9 -> 6.2 | 12.8 -> 9.3, gradients 29.5 -> 22 | 36 -> 32; beyond: 1024^3 forward
-// 13.8 -> 24 | 30 -> 53; a contraction of 4096 (128 x 128 results) 11 -> 20.5 | 14.5 -> 39; gradients of 2000 x 64 x 1000 32 -> 65 | 44 -> 87;
-// results of 13377 x 768 (stored in pieces of 16 columns) 26 -> 51.
-constexpr int64_t kFewRows = 64, kSmallProduct = 1 << 27, kSmallResult = 1 << 21, kShortForward = 1024, kShortBackward = 512;
+// Where direct_kernel takes a product.  Forward: at most 64 rows, or at most 2^27 multiplications whose contraction is short, since its steps follow each
+// other without a tile's prefetch.  Measured (bf16 | fp32, us on the GPU, tile way -> direct): 512^3 10.4 -> 6.0 | 16.2 -> 8.9, 300 x 700 x 300
+// 15.9 -> 6.2 | 12.8 -> 9.3; beyond: 1024^3 13.8 -> 24 | 30 -> 53; a contraction of 4096 (128 x 128 results) 11 -> 20.5 | 14.5 -> 39; results of
+// 13377 x 768 (stored in pieces of 16 columns) 26 -> 51.  Backward: contractions of at most 512 and, both products together, three steps a CU,
+// one workgroup each: 64 x 512 x 512 15.1 -> 11.3 | 19.3 -> 16.7, 500 x 2000 x 60 19.1 -> 15.3 | 23.9 -> 18.1; at two steps, 256 x 512 x 512, 15.5 -> 15.1 |
+// 22 -> 19.7; at three, 300 x 500 x 400, 16.6 -> 21.4 | 22 -> 30, for gradients that keep what rounding d leaves; beyond: 512^3 16.2 -> 22.3 | 25 -> 31.
+constexpr int64_t kFewRows = 64, kSmallProduct = 1 << 27, kSmallResult = 1 << 21, kShortForward = 1024, kShortBackward = 512, kBackwardSteps = 768;
 constexpr int64_t kNarrow = 1 << 21;                              // row strides that the kernels' 32-bit offsets span
 constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
 
@@ -223,10 +224,17 @@ hipError_t joins(hipStream_t st, const ColumnJob& c, const JoinJob& a, const Joi
 #define TRY(x, what) do { hipError_t e_ = (x); if (e_ != hipSuccess) return hip_fail(e_, what); } while (0)
 
 bool small_product(int64_t M, int64_t N, int64_t K) { return M * N <= kSmallResult && M * N * K <= kSmallProduct; }
+int waves_along(int64_t K) {                                      // (a wave has a whole step of 32 at least)
+    int kw = 1;
+    while (kw < 8 && 32 * 2 * kw <= K) kw *= 2;
+    return kw;
+}
+int64_t steps_of(int64_t M, int64_t N, int64_t K) {               // of all workgroups
+    const int kw = waves_along(K);
+    return cdiv(N, 16) * cdiv(M, 64 * (8 / kw)) * cdiv(K, 32 * kw);
+}
 DirectArgs direct_args(const Plane& p, const Plane& z, int act, const Plane& q, int64_t M, int64_t N, int64_t K, void* sums, const Epilogue& ep) {
-    DirectArgs a{p, z, q, act, M, N, K, 1, sums, ep};
-    while (a.kw < 8 && 32 * 2 * a.kw <= K) a.kw *= 2;             // (a wave has a whole step of 32 at least)
-    return a;
+    return DirectArgs{p, z, q, act, M, N, K, waves_along(K), sums, ep};
 }
 unsigned rows_of(const DirectArgs& a, int mt) { return (unsigned)cdiv(a.M, 16 * mt * (8 / a.kw)); }
 template <typename T, bool TRP, bool TRQ>
@@ -308,7 +316,7 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
     }
     const Epilogue to_dx{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, to_dw{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone};
     const bool narrow = p->lddy < kNarrow && (!p->dx || p->ldw < kNarrow) && (p->activation == CCSM_ACT_NONE || p->preact.ld < kNarrow) && (!p->dw || p->x.ld < kNarrow);
-    if (narrow && M <= kShortBackward && N <= kShortBackward && small_product(M, N, K)) {
+    if (narrow && M <= kShortBackward && N <= kShortBackward && steps_of(M, K, N) + steps_of(N, K, M) <= kBackwardSteps) {
         // checkpoints are made values in a launch of their own: a lane would read them code by code along the rows (bf16, both operands in 8 bits, us a
         // backward pass: 512^3 52 -> 28, 64 x 512 x 512 43 -> 23)
         Staging stage;

@@ -178,10 +178,11 @@ Pair pair_of(const int64_t (&M)[2], const int64_t (&N)[2], const int64_t (&chunk
         for (int k = 0; k < 2; ++k) tiles[k] = cdiv(M[k], tile) * cdiv(N[k], tile);
         for (int64_t sx = 1; sx == 1 || (2 * sx <= chunks[0] && tiles[0] * sx <= 2048 && sx <= 64); sx += sx < 4 ? 1 : sx / 2)
             for (int64_t sw = 1; sw == 1 || (2 * sw <= chunks[1] && tiles[1] * sw <= 2048 && sw <= 256); sw += sw < 4 ? 1 : sw / 4 + 1) {
-                const int64_t dx = cdiv(chunks[0], sx), dw = cdiv(chunks[1], sw), longest = dx > dw ? dx : dw, groups = tiles[0] * sx + tiles[1] * sw;
-                const double all = (double)(tiles[0] * sx * dx + tiles[1] * sw * dw), alike = (double)longest * (tile == 256 ? large : groups <= 256 ? alone : pair);
-                double t = tile == 256 ? all / 256 * large : all / 512 * pair;
-                if (groups > (tile == 256 ? 256 : 512)) t += 0.5 * alike;               // (a last round that is half empty)
+                const int64_t dx = cdiv(chunks[0], sx), dw = cdiv(chunks[1], sw), longest = dx > dw ? dx : dw, nx = tiles[0] * sx, nw = tiles[1] * sw;
+                const int64_t slots = tile == 256 ? 256 : 512;
+                const double chunk = tile == 256 ? large : nx + nw <= 256 ? alone : pair, alike = (double)longest * chunk;
+                double t = (double)(nx * dx + nw * dw) / (double)slots * (tile == 256 ? large : pair);
+                if (nx + nw > slots && (nx % slots || nw % slots)) t += 0.5 * (double)dw * chunk;      // (a last round that is half empty)
                 if (t < alike) t = alike;
                 if (sx > 1 || sw > 1) t += launch + per_part * (double)(sx > sw ? sx : sw);
                 if (sx > 1) t += (double)M[0] * (double)N[0] * 8 * (double)sx / 6e6;

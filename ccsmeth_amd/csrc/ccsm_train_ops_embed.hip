@@ -206,8 +206,9 @@ constexpr int kLongPiece = 32, kShortPiece = 8;
 // Workgroups [0, sums) of a column block: `groups` groups of lanes with a piece of sorted tokens each, a lane = N neighbouring columns.  A sum that lies
 // inside a piece is written at once.  What crosses pieces is put together in LDS by the group whose piece it starts in, and written if it ends in
 // this workgroup; else it leaves as the workgroup's head or tail.  The other workgroups clear the rows of the table that have no mark.
-// Measured (65536 x 1024 bf16 over 50000 rows, 15.5 thousand of them met, from memory): 84 us, 236 MB at 2.8 TB/s, the sort in front 25, the join behind 11.
-// Clearing first, or between the sums, takes 5 and 25 us more; pieces of 8, 16, 64 tokens 7, 2, 25.
+// Measured (65536 x 1024 bf16 over 50000 rows, 15.5 thousand of them met, from memory): 70 us, 236 MB at 3.4 TB/s (84 with a
+// condition on each row's load), the sort in front 26, the join behind 11.  Clearing first, or between the sums, took 5 and 25 us more; pieces of 8, 16,
+// 64 tokens 7, 2, 25; eight more rows in flight spilled.
 template <typename T, int N, int kPiece>
 __global__ __launch_bounds__(256, 3) void piece_sum_kernel(const unsigned* keys, const unsigned* at, long long n, long long rows, unsigned sums, int groups, Div lanes, int width,
                                                         const T* dy, long long lddy, float scale, T* dt, long long ldt, float* part, long long part_ld, const uint8_t* marks,

@@ -605,8 +605,8 @@ __global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) { st
 // columns, eight rows at a time, four rows of a lane in flight.
 // Rounding d: 16-bit products take 16-bit operands, and this rounding (half a step per factor, independent of each other) moves a gradient by
 // no more than the rounding of the gradient itself does.  The bias gradient takes d before it.
-// Bound by memory, and behind it by the slopes' instructions: 16384 x 4096 bf16 (gelu) 99 us, 400 MB at 4.1 TB/s; 43008 x 768 with z in e4m3 (silu)
-// 44 us, 165 MB at 3.8.
+// Bound by memory, and behind it by the slopes' instructions: 16384 x 4096 bf16 (gelu) 90 us, 400 MB at 4.5 TB/s; 43008 x 768 with z in e4m3 (silu)
+// and 43008 x 512 codes of x behind it 50 us, 231 MB at 4.6.
 // The workgroups behind the slopes' stage the products' other operands: one launch in front of both products.
 struct SlopeJob { Saved dy, z; int act; long long M; int N; void* d; long long ldd; float* part; unsigned parts, blocks; };
 template <typename T>
@@ -664,7 +664,7 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeJob job, StageJob sa, S
 // them) and the i between them; their sums are added in order through LDS.  fp32: the three bf16 parts of each operand are made in
 // registers.
 // For up to 64 rows it is bound by reading w once (1 x 512 x 768 bf16: 3.6 us; the tile kernel 9.8, four steps through LDS by six of 256 CUs); for
-// small products by its one launch (the tile kernel's way takes up to three for a product and eight for a backward pass).
+// small products by its one launch (the tile kernel's way takes up to three).
 struct DirectArgs {
     Plane P, Z, Q;                // Z, act: P's elements are multiplied by act'(Z)
     int act;

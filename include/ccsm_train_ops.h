@@ -87,7 +87,8 @@ ccsm_status ccsm_train_linear_backward(int device, const ccsm_linear_grad* p, vo
 /* ids outside [0, rows) are no tokens (padding): their row of y is zero and they have no gradient.  y (tokens, width) = scale table[ids]. */
 ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
                                          const void* table, int64_t ldt, float scale, void* y, int64_t ldy, void* stream);
-/* dtable (rows, width) is written whole.  The tokens are sorted by id on the GPU (stable), so a row's sum has one order. */
+/* dtable (rows, width) is written whole.  A row's sum has one order, which depends on the sizes and the ids alone (tokens are sorted by id on the
+ * GPU, stably; tables of few rows are added up without). */
 size_t ccsm_train_embedding_backward_workspace(int type, int64_t tokens, int64_t rows, int32_t width);
 ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
                                           const void* dy, int64_t lddy, float scale, void* dtable, int64_t ldt, void* workspace,

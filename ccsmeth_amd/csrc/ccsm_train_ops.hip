@@ -48,6 +48,9 @@ struct OnDevice {
 constexpr int64_t kFewRows = 64, kSmallProduct = 1 << 27, kSmallResult = 1 << 21, kShortForward = 1024, kShortBackward = 512, kBackwardSteps = 768;
 constexpr int64_t kNarrow = 1 << 21;                              // row strides that the kernels' 32-bit offsets span
 constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
+// The tile kernels' offsets into an operand whose contraction index is contiguous: 255 rows and a row's 128 bytes, in the 32 bits of a buffer's extent.  A
+// caller's own stride is below kNarrow; a staged copy (and d) is as wide as the contraction.  16 bits: 8421504 columns, fp32: 4210752
+constexpr int64_t kExtent = 0xfffffffe;
 
 size_t size_of(int type) { return type == CCSM_TYPE_F32 ? 4 : 2; }
 bool good_type(int t) { return t == CCSM_TYPE_F32 || t == CCSM_TYPE_F16 || t == CCSM_TYPE_BF16; }
@@ -55,6 +58,8 @@ bool off_by(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & 
 size_t up(size_t n, size_t a) { return (n + a - 1) / a * a; }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 unsigned grid_of(int64_t n, int64_t most = 1 << 20) { return (unsigned)(n < 1 ? 1 : n > most ? most : n); }
+
+bool spanned(int64_t k, int type) { return 255 * (int64_t)up((size_t)k, 8) * (int64_t)size_of(type) + 128 <= kExtent; }
 
 // scratch of a call, handed out piece by piece; without a base it only counts
 struct Scratch {
@@ -258,6 +263,7 @@ ccsm_status check_linear(const ccsm_linear* p) {
     REFUSE(!good_type(p->type), "linear: unknown type");
     REFUSE(p->activation < CCSM_ACT_NONE || p->activation > CCSM_ACT_SILU, "linear: unknown activation");
     REFUSE(p->rows < 0 || p->rows > kMostRows || p->inner <= 0 || p->inner > kMostCols || p->outer <= 0 || p->outer > kMostCols, "linear: sizes out of range");
+    REFUSE(p->rows > kFewRows && !spanned(p->inner, p->type), "linear: inner is too long for more than 64 rows");
     REFUSE(!p->w || (p->rows && (!p->x || !p->y)), "linear: x, w and y must be non-NULL");
     REFUSE(p->ldx < p->inner || p->ldw < p->inner || p->ldy < p->outer || (p->residual && p->ldr < p->outer) || (p->preact && p->ldp < p->outer), "linear: a row stride is less than the row's width");
     const size_t s = size_of(p->type);
@@ -295,6 +301,7 @@ ccsm_status check_grad(const ccsm_linear_grad* p) {
             ccsm_status e = check_saved(p->preact, p->type, p->outer, "linear_backward: an activation's slope needs the pre-activation");
             if (e != CCSM_OK) return e;
         }
+        REFUSE(p->dx && !spanned(p->outer, p->type), "linear_backward: outer is too long for dx");
         if (p->dx) REFUSE(!p->w || p->ldw < p->inner || p->lddx < p->inner, "linear_backward: dx needs w, and strides of at least inner");
         if (p->dw) {
             ccsm_status e = check_saved(p->x, p->type, p->inner, "linear_backward: dw needs x");

@@ -161,3 +161,20 @@ def test_trainer_refuses_other_widths():
     for bits in (0, 4, 16, 64):
         assert lib.ccsm_train_create_act(C.byref(w), 0, 16, None, bits, C.byref(out)) == INVALID
         assert b"activation_bits" in lib.ccsm_train_last_error()
+
+
+@pytest.mark.parametrize("kind,most", [(0, 4210752), (1, 8421504), (2, 8421504)])
+def test_contractions_whose_offsets_leave_32_bits_are_refused(kind, most):
+    """255 rows of a staged operand and a row's last 128 bytes lie within a buffer's extent of 2^32 - 2 bytes up to `most` columns, and not beyond"""
+    lib = ops.load()
+    size = 4 if kind == 0 else 2
+    assert 255 * most * size + 128 <= 2 ** 32 - 2 < 255 * (most + 8) * size + 128
+    for inner, ok in ((most, True), (most - 5, True), (most + 1, False), (9000000, False), (0x00ffff00, False)):
+        p = _linear(type=kind, rows=256, inner=inner, outer=256, ldx=inner, ldw=inner, ldy=256, ldr=256, ldp=256)
+        assert (lib.ccsm_train_linear_workspace(C.byref(p)) > 0) == ok                  # (both operands are staged: their strides are too long)
+        assert lib.ccsm_train_linear_forward(0, C.byref(p), None, 0, None) == (CAPACITY if ok else INVALID)
+        g = _grad(type=kind, rows=300, inner=256, outer=inner, lddy=inner, ldw=256, lddx=256, lddw=256, preact=ops.Saved(A, inner, 0, None, 0), x=ops.Saved(A, 256, 0, None, 0))
+        assert (lib.ccsm_train_linear_backward_workspace(C.byref(g)) > 0) == ok
+        assert lib.ccsm_train_linear_backward(0, C.byref(g), None, 0, None) == (CAPACITY if ok else INVALID)
+        g.dx = None                                                                     # dw and dbias run along rows: no limit but that of the columns
+        assert lib.ccsm_train_linear_backward(0, C.byref(g), None, 0, None) == CAPACITY

@@ -322,7 +322,7 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         LAUNCHED("linear_backward");
         return CCSM_OK;
     }
-    const Epilogue to_dx{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, to_dw{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone};
+    Epilogue to_dx{nullptr, nullptr, 0, p->dx, p->lddx, nullptr, 0, kActNone}, to_dw{nullptr, nullptr, 0, p->dw, p->lddw, nullptr, 0, kActNone};
     const bool narrow = p->lddy < kNarrow && (!p->dx || p->ldw < kNarrow) && (p->activation == CCSM_ACT_NONE || p->preact.ld < kNarrow) && (!p->dw || p->x.ld < kNarrow);
     if (narrow && M <= kShortBackward && N <= kShortBackward && steps_of(M, K, N) + steps_of(N, K, M) <= kBackwardSteps) {
         // checkpoints are made values in a launch of their own: a lane would read them code by code along the rows (bf16, both operands in 8 bits, us a
@@ -350,8 +350,14 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
     float* part = p->dbias ? ws.take<float>((size_t)parts * N) : nullptr;
     Staging stage;
     const Plane w = p->dx ? stage.of<T>(plain(p->w, p->ldw), N, K, ws) : Plane{}, x = p->dw ? stage.of<T>(saved_of(p->x), M, K, ws) : Plane{};
+    const bool scaled = TypeOf<T>::v == CCSM_TYPE_F16 && make && !none;      // (d is dy itself without an activation)
+    float *most = scaled ? ws.take<float>(kMosts) : nullptr, *factor = scaled ? ws.take<float>(1) : nullptr;
+    to_dx.factor = to_dw.factor = factor;
     if (!count && (part || make)) {
-        const SlopeJob job{dy, none ? dy : saved_of(p->preact), p->activation, M, N, made, ldd, part, (unsigned)parts, (unsigned)(parts * cdiv(N, 256))};
+        const int64_t items = M * cdiv(N, 8);
+        const int mosts = scaled ? (int)grid_of(cdiv(items, 1024), kMosts) : 0;
+        if (scaled) most_kernel<<<(unsigned)mosts, 1024, 0, st>>>((const f16*)p->dy, p->lddy, items, (unsigned)cdiv(N, 8), N, most);
+        const SlopeJob job{dy, none ? dy : saved_of(p->preact), p->activation, M, N, made, ldd, part, (unsigned)parts, (unsigned)(parts * cdiv(N, 256)), most, mosts, factor};
         slope_kernel<T><<<job.blocks + (stage.count ? stage.blocks() : 0), 256, 0, st>>>(job, stage.jobs[0], stage.jobs[1]);
         LAUNCHED("linear_backward");
     } else if (!count) TRY(stage.launch<T>(st), "linear_backward");

@@ -24,6 +24,8 @@
 // repeat the last ones, and their results are not written.  What the kernel needs: 16-byte aligned bases and row strides (multiples of 8
 // elements), the contiguous extent a multiple of 8; other operands are staged first (stage_kernel).
 #pragma once
+#include <type_traits>
+
 #include "ccsm_train_ops_common.h"
 
 namespace ccsm_ops {
@@ -51,9 +53,10 @@ template <> struct Mfma<b16> {
     static __device__ __forceinline__ void tied(s16x8 a, s16x8 b, f32x4& c) { asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b)); }
 };
 
-// what a product's results go through: z = acc + bias; y = act(z) + residual.  With `part`, the accumulators go there instead (split k)
+// what a product's results go through: z = acc (* factor) + bias; y = act(z) + residual.  With `part`, the accumulators go there instead (split k)
 struct Epilogue {
     const void* bias; const void* residual; long long ldr; void* y; long long ldy; void* pre; long long ldp; int act;
+    const float* factor = nullptr;            // fp16: z = acc * *factor (+ bias), where an operand was multiplied by its inverse
 };
 struct Plane { const void* base; long long ld; };
 struct ProductArgs {
@@ -68,6 +71,13 @@ struct ProductArgs {
 template <typename T, int N>
 __device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, int left, float (&z)[N], const float (&bias)[N], const Loose<T, N>& r) {
     constexpr bool fast = sizeof(T) == 2;
+    if constexpr (std::is_same<T, f16>::value) {
+        if (e.factor) {
+            const float f = *e.factor;
+#pragma unroll
+            for (int k = 0; k < N; ++k) z[k] *= f;
+        }
+    }
     if (e.bias) {
 #pragma unroll
         for (int k = 0; k < N; ++k) z[k] += bias[k];
@@ -601,14 +611,49 @@ __device__ __forceinline__ void stage_items(const StageJob& a, const StageJob& b
 template <typename T>
 __global__ __launch_bounds__(256) void stage_kernel(StageJob a, StageJob b) { stage_items<T>(a, b, blockIdx.x, gridDim.x); }
 
+// The largest finite magnitude of each workgroup's part of an fp16 matrix, eight values a lane and four of those in flight.  Bound
+// by memory: 16384 x 4096 in 37 us, 134 MB at 3.6 TB/s (that backward pass 945 -> 983 us, one of 43008 x 512 -> 768 138 -> 154, 4096 x 512 x 512 27 -> 35)
+constexpr int kMosts = 256;
+__global__ __launch_bounds__(1024) void most_kernel(const f16* p, long long ld, long long items, unsigned per_row, int width, float* most) {
+    __shared__ float s[16];
+    float a = 0.f;
+    const long long all = (long long)gridDim.x * 1024;
+    for (long long x = (long long)blockIdx.x * 1024 + threadIdx.x; x < items; x += 4 * all) {
+        Loose<f16, 8> v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const long long i = x + all * q < items ? x + all * q : items - 1, r = i >> 32 ? i / per_row : (unsigned)i / per_row;
+            const int c = (int)(i - r * per_row) * 8;
+            v[q] = raw_row<f16, 8>(p + r * ld + c, width - c);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float u = fabsf((float)v[q].v[k]);
+                a = fmaxf(a, u < INFINITY ? u : 0.f);
+            }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 16; ++w) a = fmaxf(a, s[w]);
+    most[blockIdx.x] = a;
+}
 // d = dy act'(z) in the call's type (16-bit types: rounded), and the column sums of 32 rows each.  One workgroup: 32 rows x 256 columns: 32 lanes of eight
 // columns, eight rows at a time, four rows of a lane in flight.
-// Rounding d: 16-bit products take 16-bit operands, and this rounding (half a step per factor, independent of each other) moves a gradient by
-// no more than the rounding of the gradient itself does.  The bias gradient takes d before it.
+// Rounding d: 16-bit products take 16-bit operands.  This rounding (half a step per factor, independent of each other) moves a gradient by as much as
+// the rounding of the gradient itself does: together sqrt 2 times that.  The bias gradient takes d before it.
+// fp16 has steps of 2^-24 below 2^-14 and ends at 65504, so d is multiplied by the power of two that brings dy's largest finite magnitude A to [2^14, 2^15)
+// (a slope is at most 1.13), and the results by its inverse: down to 2^-28 A d keeps its eleven bits, below that steps of 2^-38 A, which a sum of M rows
+// sees beside its result's own only where A |x| sqrt M is past 2^14.  (Without, the gradients of a mean loss over a large batch lost
+// their bits: dy about 2^-16 and the sigmoid's slope, 16384 rows: an error of 5.3e-3 for 2.1e-4.)
 // Bound by memory, and behind it by the slopes' instructions: 16384 x 4096 bf16 (gelu) 90 us, 400 MB at 4.5 TB/s; 43008 x 768 with z in e4m3 (silu)
 // and 43008 x 512 codes of x behind it 50 us, 231 MB at 4.6.
 // The workgroups behind the slopes' stage the products' other operands: one launch in front of both products.
-struct SlopeJob { Saved dy, z; int act; long long M; int N; void* d; long long ldd; float* part; unsigned parts, blocks; };
+struct SlopeJob { Saved dy, z; int act; long long M; int N; void* d; long long ldd; float* part; unsigned parts, blocks; const float* most; int mosts; float* factor; };
 template <typename T>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeJob job, StageJob sa, StageJob sb) {
     if (blockIdx.x >= job.blocks) {
@@ -626,6 +671,14 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeJob job, StageJob sa, S
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = (int)by * 256 + lane * 8;
     const long long m0 = (long long)bx * 32 + w;
     float acc[8] = {};
+    const bool scaled = std::is_same<T, f16>::value && job.mosts;
+    float most = 0.f, times = 1.f;
+    if (scaled) {                                          // (every wave looks at all of them)
+#pragma unroll
+        for (int b = 0; b < kMosts; b += 64) most = fmaxf(most, job.most[min(b + (int)(threadIdx.x & 63), job.mosts - 1)]);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    }
     if (c < N) {
         float v[4][8], u[4][8];
         long long r[4];
@@ -633,6 +686,11 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeJob job, StageJob sa, S
         for (int q = 0; q < 4; ++q) r[q] = m0 + 8 * q < M ? m0 + 8 * q : M - 1;      // (no condition between the loads)
         load8s<T, 4>(dy, r, c, N, v);
         if (act != kActNone) load8s<T, 4>(z, r, c, N, u);
+        if (scaled) {
+            const int e = (int)(__float_as_uint(most) >> 23) - 127;      // (fp16's values are normal in fp32)
+            times = most > 0.f ? pow2_of_byte(127 + 14 - e) : 1.f;
+            if (blockIdx.x == 0 && threadIdx.x == 0) *job.factor = 1.f / times;
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (m0 + 8 * q >= M) break;
@@ -641,9 +699,13 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeJob job, StageJob sa, S
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[q][k] = c + k < N ? v[q][k] * u[q][k] : 0.f;
             }
-            if (d) store_row<T, 8>(d + (m0 + 8 * q) * ldd + c, 8, v[q]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) acc[k] += v[q][k];
+            if (scaled) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[q][k] *= times;
+            }
+            if (d) store_row<T, 8>(d + (m0 + 8 * q) * ldd + c, 8, v[q]);
         }
     }
     if (!part) return;

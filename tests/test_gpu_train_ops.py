@@ -620,3 +620,44 @@ def test_trainer_with_gates_in_8_bits_takes_less_memory():
         tr.close()
     rows = 21 * 2 * n * 256                                          # values of one gate array: 24 arrays in fp32 against 8, and 24 of 33 / 32 bytes
     assert abs((took[0] - took[1]) - rows * (16 * 4 - 24 * 33 / 32)) < 64 << 20, took
+
+
+# ---- gradients over the whole range of dy -----------------------------------------------------------------------------
+def check_range(dy, x, w, z, act, t, got, rounds):
+    """rounds: the relative error of a d before its products.  In fp16 a d below 2^-28 of dy's largest magnitude A is off by 2^-39 A at most."""
+    d = dy.double() * slope64(z.double(), act)
+    off = 2.0 ** -20 if t is not F32 else 2.0 ** -21
+    step = 2.0 ** -39 * float(dy[torch.isfinite(dy)].abs().max()) if t is F16 else 0.0
+    M, N = d.shape
+    for out, a, b, ay, n in ((got[0], d, w.double(), dy.double(), N), (got[1], d.t(), x.double(), dy.double().t(), M)):
+        q, qy, qb = mm(a ** 2, b ** 2).sqrt(), mm(ay ** 2, b ** 2).sqrt(), (b ** 2).sum(0).sqrt()
+        within(out, mm(a, b), (sum_tol(n) + 5 * rounds) * q + 5 * off * qy + 5 * step * qb, t)
+    if got[2] is not None:
+        within(got[2], d.sum(0), sum_tol(M) * (d ** 2).sum(0).sqrt() + 5 * off * (dy.double() ** 2).sum(0).sqrt(), t)
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "gelu"])
+@pytest.mark.parametrize("by", [2.0 ** -20, 2.0 ** -16, 2.0 ** -12, 1.0, 2.0 ** 8])
+@pytest.mark.parametrize("m,k,n", [(600, 40, 72), (3000, 64, 300), (1500, 129, 33)])
+def test_fp16_gradients_of_small_and_large_dy(m, k, n, by, act):
+    """the tile kernels: more than 512 rows"""
+    dy, x, z = normal(1, m, n, t=F16, by=by), normal(2, m, k, t=F16, by=min(1.0, 1 / by)), normal(4, m, n, t=F16)
+    w = normal(3, n, k, t=F16, by=k ** -0.5)
+    check_range(dy, x, w, z, act, F16, ops.linear_backward(dy, x, w, z, activation=act), H[F16])
+
+
+def test_fp16_sums_of_many_small_gradients():
+    """32768 rows of d = 8.9e-9 (dy: the smallest magnitude that fp16 has): dw = 2.9e-4; and one d past the type's range in a batch of small ones"""
+    m = 32768
+    dy, x, z = torch.full((m, 8), 2.0 ** -24, dtype=F16, device=DEV), torch.ones(m, 8, dtype=F16, device=DEV), torch.full((m, 8), 1.5, dtype=F16, device=DEV)
+    w = normal(3, 8, 8, t=F16)
+    check_range(dy, x, w, z, "sigmoid", F16, ops.linear_backward(dy, x, w, z, activation="sigmoid"), H[F16])
+    dy = normal(1, 600, 40, t=F16, by=0.05)
+    dy[1, 3] = 60000.0                                                # gelu's slope at 1.5 is 1.127
+    x, w, z = normal(2, 600, 32, t=F16, by=0.01), normal(3, 40, 32, t=F16, by=0.01), torch.full((600, 40), 1.5, dtype=F16, device=DEV)
+    check_range(dy, x, w, z, "gelu", F16, ops.linear_backward(dy, x, w, z, activation="gelu", need_db=False), H[F16])      # (db itself is past the range)
+
+
+def test_fp16_gradients_of_a_zero_dy():
+    dy, x, w, z = torch.zeros(600, 40, dtype=F16, device=DEV), normal(2, 600, 32, t=F16), normal(3, 40, 32, t=F16), normal(4, 600, 40, t=F16)
+    assert not any(v.any() for v in ops.linear_backward(dy, x, w, z, activation="gelu"))

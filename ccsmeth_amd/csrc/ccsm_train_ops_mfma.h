@@ -192,9 +192,47 @@ __device__ __forceinline__ Place place_of(int b, int tiles_i, int tiles_j, int s
     return Place{8 * band + in % rows, in / rows, split};
 }
 
-// a wave's 16 FI x 16 FJ results from (i_wave, jw) on
-template <typename T, int FI, int FJ, int NW>
-__device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, int wave, int lane, int i_wave, int jw, int split, const f32x4 (&acc)[FI][FJ]) {
+// Sums of products of values in pieces are NaN wherever an operand is infinite (its other pieces are NaN, and infinity times an empty piece is), or where
+// the largest products pass fp32's range and smaller ones of the other sign do too.  A wave that finds a NaN among its results makes
+// those sums again from one piece of each value: infinities, opposite infinities, infinity times zero and NaN then give what they give in fp32.
+// Finite results cost the look (one instruction for two of them).
+//
+// one piece of v: sign, exponent and seven bits; a NaN stays one, what is not zero does not become it
+__device__ __forceinline__ short leading(float v) {
+    const unsigned u = __float_as_uint(v), m = u & 0x7fffffffu;
+    return (short)((m > 0x7f800000u ? 0x7fc0u : m != 0 && m < 0x00800000u ? 0x0080u : m >> 16) | (u >> 16 & 0x8000u));
+}
+__device__ __forceinline__ s16x8 leading8(const float (&v)[8]) {
+    s16x8 p;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) p[k] = leading(v[k]);
+    return p;
+}
+__device__ __forceinline__ bool any_nan(const f32x4& v) { return __builtin_isunordered(v[0], v[1]) || __builtin_isunordered(v[2], v[3]); }
+__device__ __forceinline__ void replace_nan(f32x4& v, const f32x4& by) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] != v[e] ? by[e] : v[e];
+}
+// the sums over [first, last) of a 16 x 16 tile from (i0, j0) on, from one piece of each fp32 value; straight from memory, with a bounds check each
+template <bool TRP, bool TRQ>
+__device__ __forceinline__ f32x4 tile_of_leading(Plane P, Plane Q, int i0, int j0, int M, int N, int first, int last, int lane) {
+    const long long i = i0 + (lane & 15) < M ? i0 + (lane & 15) : M - 1, j = j0 + (lane & 15) < N ? j0 + (lane & 15) : N - 1;
+    auto eight = [&](const Plane& s, bool tr, long long r, int k) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = k + q < last ? ((const float*)s.base)[tr ? (k + q) * s.ld + r : r * s.ld + k + q] : 0.f;
+        return leading8(v);
+    };
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = first; k0 < last; k0 += 32) {
+        const int k = k0 + 8 * (lane >> 4);
+        acc = Mfma<b16>::run(eight(Q, TRQ, j, k), eight(P, TRP, i, k), acc);
+    }
+    return acc;
+}
+// a wave's 16 FI x 16 FJ results from (i_wave, jw) on; again(i, j): what the NaN among those of a 16 x 16 tile are replaced by (fp32)
+template <typename T, int FI, int FJ, int NW, typename Again>
+__device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, int wave, int lane, int i_wave, int jw, int split, f32x4 (&acc)[FI][FJ], Again again) {
     // The results leave through the wave's own part of LDS, 32 rows of i at a time (rows 16 bytes longer than they need: the lanes' writes fall on
     // different banks), and from there in pieces of eight neighbours of a row.  A lane's column does not change, so its bias is loaded once; a
     // round's residual is loaded a round ahead (one load at a time, 128 loads one behind the other, took 170 of 640 us of a 16384 x 4096 x 4096
@@ -203,6 +241,38 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, float* smem, in
     constexpr int WJT = 16 * FJ, kRow = WJT + 4, kPer = WJT / 8, kIt = 32 * kPer / 64, kRowsIt = 64 / kPer;
     static_assert(NW * 32 * kRow * 4 <= (NW == 8 ? 160 : 80) * 1024 && 64 % kPer == 0, "the waves' rows fit into the stages");
     float* out = smem + wave * 32 * kRow;
+    if constexpr (sizeof(T) == 4) {
+        bool nan = false;
+#pragma unroll
+        for (int p = 0; p < FI; ++p)
+#pragma unroll
+            for (int q = 0; q < FJ; ++q) nan |= any_nan(acc[p][q]);
+        if (__any(nan)) {                                  // (a row of tiles at a time, through the wave's part of LDS)
+            f32x4* mine = (f32x4*)out + lane;
+#pragma unroll 1
+            for (int h = 0; h < FI; ++h) {
+#pragma unroll
+                for (int p = 0; p < FI; ++p) {
+                    if (p != h) continue;
+#pragma unroll
+                    for (int q = 0; q < FJ; ++q) mine[64 * q] = acc[p][q];
+                }
+#pragma unroll 1
+                for (int q = 0; q < FJ; ++q) {
+                    f32x4 v = mine[64 * q];
+                    if (!__any(any_nan(v)) || i_wave + 16 * h >= a.M || jw + 16 * q >= a.N) continue;
+                    replace_nan(v, again(i_wave + 16 * h, jw + 16 * q));
+                    mine[64 * q] = v;
+                }
+#pragma unroll
+                for (int p = 0; p < FI; ++p) {
+                    if (p != h) continue;
+#pragma unroll
+                    for (int q = 0; q < FJ; ++q) acc[p][q] = mine[64 * q];
+                }
+            }
+        }
+    }
     const int c = lane % kPer * 8, j = jw + c, left_j = a.N - j, iw = i_wave + lane / kPer;
     const bool res = !a.part && a.ep.residual && left_j > 0;
     float bias[8];
@@ -361,11 +431,11 @@ __device__ __forceinline__ void product_mfma(const ProductArgs& a, int block) {
     for (int p = 0; p < FI; ++p)
 #pragma unroll
         for (int q = 0; q < FJ; ++q) asm volatile("" : "+v"(acc[p][q]));
-    store_tile<T, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), split, acc);
+    store_tile<T, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), split, acc, [](int, int) { return f32x4{}; });
 }
 
 // v as three bf16 values whose sum it is: the first eight bits cut off (so that no finite value becomes infinite), the rest rounded to nearest twice;
-// infinities and NaN make all of a product NaN
+// an infinity's are infinity and NaN twice
 __device__ __forceinline__ void three(float v, b16 (&p)[3]) {
     const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u), r = v - h;
     p[0] = __builtin_bit_cast(b16, (unsigned short)(__float_as_uint(v) >> 16));
@@ -504,7 +574,8 @@ __device__ __forceinline__ void product_f32(const ProductArgs& a, int block) {
         for (int r = 0; r < kReq; ++r) request_p(r, bp ^ kP);
         __builtin_amdgcn_sched_barrier(0);
     }
-    store_tile<float, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), at.split, acc);
+    store_tile<float, FI, FJ, NW>(a, reinterpret_cast<float*>(ops_smem), wave, lane, i0 + wi * HW, j0 + wj * (BJ / WJ), at.split, acc,
+                                  [&](int i, int j) { return tile_of_leading<TRP, TRQ>(a.P, a.Q, i, j, a.M, a.N, first, last, lane); });
 }
 
 template <typename T, bool TRP, bool TRQ, int B>
@@ -865,6 +936,39 @@ __device__ __forceinline__ void direct_product(const DirectArgs& a, DirectRoom<T
             for (int t = 0; t < G; ++t) multiply(x, pv[t], acc[t0 + t]);
             if (G < MT) __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    bool nan = false;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) nan |= any_nan(acc[t]);
+    if ((sizeof(T) == 4 || slope) && a.ep.y && __any(nan)) {      // (above: from one piece of each value)
+        f32x4 again[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) again[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (k0 = 0; k0 < a.K; k0 += step) {
+            const Loose<T, 8> qv = eight(a.Q, TRQ, j, k0, kl);
+            float v[8], u[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (float)qv.v[q];
+            const s16x8 x = leading8(v);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const Loose<T, 8> pv = eight(a.P, TRP, i[t], k0, kl);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = (float)pv.v[q];
+                if (slope) {
+                    const Loose<T, 8> zv = eight(a.Z, TRP, i[t], k0, kl);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) u[q] = (float)zv.v[q];
+                    slope_all<fast, 8>(u, a.act);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] *= u[q];
+                }
+                again[t] = Mfma<b16>::run(x, leading8(v), again[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) replace_nan(acc[t], again[t]);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) sum[wave][t][lane] = acc[t];

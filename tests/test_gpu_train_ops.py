@@ -661,3 +661,73 @@ def test_fp16_sums_of_many_small_gradients():
 def test_fp16_gradients_of_a_zero_dy():
     dy, x, w, z = torch.zeros(600, 40, dtype=F16, device=DEV), normal(2, 600, 32, t=F16), normal(3, 40, 32, t=F16), normal(4, 600, 40, t=F16)
     assert not any(v.any() for v in ops.linear_backward(dy, x, w, z, activation="gelu"))
+
+
+# ---- infinities and NaN -----------------------------------------------------------------------------------------------
+def check_special(got, ref, tol, t):
+    """infinite, of one sign or the other, and NaN where the 64-bit form is; within tolerance elsewhere"""
+    got, ref = got.cpu(), ref.cpu()
+    fin = torch.isfinite(ref)
+    assert 0 < int(fin.sum()) < fin.numel()
+    assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got == float("inf"), ref == float("inf")) and torch.equal(got == -float("inf"), ref == -float("inf"))
+    within(got[fin], ref[fin], tol.cpu()[fin], t)
+
+
+def host_mm(a, b):
+    return torch.mm(a.double().cpu(), b.double().cpu())
+
+
+def with_specials(v, rows, odd=0):
+    """v with infinities of both signs, a NaN, and zeros beside them, in the named rows"""
+    inf = float("inf")
+    v[rows[0], 3 + odd], v[rows[1], 5], v[rows[2], 0], v[rows[2], 7], v[rows[3], 2] = inf, -inf, inf, -inf, float("nan")
+    v[rows[4], 3], v[rows[4], 5] = 0.0, 0.0                            # (an infinity of the other operand meets a zero)
+    return v
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", [(6, 24, 40), (70, 1100, 40), (90, 1101, 33), (200, 40, 72), (3000, 64, 777)])
+def test_infinities_forward(t, m, k, n):
+    """the small kernel, the tiles with a split contraction, with staged operands, and without"""
+    x, w = with_specials(normal(1, m, k, t=t), (1, 2, 3, 4, 5)), normal(2, n, k, t=t, by=k ** -0.5)
+    w[7, 3], w[8, 5] = 0.0, 0.0
+    w[9, 1], w[10, 2] = float("inf"), -float("inf")
+    ref = host_mm(x, w.t())
+    tol = sum_tol(k) * host_mm(x.double() ** 2, w.double().t() ** 2).sqrt()
+    check_special(ops.linear(x, w), ref, tol, t)
+    y, z = ops.linear(x, w, None, x.new_ones(m, n), activation="relu", keep_preact=True)
+    check_special(z, ref, tol, t)
+    check_special(y, ref.clamp_min(0) + 1, tol + 2.0 ** -23 * (ref.abs() + 1), t)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ["none", "silu", "relu"])
+@pytest.mark.parametrize("m,k,n", [(8, 40, 64), (200, 40, 72), (700, 40, 72), (1500, 65, 77)])
+def test_infinities_backward(t, act, m, k, n):
+    dy, x, w = with_specials(normal(1, m, n, t=t, by=0.05), (1, 2, 3, 4, 5)), with_specials(normal(2, m, k, t=t), (0, 1, 6, 7, 5), 1), normal(3, n, k, t=t, by=0.2)
+    z = normal(4, m, n, t=t)
+    w[9, 1], w[10, 2] = float("inf"), -float("inf")
+    d = dy.double().cpu() * (slope64(z.double(), act).cpu() if act != "none" else 1.0)
+    got = ops.linear_backward(dy, x, w, z if act != "none" else None, activation=act)
+    hd, off = (0.0 if t is F32 or act == "none" else 5 * H[t]), (0.0 if act == "none" else 2.0 ** -20)
+    for out, a, b, ay, c in ((got[0], d, w, dy.cpu(), n), (got[1], d.t(), x, dy.cpu().t(), m)):
+        b = b.double().cpu()
+        check_special(out, host_mm(a, b), (sum_tol(c) + hd) * host_mm(a ** 2, b ** 2).sqrt() + 5 * off * host_mm(ay.double() ** 2, b ** 2).sqrt(), t)
+    check_special(got[2], d.sum(0), sum_tol(m) * (d ** 2).sum(0).sqrt() + 5 * off * (dy.double().cpu() ** 2).sum(0).sqrt(), t)
+
+
+@pytest.mark.parametrize("m,k,n", [(6, 24, 40), (70, 1100, 40), (3000, 64, 777)])
+def test_products_past_the_range_of_fp32_are_infinite(m, k, n):
+    """finite operands; and a NaN whose bits beyond the first sixteen alone say so, values of the smallest kind beside an infinity"""
+    x, w = normal(1, m, k), normal(2, n, k, by=k ** -0.5)
+    x[1, 3], x[2, 3] = 3.0e38, -3.0e38
+    w[:, 3] = 1.7e38
+    x[4, 5] = torch.tensor(0x7f800001, dtype=torch.int32).view(torch.float32)
+    x[5, 7], w[:, 7] = float("inf"), 2.0 ** -149
+    w[3, 7] = -2.0 ** -149
+    x[0, 3] = x[3, 3] = 0.0
+    x[5:, 3] = 0.0
+    y = ops.linear(x, w)
+    assert bool((y[1] == float("inf")).all()) and bool((y[2] == -float("inf")).all()) and bool(y[4].isnan().all())
+    assert float(y[5, 3]) == -float("inf") and bool((y[5, :3] == float("inf")).all()) and bool((y[5, 4:] == float("inf")).all())
+    assert torch.isfinite(y[0]).all() and torch.isfinite(y[3]).all()

@@ -459,6 +459,18 @@ __device__ __forceinline__ void three8(const float (&v)[8], s16x8 (&p)[3]) {
 #pragma unroll
     for (int q = 0; q < 3; ++q) p[q] = __builtin_bit_cast(s16x8, u32x4{o[q][0], o[q][1], o[q][2], o[q][3]});
 }
+// eight values as two fragments, rounded to nearest twice
+__device__ __forceinline__ void two8(const float (&v)[8], s16x8 (&p)[2]) {
+    unsigned o[2][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        o[0][k] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{v[2 * k], v[2 * k + 1]}), b16x2));
+        const f32x2 r{v[2 * k] - __uint_as_float(o[0][k] << 16), v[2 * k + 1] - __uint_as_float(o[0][k] & 0xffff0000u)};
+        o[1][k] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, b16x2));
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) p[q] = __builtin_bit_cast(s16x8, u32x4{o[q][0], o[q][1], o[q][2], o[q][3]});
+}
 // The fp32 product: the same tiles, rings and requests with chunks of 32 k; a fragment's eight values are read as fp32 and split into three bf16
 // fragments in registers (5.5 instructions a value), and each pair of fragments is multiplied six times: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); what is
 // left out is below 2^-22 of each product, 2^-25 in the mean.  Bound by the matrix pipe: 192 instructions of 16 cycles a chunk and wave, beside 2100
@@ -850,23 +862,37 @@ __device__ __forceinline__ void direct_product(const DirectArgs& a, DirectRoom<T
         for (int q = 0; q < 8; ++q) o.v[q] = q < left ? *(const T*)(p + q * s.ld * (long long)sizeof(T) + own) : (T)0.f;
         return o;
     };
-    // v becomes v act'(z), rounded, and `low` what the rounding leaves: both are multiplied, so that a 16-bit product here is as exact as one of the
-    // unrounded v act'(z) (the tile kernels' is rounded once: an error of 0.21e-3 of the values in fp16, beside the result's own of as
-    // much).  The second piece costs 1 us of 25
-    auto sloped = [&](Loose<T, 8>& v, const Loose<T, 8>& z, Loose<T, 8>& low, float& t) {
-        float u[8];
+    // d = v act'(z) and its sum
+    auto sloped = [&](const Loose<T, 8>& v, const Loose<T, 8>& z, float (&d)[8], float& t) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) u[q] = (float)z.v[q];
-        slope_all<fast, 8>(u, a.act);
+        for (int q = 0; q < 8; ++q) d[q] = (float)z.v[q];
+        slope_all<fast, 8>(d, a.act);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const float d = (float)v.v[q] * u[q];
-            t += d;
-            v.v[q] = (T)d;
-            if constexpr (sizeof(T) == 2) {
-                const float left = d - (float)v.v[q];             // (an infinity leaves nothing: not the other infinity, nor NaN)
-                low.v[q] = fabsf(left) < INFINITY ? (T)left : (T)0.f;
-            }
+            d[q] = (float)v.v[q] * d[q];
+            t += d[q];
+        }
+    };
+    // 16-bit products of unrounded d: two bf16 pieces of d, whose range is fp32's (fp16 pieces lost a d below 2^-14 and made one above 65504 infinite),
+    // with x as it is (bf16) or as the two bf16 pieces whose sum an fp16 value is.  What is left out of d is below 2^-16 of it.  (The tile kernels' d is
+    // rounded once to its type, an error beside the result's own of as much.)  The second piece of a bf16 d costs 1 us of 25
+    auto multiply_sloped = [&](const Loose<T, 8>& xv, const float (&d)[8], f32x4& c) {
+        s16x8 y[2];
+        two8(d, y);
+        if constexpr (std::is_same<T, f16>::value) {
+            float v[8];
+            s16x8 x[2];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (float)xv.v[q];
+            two8(v, x);
+            c = Mfma<b16>::run(x[1], y[1], c);
+            c = Mfma<b16>::run(x[0], y[1], c);
+            c = Mfma<b16>::run(x[1], y[0], c);
+            c = Mfma<b16>::run(x[0], y[0], c);
+        } else if constexpr (sizeof(T) == 2) {
+            const s16x8 x = __builtin_bit_cast(s16x8, xv);
+            c = Mfma<b16>::run(x, y[1], c);
+            c = Mfma<b16>::run(x, y[0], c);
         }
     };
     auto multiply = [&](const s16x8 (&x)[NP], const Loose<T, 8>& p, f32x4& c) {
@@ -922,18 +948,25 @@ __device__ __forceinline__ void direct_product(const DirectArgs& a, DirectRoom<T
             if (slope) {
 #pragma unroll
                 for (int t = 0; t < G; ++t) {
-                    Loose<T, 8> low;
-                    sloped(pv[t], zv[t], low, tot[t0 + t]);
-                    if constexpr (sizeof(T) == 2) multiply(x, low, acc[t0 + t]);
+                    float d[8];
+                    sloped(pv[t], zv[t], d, tot[t0 + t]);
+                    if constexpr (sizeof(T) == 2) multiply_sloped(qv, d, acc[t0 + t]);
+                    else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) pv[t].v[q] = d[q];
+                        multiply(x, pv[t], acc[t0 + t]);
+                    }
                 }
-            } else if (want) {
+            } else {
 #pragma unroll
-                for (int t = 0; t < G; ++t)
+                for (int t = 0; t < G; ++t) {
+                    if (want) {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) tot[t0 + t] += (float)pv[t].v[q];
+                        for (int q = 0; q < 8; ++q) tot[t0 + t] += (float)pv[t].v[q];
+                    }
+                    multiply(x, pv[t], acc[t0 + t]);
+                }
             }
-#pragma unroll
-            for (int t = 0; t < G; ++t) multiply(x, pv[t], acc[t0 + t]);
             if (G < MT) __builtin_amdgcn_sched_barrier(0);
         }
     }

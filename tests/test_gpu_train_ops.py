@@ -731,3 +731,22 @@ def test_products_past_the_range_of_fp32_are_infinite(m, k, n):
     assert bool((y[1] == float("inf")).all()) and bool((y[2] == -float("inf")).all()) and bool(y[4].isnan().all())
     assert float(y[5, 3]) == -float("inf") and bool((y[5, :3] == float("inf")).all()) and bool((y[5, 4:] == float("inf")).all())
     assert torch.isfinite(y[0]).all() and torch.isfinite(y[3]).all()
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "gelu"])
+@pytest.mark.parametrize("by", [2.0 ** -20, 2.0 ** -16, 2.0 ** -12, 1.0, 2.0 ** 8])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 72), (20, 600, 300), (300, 129, 33), (500, 200, 60)])
+def test_fp16_gradients_of_small_and_large_dy_small_products(m, k, n, by, act):
+    """the small kernel takes d in two pieces of bf16: off by 2^-16 of it (and 2^-133, bf16's smallest step, which is none beside fp16's)"""
+    dy, x, z = normal(1, m, n, t=F16, by=by), normal(2, m, k, t=F16, by=min(1.0, 1 / by)), normal(4, m, n, t=F16)
+    w = normal(3, n, k, t=F16, by=k ** -0.5)
+    check_range(dy, x, w, z, act, F16, ops.linear_backward(dy, x, w, z, activation=act), 2.0 ** -16)
+
+
+def test_fp16_small_products_of_a_d_past_the_range():
+    dy = normal(1, 60, 40, t=F16, by=0.05)
+    dy[1, 3], dy[7, 0], dy[8, 0] = 60000.0, 2.0 ** -24, -2.0 ** -20      # gelu's slope at 1.5 is 1.127
+    dy[7, 1:], dy[8, 1:] = 0.0, 0.0
+    x, w, z = normal(2, 60, 32, t=F16, by=0.01), normal(3, 40, 32, t=F16, by=0.01), torch.full((60, 40), 1.5, dtype=F16, device=DEV)
+    w[0] = 60.0
+    check_range(dy, x, w, z, "gelu", F16, ops.linear_backward(dy, x, w, z, activation="gelu", need_db=False), 2.0 ** -16)

@@ -61,10 +61,12 @@ unsigned grid_of(int64_t n, int64_t most = 1 << 20) { return (unsigned)(n < 1 ? 
 
 bool spanned(int64_t k, int type) { return 255 * (int64_t)up((size_t)k, 8) * (int64_t)size_of(type) + 128 <= kExtent; }
 
-// scratch of a call, handed out piece by piece; without a base it only counts
+// scratch of a call, handed out piece by piece; without a base it only counts.  What the call takes beside it: the tile's edge (0: the small kernel) and
+// the parts of each product's contraction (0: no such product), operands staged
 struct Scratch {
     char* base = nullptr;
     size_t used = 0;
+    int tile = 0, parts[2] = {0, 0}, staged = 0;
     template <typename T> T* take(size_t n) {
         T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
         used += up(n * sizeof(T), 256);
@@ -109,6 +111,7 @@ struct Staging {
         const int64_t ld = (int64_t)up(width, 8);
         T* out = ws.take<T>((size_t)rows * ld);
         jobs[count++] = StageJob{s, rows * ld / 8, (int)width, out, ld};
+        ws.staged = count;
         return Plane{out, ld};
     }
     unsigned blocks() const { return grid_of(cdiv(jobs[0].items + jobs[1].items, 256), 1 << 16); }
@@ -217,6 +220,8 @@ template <typename T, bool TRP, bool TRQ>
 hipError_t product(hipStream_t st, const Plane& p, const Plane& q, int64_t M, int64_t N, int64_t K, const Epilogue& ep, Scratch& ws, JoinJob* join, bool count) {
     const Shape shape = shape_of(M, N, chunks_of<T>(K), sizeof(T) == 4);
     const ProductArgs a = product_args<T>(p, q, M, N, K, chunks_of<T>(K), shape, ep, ws, join);
+    ws.tile = shape.tile;
+    ws.parts[TRP] = a.splits;
     if (count) return hipSuccess;
     return shape.tile == 256 ? launch_product<T, TRP, TRQ, 256>(a, st) : launch_product<T, TRP, TRQ, 128>(a, st);
 }
@@ -367,6 +372,9 @@ ccsm_status linear_backward(const ccsm_linear_grad* p, Scratch& ws, hipStream_t 
         const Pair both = pair_of({M, (int64_t)N}, {(int64_t)K, (int64_t)K}, chunks, sizeof(T) == 4);
         const ProductArgs ax = product_args<T>(d, w, M, K, N, chunks[0], Shape{both.tile, both.splits[0]}, to_dx, ws, &join_x);
         const ProductArgs aw = product_args<T>(d, x, N, K, M, chunks[1], Shape{both.tile, both.splits[1]}, to_dw, ws, &join_w);
+        ws.tile = both.tile;
+        ws.parts[0] = ax.splits;
+        ws.parts[1] = aw.splits;
         if (!count) TRY((both.tile == 256 ? launch_pair<T, 256>(ax, aw, st) : launch_pair<T, 128>(ax, aw, st)), "linear_backward: dx and dw");
     } else if (p->dx) TRY((product<T, false, true>(st, d, w, M, K, N, to_dx, ws, &join_x, count)), "linear_backward: dx");
     else if (p->dw) TRY((product<T, true, true>(st, d, x, N, K, M, to_dw, ws, &join_w, count)), "linear_backward: dw");
@@ -496,6 +504,26 @@ ccsm_status ccsm_train_linear_backward(int device, const ccsm_linear_grad* p, vo
     Scratch ws;
     ws.base = (char*)workspace;
     TYPED(p->type, return linear_backward<T>(p, ws, (hipStream_t)stream, false));
+}
+
+static void way_of(const Scratch& ws, int32_t* way) { way[0] = ws.tile; way[1] = ws.parts[0]; way[2] = ws.parts[1]; way[3] = ws.staged; }
+ccsm_status ccsm_train_linear_way(const ccsm_linear* p, int32_t* way) {
+    const ccsm_status e = check_linear(p);
+    if (e != CCSM_OK) return e;
+    REFUSE(!way, "linear_way: NULL argument");
+    Scratch ws;
+    if (p->rows) TYPED(p->type, (void)linear_forward<T>(p, ws, nullptr, true));
+    way_of(ws, way);
+    return CCSM_OK;
+}
+ccsm_status ccsm_train_linear_backward_way(const ccsm_linear_grad* p, int32_t* way) {
+    const ccsm_status e = check_grad(p);
+    if (e != CCSM_OK) return e;
+    REFUSE(!way, "linear_backward_way: NULL argument");
+    Scratch ws;
+    TYPED(p->type, (void)linear_backward<T>(p, ws, nullptr, true));
+    way_of(ws, way);
+    return CCSM_OK;
 }
 
 ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,

@@ -21,7 +21,7 @@ from . import _lib
 from . import train as _train
 
 EXPORTS = ("ccsm_train_ops_last_error", "ccsm_train_linear_workspace", "ccsm_train_linear_forward", "ccsm_train_linear_backward_workspace",
-           "ccsm_train_linear_backward", "ccsm_train_embedding_forward", "ccsm_train_embedding_backward_workspace",
+           "ccsm_train_linear_backward", "ccsm_train_linear_way", "ccsm_train_linear_backward_way", "ccsm_train_embedding_forward", "ccsm_train_embedding_backward_workspace",
            "ccsm_train_embedding_backward", "ccsm_train_act8_pack", "ccsm_train_act8_unpack")
 ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "sigmoid": 3, "gelu": 4, "silu": 5}
 CODES = {"int8": 1, "e4m3": 2}
@@ -66,6 +66,7 @@ def load():
     lib.ccsm_train_linear_backward_workspace.argtypes = [vp]
     lib.ccsm_train_linear_backward_workspace.restype = cs
     lib.ccsm_train_linear_backward.argtypes = [ci, vp, vp, cs, vp]
+    lib.ccsm_train_linear_way.argtypes = lib.ccsm_train_linear_backward_way.argtypes = [vp, vp]
     lib.ccsm_train_embedding_forward.argtypes = [ci, ci, ci, cl, vp, cl, C.c_int32, vp, cl, cf, vp, cl, vp]
     lib.ccsm_train_embedding_backward_workspace.argtypes = [ci, cl, cl, C.c_int32]
     lib.ccsm_train_embedding_backward_workspace.restype = cs

@@ -85,6 +85,12 @@ ccsm_status ccsm_train_linear_forward(int device, const ccsm_linear* p, void* wo
 size_t ccsm_train_linear_backward_workspace(const ccsm_linear_grad* p);
 ccsm_status ccsm_train_linear_backward(int device, const ccsm_linear_grad* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Which kernels such a call takes, for tests and profiles; nothing is launched.  way[0]: the edge of the products' tiles (256 or 128; 0: the kernel for
+ * small products and few rows, or none); way[1], way[2]: into how many parts the contraction is split (forward: way[1]; backward: of dx, of dw;
+ * 0: no tiles); way[3]: operands staged in front. */
+ccsm_status ccsm_train_linear_way(const ccsm_linear* p, int32_t* way);
+ccsm_status ccsm_train_linear_backward_way(const ccsm_linear_grad* p, int32_t* way);
+
 /* ids outside [0, rows) are no tokens (padding): their row of y is zero and they have no gradient.  y (tokens, width) = scale table[ids]. */
 ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int32_t width,
                                          const void* table, int64_t ldt, float scale, void* y, int64_t ldy, void* stream);

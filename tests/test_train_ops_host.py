@@ -178,3 +178,16 @@ def test_contractions_whose_offsets_leave_32_bits_are_refused(kind, most):
         assert lib.ccsm_train_linear_backward(0, C.byref(g), None, 0, None) == (CAPACITY if ok else INVALID)
         g.dx = None                                                                     # dw and dbias run along rows: no limit but that of the columns
         assert lib.ccsm_train_linear_backward(0, C.byref(g), None, 0, None) == CAPACITY
+
+
+def test_the_way_of_a_call():
+    """the query that tests and profiles ask which kernel a call takes"""
+    lib, way = ops.load(), (C.c_int32 * 4)()
+    for m, k, n, want in ((64, 4096, 4096, (0, 0, 0, 0)), (300, 500, 400, (0, 0, 0, 0)), (3001, 67, 777, (128, 1, 0, 2)), (16384, 4096, 4096, (256, 1, 0, 0))):
+        assert lib.ccsm_train_linear_way(C.byref(_linear(rows=m, inner=k, outer=n, ldx=k, ldw=k, ldy=n, ldr=n, ldp=n)), way) == 0 and tuple(way) == want
+    for m, k, n, tile in ((20, 60, 40, 0), (600, 40, 72, 128), (16384, 4096, 4096, 256)):
+        g = _grad(rows=m, inner=k, outer=n, lddy=n, ldw=k, lddx=k, lddw=k, x=ops.Saved(A, k, 0, None, 0), preact=ops.Saved(A, n, 0, None, 0))
+        assert lib.ccsm_train_linear_backward_way(C.byref(g), way) == 0 and way[0] == tile
+    assert lib.ccsm_train_linear_way(C.byref(_linear(rows=0)), way) == 0 and tuple(way) == (0, 0, 0, 0)
+    assert lib.ccsm_train_linear_way(None, way) == INVALID and lib.ccsm_train_linear_way(C.byref(_linear(inner=0)), way) == INVALID
+    assert lib.ccsm_train_linear_way(C.byref(_linear()), None) == INVALID and lib.ccsm_train_linear_backward_way(C.byref(_grad()), None) == INVALID

@@ -11,8 +11,8 @@ What torch.nn does for the reference here: nn.Embedding (ccsmeth/models.py:35, 9
 
 Tensors are float32, float16 or bfloat16 on one GPU, one type per call.  Work is enqueued on `stream` (a torch.cuda.Stream; default: torch's
 current stream of the tensors' device) and nothing waits for the GPU; calls can be captured into a graph.  Row-strided views are taken as
-they are, other layouts are copied.  There is no autograd: gradients are calls, as in Trainer.forward_backward, and inputs that require a
-gradient are refused while grad mode is on.  There is no CPU path.
+they are, other layouts are copied.  There is no autograd: gradients are calls, as in Trainer.forward_backward; inputs that require a
+gradient are refused while grad mode is on, and those with a forward-mode tangent.  There is no CPU path.
 """
 import ctypes as C
 import struct
@@ -87,13 +87,14 @@ def _types():
     return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}, {torch.uint8: 0, torch.int32: 1, torch.int64: 2}
 
 
-_TYPE = _ID = _torch = _Tensor = None
+_TYPE = _ID = _torch = _Tensor = _forward = None
 
 
 def _init():
-    global _TYPE, _ID, _torch, _Tensor
+    global _TYPE, _ID, _torch, _Tensor, _forward
     if _torch is None:
         import torch
+        import torch.autograd.forward_ad as _forward
         _TYPE, _ID = _types()
         _torch, _Tensor = torch, torch.Tensor
     return _torch
@@ -111,7 +112,14 @@ def _tensor(t, name, dtype=None, device=None):
         raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires a gradient: these calls are not seen by autograd (use torch.no_grad() and the *_backward calls)" % name)
+    if _dual() and _forward.unpack_dual(t).tangent is not None:
+        raise ValueError("%s has a forward-mode tangent: these calls are not seen by autograd" % name)
     return t
+
+
+def _dual():
+    """whether tensors may have forward-mode tangents (a dual level is entered)"""
+    return getattr(_forward, "_current_level", 0) >= 0
 
 
 def _on_gpu(t, name):
@@ -123,7 +131,7 @@ def _on_gpu(t, name):
 # leave it to the ones above to say what is.
 def _lead(t, name):
     """the type and the device's number of a call's first tensor"""
-    if type(t) is not _Tensor or t.dtype not in _TYPE or t.requires_grad or not t.is_cuda:
+    if type(t) is not _Tensor or t.dtype not in _TYPE or t.requires_grad or not t.is_cuda or _dual():
         _tensor(t, name)
         _on_gpu(t, name)
     return t.dtype, t.get_device()
@@ -131,7 +139,7 @@ def _lead(t, name):
 
 def _same(t, name, dtype, at, lead):
     """t, of the call's type and on its device"""
-    if type(t) is _Tensor and t.dtype is dtype and t.get_device() == at and not t.requires_grad:
+    if type(t) is _Tensor and t.dtype is dtype and t.get_device() == at and not t.requires_grad and not _dual():
         return t
     return _tensor(t, name, dtype, lead.device)
 

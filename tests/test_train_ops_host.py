@@ -191,3 +191,20 @@ def test_the_way_of_a_call():
     assert lib.ccsm_train_linear_way(C.byref(_linear(rows=0)), way) == 0 and tuple(way) == (0, 0, 0, 0)
     assert lib.ccsm_train_linear_way(None, way) == INVALID and lib.ccsm_train_linear_way(C.byref(_linear(inner=0)), way) == INVALID
     assert lib.ccsm_train_linear_way(C.byref(_linear()), None) == INVALID and lib.ccsm_train_linear_backward_way(C.byref(_grad()), None) == INVALID
+
+
+def test_forward_mode_tangents_are_refused():
+    """they would be lost: in every place of a call, and of other tensors' levels nothing is refused"""
+    import torch.autograd.forward_ad as fw
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.linear(dual, w), lambda: ops.linear_backward(dual, x, torch.zeros(8, 8)), lambda: ops.checkpoint8(dual),
+                     lambda: ops.embedding(torch.zeros(3, dtype=torch.int64), dual), lambda: ops.embedding_backward(dual, torch.zeros(4, dtype=torch.int64), 5)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        with pytest.raises(ValueError, match="tangent"):
+            ops._same(dual, "weight", torch.float32, -1, x)
+        with pytest.raises(ValueError, match="GPU"):
+            ops.linear(x, w)
+        assert ops._same(w, "weight", torch.float32, -1, x) is w

@@ -80,6 +80,28 @@ struct Scratch {
         else { typedef b16 T; __VA_ARGS__; }                                   \
     } while (0)
 
+// a matrix in memory: rows of `wide` bytes, `ld` bytes from one to the next
+struct Held { const void* p; int64_t ld, rows, wide; };
+Held held(const void* p, int64_t ld, int64_t rows, int64_t cols, size_t size) { return Held{p, ld * (int64_t)size, rows, cols * (int64_t)size}; }
+// whether two of them share memory: their ranges meet, and they are not different columns of the same rows (of one row, the other's stride)
+bool meet(const Held& a, const Held& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+    const char *pa = (const char*)a.p, *pb = (const char*)b.p;
+    if (pb >= pa + (a.rows - 1) * a.ld + a.wide || pa >= pb + (b.rows - 1) * b.ld + b.wide) return false;
+    if (a.rows == 1 && b.rows == 1) return true;
+    if (a.rows > 1 && b.rows > 1 && a.ld != b.ld) return true;
+    const int64_t step = a.rows > 1 ? a.ld : b.ld, off = ((pb - pa) % step + step) % step;
+    return off < a.wide || off + b.wide > step;
+}
+template <size_t NO, size_t NI>
+bool shared(const Held (&out)[NO], const Held (&in)[NI]) {
+    for (size_t o = 0; o < NO; ++o) {
+        for (const Held& i : in) if (meet(out[o], i)) return true;
+        for (size_t q = o + 1; q < NO; ++q) if (meet(out[o], out[q])) return true;
+    }
+    return false;
+}
+
 ccsm_status check_saved(const ccsm_saved& s, int type, int64_t width, const char* what) {
     REFUSE(!s.data, what);
     if (s.code == CCSM_CODE_NONE) {
@@ -92,6 +114,12 @@ ccsm_status check_saved(const ccsm_saved& s, int type, int64_t width, const char
     REFUSE(s.ld % 32 != 0 || s.ld < (int64_t)up(width, 32) || s.lds < cdiv(width, 32), "a kept matrix in 8 bits: ld is a multiple of 32 and covers whole blocks, lds the blocks");
     REFUSE(off_by(s.data, 16), "a kept matrix in 8 bits is 16-byte aligned");
     return CCSM_OK;
+}
+Held held(const ccsm_saved& s, int64_t rows, int64_t cols, int type) {
+    return s.code == CCSM_CODE_NONE ? held(s.data, s.ld, rows, cols, size_of(type)) : held(s.data, s.ld, rows, (int64_t)up((size_t)cols, 32), 1);
+}
+Held held_scales(const ccsm_saved& s, int64_t rows, int64_t cols) {
+    return s.code == CCSM_CODE_NONE ? Held{nullptr, 0, 0, 0} : held(s.scales, s.lds, rows, cdiv(cols, 32), 1);
 }
 Saved saved_of(const ccsm_saved& s) { return Saved{s.data, s.ld, s.code, s.scales, s.lds}; }
 Saved plain(const void* p, int64_t ld) { return Saved{p, ld, kCodeNone, nullptr, 0}; }
@@ -275,6 +303,13 @@ ccsm_status check_linear(const ccsm_linear* p) {
     REFUSE(off_by(p->x, s) || off_by(p->w, s) || off_by(p->y, s) || off_by(p->bias, s) || off_by(p->residual, s) || off_by(p->preact, s), "linear: a pointer is not aligned to its elements");
     return CCSM_OK;
 }
+ccsm_status apart(const ccsm_linear* p) {
+    const size_t s = size_of(p->type);
+    const Held y = held(p->y, p->ldy, p->rows, p->outer, s), pre = held(p->preact, p->ldp, p->rows, p->outer, s), r = held(p->residual, p->ldr, p->rows, p->outer, s);
+    const Held out[] = {y, pre}, in[] = {held(p->x, p->ldx, p->rows, p->inner, s), held(p->w, p->ldw, p->outer, p->inner, s), held(p->bias, p->outer, 1, p->outer, s)};
+    REFUSE(shared(out, in) || meet(pre, r) || (meet(y, r) && (p->y != p->residual || (p->rows > 1 && p->ldy != p->ldr))), "linear: an output shares memory with another tensor");
+    return CCSM_OK;
+}
 template <typename T>
 ccsm_status linear_forward(const ccsm_linear* p, Scratch& ws, hipStream_t st, bool count) {
     const Epilogue ep{p->bias, p->residual, p->ldr, p->y, p->ldy, p->preact, p->ldp, p->activation};
@@ -314,6 +349,15 @@ ccsm_status check_grad(const ccsm_linear_grad* p) {
         }
     }
     REFUSE(p->dw && p->lddw < p->inner, "linear_backward: a row stride is less than the row's width");
+    return CCSM_OK;
+}
+ccsm_status apart(const ccsm_linear_grad* p) {
+    const size_t s = size_of(p->type);
+    const int64_t M = p->rows, K = p->inner, N = p->outer;
+    const ccsm_saved none = {}, x = p->dw ? p->x : none, z = p->activation == CCSM_ACT_NONE ? none : p->preact;
+    const Held out[] = {held(p->dx, p->lddx, M, K, s), held(p->dw, p->lddw, N, K, s), held(p->dbias, N, 1, N, s)};
+    const Held in[] = {held(p->dy, p->lddy, M, N, s), held(p->dx ? p->w : nullptr, p->ldw, N, K, s), held(x, M, K, p->type), held_scales(x, M, K), held(z, M, N, p->type), held_scales(z, M, N)};
+    REFUSE(shared(out, in), "linear_backward: an output shares memory with another tensor");
     return CCSM_OK;
 }
 template <typename T>
@@ -444,6 +488,7 @@ void few_sums(hipStream_t st, const FewPlan& f, const void* ids, int id_type, in
                                                                                         (const T*)dy, lddy, part, f.part_ld);
     few_join_kernel<T><<<(unsigned)cdiv(rows * f.part_ld, 64), 256, 0, st>>>(part, f.part_ld, (int)f.blocks, rows, width, scale, (T*)dt, ldt);
 }
+Held held_ids(const void* ids, int id_type, int64_t tokens) { return held(ids, tokens, 1, tokens, id_type == CCSM_ID_U8 ? 1 : id_type == CCSM_ID_I32 ? 4 : 8); }
 ccsm_status check_embedding(int type, int id_type, int64_t tokens, const void* ids, int64_t rows, int width) {
     REFUSE(!good_type(type), "embedding: unknown type");
     REFUSE(id_type < CCSM_ID_U8 || id_type > CCSM_ID_I64, "embedding: unknown type of ids");
@@ -483,7 +528,7 @@ size_t ccsm_train_linear_workspace(const ccsm_linear* p) {
 ccsm_status ccsm_train_linear_forward(int device, const ccsm_linear* p, void* workspace, size_t workspace_bytes, void* stream) {
     ccsm_status e = check_linear(p);
     if (e != CCSM_OK || p->rows == 0) return e;
-    if ((e = check_room(ccsm_train_linear_workspace(p), workspace, workspace_bytes)) != CCSM_OK) return e;
+    if ((e = check_room(ccsm_train_linear_workspace(p), workspace, workspace_bytes)) != CCSM_OK || (e = apart(p)) != CCSM_OK) return e;
     ON_DEVICE(device);
     Scratch ws;
     ws.base = (char*)workspace;
@@ -499,7 +544,7 @@ size_t ccsm_train_linear_backward_workspace(const ccsm_linear_grad* p) {
 ccsm_status ccsm_train_linear_backward(int device, const ccsm_linear_grad* p, void* workspace, size_t workspace_bytes, void* stream) {
     ccsm_status e = check_grad(p);
     if (e != CCSM_OK) return e;
-    if ((e = check_room(ccsm_train_linear_backward_workspace(p), workspace, workspace_bytes)) != CCSM_OK) return e;
+    if ((e = check_room(ccsm_train_linear_backward_workspace(p), workspace, workspace_bytes)) != CCSM_OK || (e = apart(p)) != CCSM_OK) return e;
     ON_DEVICE(device);
     Scratch ws;
     ws.base = (char*)workspace;
@@ -532,6 +577,8 @@ ccsm_status ccsm_train_embedding_forward(int device, int type, int id_type, int6
     if (e != CCSM_OK || tokens == 0) return e;
     REFUSE(!table || !y || ldt < width || ldy < width, "embedding: table and y must be non-NULL, their strides at least the width");
     REFUSE(off_by(table, size_of(type)) || off_by(y, size_of(type)), "embedding: a pointer is not aligned to its elements");
+    const Held out[] = {held(y, ldy, tokens, width, size_of(type))}, in[] = {held(table, ldt, rows, width, size_of(type)), held_ids(ids, id_type, tokens)};
+    REFUSE(shared(out, in), "embedding: y shares memory with another tensor");
     ON_DEVICE(device);
     hipStream_t st = (hipStream_t)stream;
     TYPED(type, constexpr int P = 16 / sizeof(T); const int64_t pieces = cdiv(width, P);
@@ -561,6 +608,8 @@ ccsm_status ccsm_train_embedding_backward(int device, int type, int id_type, int
     REFUSE(!dtable || ldt < width || (tokens && (!dy || lddy < width)), "embedding: dy and dtable must be non-NULL, their strides at least the width");
     REFUSE(off_by(dtable, size_of(type)) || off_by(dy, size_of(type)), "embedding: a pointer is not aligned to its elements");
     if ((e = check_room(ccsm_train_embedding_backward_workspace(type, tokens, rows, width), workspace, workspace_bytes)) != CCSM_OK) return e;
+    const Held out[] = {held(dtable, ldt, rows, width, size_of(type))}, in[] = {held(dy, lddy, tokens, width, size_of(type)), held_ids(ids, id_type, tokens)};
+    REFUSE(shared(out, in), "embedding: dtable shares memory with another tensor");
     ON_DEVICE(device);
     hipStream_t st = (hipStream_t)stream;
     if (tokens == 0) {
@@ -604,6 +653,9 @@ ccsm_status ccsm_train_act8_pack(int device, int type, int code, int64_t rows, i
     REFUSE(!x || ldx < width || off_by(x, size_of(type)), "act8_pack: x must be non-NULL and aligned to its elements, its stride at least the width");
     ccsm_status e = check_saved(ccsm_saved{codes, ldc, code, scales, lds}, type, width, "act8_pack: codes must be non-NULL");
     if (e != CCSM_OK) return e;
+    const ccsm_saved s{codes, ldc, code, scales, lds};
+    const Held out[] = {held(s, rows, width, type), held_scales(s, rows, width)}, in[] = {held(x, ldx, rows, width, size_of(type))};
+    REFUSE(shared(out, in), "act8_pack: codes or scales share memory with another tensor");
     ON_DEVICE(device);
     const int64_t per = 2 * cdiv(width, 32);
     TYPED(type, in_ranges(rows, per, [&](int64_t r, int64_t n) {
@@ -623,6 +675,8 @@ ccsm_status ccsm_train_act8_unpack(int device, int type, int64_t rows, int32_t w
     ccsm_status e = check_saved(*s, type, width, "act8_unpack: codes must be non-NULL");
     if (e != CCSM_OK) return e;
     REFUSE(!y || ldy < width || off_by(y, size_of(type)), "act8_unpack: y must be non-NULL and aligned to its elements, its stride at least the width");
+    const Held out[] = {held(y, ldy, rows, width, size_of(type))}, in[] = {held(*s, rows, width, type), held_scales(*s, rows, width)};
+    REFUSE(shared(out, in), "act8_unpack: y shares memory with another tensor");
     ON_DEVICE(device);
     const int64_t per = cdiv(width, 16);
     TYPED(type, in_ranges(rows, per, [&](int64_t r, int64_t n) {

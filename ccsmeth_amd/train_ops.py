@@ -258,7 +258,7 @@ class Checkpoint8:
             y, width = codes.new_empty(shape, dtype=dtype), shape[-1]
             ldy = width
         else:
-            y, width = _out(out, shape, dtype, self.device, "out"), shape[-1]
+            y, width = _out(_tensor(out, "out"), shape, dtype, self.device, "out"), shape[-1]
             ldy = _rows(y)[1]
         at = codes.get_device()
         _check(lib.ccsm_train_act8_unpack(at, _TYPE[dtype], codes.shape[0], width, _SAVED.pack(*self._saved()), y.data_ptr(), ldy, _raw_stream(at)))
@@ -289,7 +289,8 @@ def checkpoint8(x, code="int8", *, stream=None):
 
 def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=False, *, out=None, stream=None):
     """y = act(x weight^T + bias) + residual; x (..., inner), weight (outer, inner), bias (outer), residual and y (..., outer).
-    keep_preact: -> (y, z) with z = x weight^T + bias as linear_backward takes it.  out: where y goes (it may be the residual)."""
+    keep_preact: -> (y, z) with z = x weight^T + bias as linear_backward takes it.  out: where y goes; it may be the residual and shares no memory with
+    the other tensors."""
     lib = _library()
     act = _activation(activation)
     t, at = _lead(x, "x")

@@ -17,8 +17,8 @@
  * captured into a graph; nothing is kept from one call for the next.  `workspace` is scratch of at least *_workspace() bytes, 256-byte
  * aligned, used until the enqueued work is done: calls that may run at the same time, two captured graphs among them, need one each.
  * The current device is the caller's again when a call returns.  Sums, activations and their slopes are computed in 32 bits or more and
- * rounded once; results do not depend on timing (no floating-point atomics).  Outputs may not overlap inputs, except y the residual (same
- * base and stride).  Zero rows (or tokens) are allowed: gradients of weights are then zero.  Refusals: CCSM_ERR_INVALID_ARG (text in
+ * rounded once; results do not depend on timing (no floating-point atomics).  Outputs share no memory with inputs or each other, except y the residual
+ * (same base and stride); columns of the same rows are apart, other views whose ranges of memory meet count as shared.  Zero rows (or tokens) are allowed: gradients of weights are then zero.  Refusals: CCSM_ERR_INVALID_ARG (text in
  * ccsm_train_ops_last_error), CCSM_ERR_CAPACITY for a workspace that is too small.
  */
 #ifndef CCSM_TRAIN_OPS_H_

@@ -13,6 +13,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from ccsmeth_amd import train_ops as ops  # noqa: E402
+from ccsmeth_amd._lib import CcsmError  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -750,3 +751,22 @@ def test_fp16_small_products_of_a_d_past_the_range():
     x, w, z = normal(2, 60, 32, t=F16, by=0.01), normal(3, 40, 32, t=F16, by=0.01), torch.full((60, 40), 1.5, dtype=F16, device=DEV)
     w[0] = 60.0
     check_range(dy, x, w, z, "gelu", F16, ops.linear_backward(dy, x, w, z, activation="gelu", need_db=False), 2.0 ** -16)
+
+
+def test_outputs_that_share_memory_are_refused():
+    hold = normal(1, 40, 96)
+    x, y, w = hold[:, :32], hold[:, 32:64], normal(2, 32, 32)
+    want = ops.linear(x, w, residual=y)
+    for call in (lambda: ops.linear(x, w, out=x), lambda: ops.linear(x, w, out=hold[:, 20:52]), lambda: ops.linear(x[:32], w, out=w), lambda: ops.linear(x, w, residual=hold[:, 40:72], out=y),
+                 lambda: ops.linear(x, w, bias=hold[3, 33:65], out=y), lambda: ops.embedding(torch.zeros(32, dtype=torch.int64, device=DEV), w, out=w),
+                 lambda: ops.embedding_backward(x, torch.zeros(40, dtype=torch.int64, device=DEV), 32, out=hold[:32, 16:48])):
+        with pytest.raises(CcsmError, match="shares memory"):
+            call()
+    got = ops.linear(x, w, residual=y, out=y)                         # beside x in the same rows, and the residual itself
+    assert got is y and torch.equal(y, want)
+    room = torch.zeros(40 * 32 * 4, dtype=torch.uint8, device=DEV)
+    c = ops.checkpoint8(x)
+    room[:1280].copy_(c.codes.reshape(-1))
+    c = ops.Checkpoint8(room[:1280].view(40, 32), c.scales, c.shape, F32, "int8")
+    with pytest.raises(CcsmError, match="shares memory"):
+        c.values(out=room.view(F32).view(40, 32))

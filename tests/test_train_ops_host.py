@@ -208,3 +208,32 @@ def test_forward_mode_tangents_are_refused():
         with pytest.raises(ValueError, match="GPU"):
             ops.linear(x, w)
         assert ops._same(w, "weight", torch.float32, -1, x) is w
+
+
+def test_outputs_that_share_memory_are_refused():
+    """(on no device: a call that were not refused would end there)"""
+    nowhere = 1 << 20
+    lib = ops.load()
+    apart = dict(x=A, w=A << 1, bias=A << 2, residual=A << 3, y=A << 4, preact=A << 5)
+    wide = dict(apart, ldy=112, ldx=112)                             # x beside y in the same rows
+    y = A << 4
+    for kw in (dict(apart, y=A), dict(apart, y=A << 1), dict(apart, y=(A << 2) + 94), dict(apart, y=A << 5), dict(apart, y=(A << 3) + 2), dict(apart, y=A << 3, ldy=50),
+               dict(apart, preact=A << 3), dict(apart, preact=A + 32), dict(apart, x=y + 96, ldx=49), dict(wide, x=y + 94), dict(wide, x=y + 224 - 62), dict(wide, x=y + 224 + 94),
+               dict(apart, y=A + 63 * 64 + 62), dict(apart, y=A - 64 * 96 + 2)):
+        assert lib.ccsm_train_linear_forward(nowhere, C.byref(_linear(**kw)), None, 0, None) == INVALID, kw
+        assert b"shares memory" in lib.ccsm_train_ops_last_error(), kw
+    far = dict(dy=A, w=A << 1, dx=A << 2, dw=A << 3, dbias=A << 4, x=ops.Saved(A << 5, 32, 1, A << 6, 1), preact=ops.Saved(A << 7, 64, 2, A << 8, 2))
+    for kw in (dict(dx=A), dict(dx=A << 1), dict(dw=(A << 5) + 64), dict(dw=(A << 6) + 2), dict(dbias=A << 7), dict(dbias=(A << 8) + 126), dict(dw=A << 2), dict(dbias=A << 3), dict(dbias=(A << 2) - 2)):
+        assert lib.ccsm_train_linear_backward(nowhere, C.byref(_grad(**dict(far, **kw))), A << 9, 1 << 40, None) == INVALID, kw
+        assert b"shares memory" in lib.ccsm_train_ops_last_error(), kw
+    for ids, table, out in ((A, A << 1, A), (A, A << 1, (A << 1) + 64), (A, A << 1, A - 156), (A, A << 1, A + 76)):
+        assert lib.ccsm_train_embedding_forward(nowhere, 0, 2, 10, ids, 5, 8, table, 8, 1.0, out, 8, None) == INVALID
+        assert lib.ccsm_train_embedding_backward(nowhere, 0, 2, 10, ids, 5, 8, table, 8, 1.0, out, 8, A << 9, 1 << 40, None) == INVALID
+    for x, codes, scales in ((A, A, A << 1), (A, A << 1, A + 48), (A, A << 1, (A << 1) + 255)):
+        assert lib.ccsm_train_act8_pack(nowhere, 0, 1, 4, 40, x, 40, codes, 64, scales, 2, None) == INVALID
+        assert b"share memory" in lib.ccsm_train_ops_last_error()
+    for y, codes, scales in ((A, A, A << 1), (A, A << 1, A + 48)):
+        assert lib.ccsm_train_act8_unpack(nowhere, 0, 4, 40, C.byref(ops.Saved(codes, 64, 1, scales, 2)), y, 40, None) == INVALID
+    apart = dict(apart, y=A << 4)
+    for kw in (apart, dict(wide, x=y + 96), dict(wide, x=y + 224 - 64), dict(apart, y=A << 3), dict(apart, residual=None, preact=None), dict(apart, y=A + 64 * 64), dict(apart, y=A - 64 * 96)):
+        assert lib.ccsm_train_linear_forward(nowhere, C.byref(_linear(**kw)), None, 0, None) == _lib.ERR_HIP, kw      # nothing is shared

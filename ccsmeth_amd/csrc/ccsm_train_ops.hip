@@ -51,6 +51,8 @@ constexpr int64_t kMostRows = 0x7fffff00, kMostCols = 0x00ffff00;
 // The tile kernels' offsets into an operand whose contraction index is contiguous: 255 rows and a row's 128 bytes, in the 32 bits of a buffer's extent.  A
 // caller's own stride is below kNarrow; a staged copy (and d) is as wide as the contraction.  16 bits: 8421504 columns, fp32: 4210752
 constexpr int64_t kExtent = 0xfffffffe;
+// slope_kernel takes 32 rows x 256 columns a workgroup; a launch has less than 2^32 lanes, staging's workgroups among them
+constexpr int64_t kSlopeBlocks = (1 << 24) - (1 << 16) - 1;
 
 size_t size_of(int type) { return type == CCSM_TYPE_F32 ? 4 : 2; }
 bool good_type(int t) { return t == CCSM_TYPE_F32 || t == CCSM_TYPE_F16 || t == CCSM_TYPE_BF16; }
@@ -341,6 +343,7 @@ ccsm_status check_grad(const ccsm_linear_grad* p) {
             ccsm_status e = check_saved(p->preact, p->type, p->outer, "linear_backward: an activation's slope needs the pre-activation");
             if (e != CCSM_OK) return e;
         }
+        REFUSE(cdiv(p->rows, 32) * cdiv(p->outer, 256) > kSlopeBlocks, "linear_backward: more rows than a launch covers");
         REFUSE(p->dx && !spanned(p->outer, p->type), "linear_backward: outer is too long for dx");
         if (p->dx) REFUSE(!p->w || p->ldw < p->inner || p->lddx < p->inner, "linear_backward: dx needs w, and strides of at least inner");
         if (p->dw) {

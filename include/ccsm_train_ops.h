@@ -13,7 +13,8 @@
  * Conventions: every pointer is device memory of `device`; all matrices of a call share one type; `ld*` are row strides in elements (at
  * least the row's width); rows, columns and strides may be odd and bases need the alignment of one element only (rows of whole, aligned
  * 16-byte pieces are fastest).  At most 0x7fffff00 rows and 0x00ffff00 columns; a contraction along rows (linear_forward over `inner` with more than
- * 64 rows, dx over `outer`) has at most 8421504 columns in 16 bits and 4210752 in fp32.  Work is enqueued on `stream` (NULL = the default stream) and never waits for the GPU, so every call can be
+ * 64 rows, dx over `outer`) has at most 8421504 columns in 16 bits and 4210752 in fp32; linear_backward takes up to 534773728 rows for each 256
+ * columns of `outer`.  Work is enqueued on `stream` (NULL = the default stream) and never waits for the GPU, so every call can be
  * captured into a graph; nothing is kept from one call for the next.  `workspace` is scratch of at least *_workspace() bytes, 256-byte
  * aligned, used until the enqueued work is done: calls that may run at the same time, two captured graphs among them, need one each.
  * The current device is the caller's again when a call returns.  Sums, activations and their slopes are computed in 32 bits or more and

@@ -237,3 +237,12 @@ def test_outputs_that_share_memory_are_refused():
     apart = dict(apart, y=A << 4)
     for kw in (apart, dict(wide, x=y + 96), dict(wide, x=y + 224 - 64), dict(apart, y=A << 3), dict(apart, residual=None, preact=None), dict(apart, y=A + 64 * 64), dict(apart, y=A - 64 * 96)):
         assert lib.ccsm_train_linear_forward(nowhere, C.byref(_linear(**kw)), None, 0, None) == _lib.ERR_HIP, kw      # nothing is shared
+
+
+def test_more_rows_than_a_launch_covers_are_refused():
+    """32 rows x 256 columns a workgroup of 256 lanes, 65536 more workgroups for what is staged: less than 2^32 lanes in all"""
+    lib, most = ops.load(), 534773728
+    assert (most // 32 + 65536) * 256 < 2 ** 32 and most % 32 == 0
+    for outer, rows, ok in ((1, most, True), (256, most, True), (256, most + 1, False), (257, most, False), (257, most // 2 // 32 * 32, True), (8, 0x7fffff00, False)):
+        g = _grad(rows=rows, inner=1, outer=outer, lddy=outer, ldw=1, lddx=1, lddw=1, x=ops.Saved(A, 1, 0, None, 0), preact=ops.Saved(A, outer, 0, None, 0))
+        assert lib.ccsm_train_linear_backward(1 << 20, C.byref(g), None, 0, None) == (CAPACITY if ok else INVALID), (outer, rows)

@@ -303,8 +303,7 @@ __global__ __launch_bounds__(256, 3) void piece_sum_kernel(const unsigned* keys,
         flush(after == cur);
         kind[j] = is;                                      // (every lane of the group writes the same)
     }
-    __syncthreads();
-    if (!on) return;
+    __syncthreads();                                       // (lanes without a piece stay for the barriers below)
     // head[j] <- what the pieces from j on add to a sum that is open in front of j: a scan from behind, in steps of 1, 2, 4 ... groups (one by one, 128
     // groups of two lanes took 16 us)
     const int live = (int)(((n - (long long)blockIdx.x * groups * kPiece) + kPiece - 1) / kPiece), end = live < groups ? live : groups;

@@ -146,8 +146,9 @@ def _same(t, name, dtype, at, lead):
 
 def _rows(t):
     """(tensor whose rows are contiguous, its row stride): t as it is, or a copy"""
-    if t.is_contiguous() and t.dim():
+    if t.is_contiguous() and t.dim() and not t.is_neg():
         return t, t.shape[-1]
+    t = t.resolve_neg()                                    # (the imaginary part of a conjugate: its memory holds the other sign)
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1]) if t.dim() else t.reshape(1, 1)
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
@@ -205,6 +206,8 @@ def _out(out, shape, dtype, device, name):
     if out.dim() > 1 and not out.is_contiguous() and (out.dim() != 2 or out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]) or \
             out.dim() == 1 and out.numel() > 1 and out.stride(0) != 1:
         raise ValueError("%s must have contiguous rows" % name)
+    if out.is_neg():
+        raise ValueError("%s is a view with its sign turned" % name)
     return out
 
 
@@ -312,7 +315,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=F
     z = x.new_empty(shape) if keep_preact else None
     x2, ldx = _rows(x)
     w2, ldw = _rows(weight)
-    b1 = None if bias is None else bias.contiguous()
+    b1 = None if bias is None else bias.resolve_neg().contiguous()
     r2, ldr = (None, 0) if residual is None else _rows(residual)
     p = _LINEAR.pack(_TYPE[t], act, x.numel() // inner, inner, outer, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b1), _ptr(r2), ldr, y.data_ptr(), ldy, _ptr(z), outer)
     need = lib.ccsm_train_linear_workspace(p)

@@ -246,3 +246,15 @@ def test_more_rows_than_a_launch_covers_are_refused():
     for outer, rows, ok in ((1, most, True), (256, most, True), (256, most + 1, False), (257, most, False), (257, most // 2 // 32 * 32, True), (8, 0x7fffff00, False)):
         g = _grad(rows=rows, inner=1, outer=outer, lddy=outer, ldw=1, lddx=1, lddw=1, x=ops.Saved(A, 1, 0, None, 0), preact=ops.Saved(A, outer, 0, None, 0))
         assert lib.ccsm_train_linear_backward(1 << 20, C.byref(g), None, 0, None) == (CAPACITY if ok else INVALID), (outer, rows)
+
+
+def test_views_with_their_sign_turned_are_copied():
+    ops._init()
+    c = torch.tensor([[1 + 2j, 3 - 4j], [5 + 6j, -7 - 8j]], dtype=torch.complex64)
+    for v in (c.conj().imag, c.conj().imag[:, :1], c.conj().imag[:1, :1], torch._neg_view(torch.ones(3, 4))):
+        assert v.is_neg()
+        t, ld = ops._rows(v)
+        assert not t.is_neg() and torch.equal(t, v.resolve_neg()) and ld >= t.shape[1]
+        with pytest.raises(ValueError):
+            ops._out(v, v.shape, torch.float32, v.device, "out")
+    assert ops._rows(c.real)[0].data_ptr() != c.data_ptr() and ops._rows(torch.ones(3, 4))[1] == 4

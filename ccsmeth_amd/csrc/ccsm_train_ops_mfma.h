@@ -195,7 +195,8 @@ __device__ __forceinline__ Place place_of(int b, int tiles_i, int tiles_j, int s
 // Sums of products of values in pieces are NaN wherever an operand is infinite (its other pieces are NaN, and infinity times an empty piece is), or where
 // the largest products pass fp32's range and smaller ones of the other sign do too.  A wave that finds a NaN among its results makes
 // those sums again from one piece of each value: infinities, opposite infinities, infinity times zero and NaN then give what they give in fp32.
-// Finite results cost the look (one instruction for two of them).
+// Finite results cost the look (one instruction for two of them).  Again costs a 16 x 16 tile its contraction step by step: 21504 x 512 -> 768 takes 100 us
+// more with one infinity, and 1.8 ms with an operand full of NaN.
 //
 // one piece of v: sign, exponent and seven bits; a NaN stays one, what is not zero does not become it
 __device__ __forceinline__ short leading(float v) {

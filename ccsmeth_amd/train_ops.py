@@ -328,6 +328,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", keep_preact=F
 
 def linear_backward(dy, x, weight, preact=None, activation="none", *, need_dx=True, need_dw=True, need_db=True, stream=None):
     """The gradients of y = act(x weight^T + bias) (+ residual, whose gradient is dy itself): (dx, dw, db), None for what is not needed.
+    Large 16-bit products with an activation take dy act'(preact) rounded to the type: their dx and dw carry two roundings (include/ccsm_train_ops.h).
     dy (..., outer); x (..., inner) and preact (..., outer) are tensors or Checkpoint8s; preact only where there is an activation."""
     lib = _library()
     act = _activation(activation)

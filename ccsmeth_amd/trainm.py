@@ -66,7 +66,7 @@ def build_parser():
     p.add_argument('--node_rank', type=int, default=0)
     p.add_argument('--epoch_sync', action="store_true", default=False)
     p.add_argument('--activation_bits', type=int, default=32, choices=(32, 8),
-                   help="what the forward pass keeps of the GRU gates: fp32, or int8 checkpoints (a fifth less memory per site; not a flag of the reference)")
+                   help="what the forward pass keeps of the GRU gates: fp32, or int8 checkpoints (a sixth less memory per site; not a flag of the reference)")
     return p
 
 

@@ -84,7 +84,9 @@ struct Scratch {
 
 // a matrix in memory: rows of `wide` bytes, `ld` bytes from one to the next
 struct Held { const void* p; int64_t ld, rows, wide; };
-Held held(const void* p, int64_t ld, int64_t rows, int64_t cols, size_t size) { return Held{p, ld * (int64_t)size, rows, cols * (int64_t)size}; }
+Held held(const void* p, int64_t ld, int64_t rows, int64_t cols, size_t size) {      // (one row's stride may be anything)
+    return Held{p, rows > 1 ? ld * (int64_t)size : 0, rows, cols * (int64_t)size};
+}
 // whether two of them share memory: their ranges meet, and they are not different columns of the same rows (of one row, the other's stride)
 bool meet(const Held& a, const Held& b) {
     if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;

@@ -770,3 +770,81 @@ def test_outputs_that_share_memory_are_refused():
     c = ops.Checkpoint8(room[:1280].view(40, 32), c.scales, c.shape, F32, "int8")
     with pytest.raises(CcsmError, match="shares memory"):
         c.values(out=room.view(F32).view(40, 32))
+
+
+# ---- sizes past 32 bits -------------------------------------------------------------------------------------------------
+def test_products_of_more_than_2_to_32_elements():
+    """x of 4.4e9 elements: the last rows are what a call on them alone gives, dw is the sum of its halves'"""
+    m, k, n = (1 << 23) + 77, 520, 16
+    x = torch.empty(m, k, dtype=BF16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(1))
+    w, dy = normal(2, n, k, t=BF16, by=k ** -0.5), normal(3, m, n, t=BF16, by=2.0 ** -6)
+    y = ops.linear(x, w)
+    for part in (slice(0, 1000), slice(m // 2, m // 2 + 1000), slice(m - 1000, m)):
+        check_linear(x[part], w, None, None, "none", BF16, y[part])
+    dx, dw, db = ops.linear_backward(dy, x, w)
+    ref, q = torch.zeros(n, k, dtype=torch.float64, device=DEV), torch.zeros(n, k, dtype=torch.float64, device=DEV)
+    for i in range(0, m, 1 << 20):
+        a, b = dy[i:i + (1 << 20)].double().t().contiguous(), x[i:i + (1 << 20)].double()
+        ref += mm(a, b)
+        q += mm(a ** 2, b ** 2)
+    within(dw, ref, sum_tol(m) * q.sqrt(), BF16)
+    within(db, dy.double().sum(0), sum_tol(m) * (dy.double() ** 2).sum(0).sqrt(), BF16)
+    d, w6 = dy[m - 1000:].double(), w.double()
+    within(dx[m - 1000:], mm(d, w6), sum_tol(n) * mm(d ** 2, w6 ** 2).sqrt(), BF16)
+
+
+def test_lookups_of_more_than_2_to_30_pieces():
+    """what a launch covers, and 40 tokens more; dy of more than 2^32 elements"""
+    tokens, rows, width = (1 << 27) + 40, 251, 64
+    table = normal(1, rows, width, t=BF16)
+    ids = (torch.arange(tokens, device=DEV) % rows).to(torch.uint8)
+    y = ops.embedding(ids, table)
+    for at in (0, (1 << 27) - rows, tokens - rows):
+        assert torch.equal(y[at:at + rows], table[ids[at:at + rows].long()])
+    y.normal_(generator=torch.Generator(DEV).manual_seed(1))
+    d = ops.embedding_backward(y, ids, rows)
+    ref, sq = torch.zeros(rows, width, dtype=torch.float64, device=DEV), torch.zeros(rows, width, dtype=torch.float64, device=DEV)
+    for i in range(0, tokens, rows << 13):                            # (whole rounds of ids, and the last one's start)
+        v = y[i:i + (rows << 13)].double()
+        whole = len(v) // rows * rows
+        ref += v[:whole].view(-1, rows, width).sum(0)
+        sq += (v[:whole] ** 2).view(-1, rows, width).sum(0)
+        ref[:len(v) - whole] += v[whole:]
+        sq[:len(v) - whole] += v[whole:] ** 2
+    n = torch.bincount(ids.long(), minlength=rows).double().sqrt()[:, None]
+    within(d, ref, 2.0 ** -24 * (8 * n + 8) * sq.sqrt(), BF16)
+
+
+def test_checkpoints_of_more_than_2_to_30_pieces():
+    rows, width = (1 << 29) + 40, 17
+    x = torch.empty(rows, width, dtype=BF16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(2))
+    c = ops.checkpoint8(x, "int8")
+    v = c.values()
+    for at in (0, (1 << 29) - 100, rows - 100):
+        same(v[at:at + 100], in8(x[at:at + 100], "int8"))
+        assert not c.codes[at:at + 100, width:].any()
+
+
+def test_single_rows_and_tokens():
+    """one token without a row of ids, one row without rows, checkpoints of one value, of leading dimensions and into a caller's tensor"""
+    for t in TYPES:
+        w, x = normal(1, 12, 20, t=t), normal(2, 20, t=t)
+        y = ops.linear(x, w, activation="gelu")
+        assert y.shape == (12,) and torch.equal(y, ops.linear(x[None], w, activation="gelu")[0])
+        a, b = ops.linear_backward(y, x, w), ops.linear_backward(y[None], x[None], w)
+        assert a[0].shape == (20,) and torch.equal(a[0], b[0][0]) and torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+        i = torch.tensor(3, device=DEV)
+        e = ops.embedding(i, w, 0.5)
+        assert e.shape == (20,) and torch.equal(e, (w[3].float() * 0.5).to(t))
+        g = ops.embedding_backward(e, i, 12)
+        assert torch.equal(g[3], e) and not g[:3].any() and not g[4:].any()
+        one = ops.checkpoint8(x[:1], "e4m3")
+        assert one.values().shape == (1,) and one.codes.shape == (1, 32)
+        v = normal(3, 2, 3, 20, t=t)
+        c = ops.checkpoint8(v)
+        hold = torch.full((6, 25), 7.0, dtype=t, device=DEV)
+        same(c.values(), in8(v, "int8"))
+        c2 = ops.checkpoint8(v.reshape(6, 20))
+        assert c2.values(out=hold[:, 2:22]) is not None and torch.equal(hold[:, 2:22], c.values().reshape(6, 20))
+        hold[:, 2:22] = 7.0
+        assert bool((hold == 7).all())

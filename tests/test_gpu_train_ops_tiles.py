@@ -144,3 +144,23 @@ def test_fp16_gradients_of_small_and_large_dy(by):
     dy, x, w, z = normal(1, m, n, t=F16, by=by), normal(2, m, k, t=F16, by=min(1.0, 1 / by)), normal(3, n, k, t=F16, by=k ** -0.5), normal(4, m, n, t=F16)
     assert way_backward(dy, x, w, z, "gelu") == (256, False, True)
     base.check_range(dy, x, w, z, "gelu", F16, ops.linear_backward(dy, x, w, z, activation="gelu"), base.H[F16])
+
+
+@pytest.mark.parametrize("t,k,tile", [(F32, 4210752, 256), (F16, 8421504, 256), (BF16, 8421504 - 3, 256)])
+def test_the_longest_contraction(t, k, tile):
+    """offsets of the last rows' last pieces end 126 bytes below 2^32; first and last rows differ"""
+    m = n = 256
+    g = torch.Generator(DEV)
+    x, w = (torch.empty(m, k, dtype=t, device=DEV).normal_(generator=g.manual_seed(s)) for s in (1, 2))
+    assert way_forward(x, w, torch.empty(m, n, dtype=t, device=DEV))[0] == tile
+    w *= 2.0 ** -11
+    ref, q = torch.zeros(m, n, dtype=torch.float64, device=DEV), torch.zeros(m, n, dtype=torch.float64, device=DEV)
+    for i in range(0, k, 1 << 18):
+        a, b = x[:, i:i + (1 << 18)].double(), w[:, i:i + (1 << 18)].double().t()
+        ref += torch.mm(a, b.contiguous())
+        q += torch.mm(a ** 2, (b ** 2).contiguous())
+    base.within(ops.linear(x, w), ref, base.sum_tol(k) * q.sqrt(), t)
+    dx, _, db = ops.linear_backward(x, None, w.t().contiguous(), need_dw=False)        # (m, k) by (k, n): the same sums
+    base.within(dx, ref, base.sum_tol(k) * q.sqrt(), t)
+    base.within(db[:1000], x[:, :1000].double().sum(0), base.sum_tol(m) * (x[:, :1000].double() ** 2).sum(0).sqrt(), t)
+    base.within(db[k - 1000:], x[:, k - 1000:].double().sum(0), base.sum_tol(m) * (x[:, k - 1000:].double() ** 2).sum(0).sqrt(), t)

@@ -20,7 +20,8 @@
  * The current device is the caller's again when a call returns.  Sums, activations and their slopes are computed in 32 bits or more and
  * rounded once, with one exception: linear_backward in 16 bits takes d = dy act'(z) rounded to its type into dx and dw (not into dbias) where an
  * activation meets products in tiles (ccsm_train_linear_backward_way), so that those gradients carry two roundings, sqrt 2 times the error of
- * one.  fp16's d is brought into the type's range by a power of two first.  Smaller products keep d to 2^-16.  fp32 products are made of bf16
+ * one.  fp16's d is brought into the type's range by a power of two first (a d below 2^-28 of dy's largest finite magnitude A is off by up to
+ * 2^-39 A).  Smaller products keep d to 2^-16.  fp32 products are made of bf16
  * pieces; what is left out is below 2^-22 of each product, 2^-25 in the mean.  Infinities and NaN of operands give what they give in the
  * formulas above.  Results do not depend on timing (no floating-point atomics).  Outputs share no memory with inputs or each other, except y the residual
  * (same base and stride); columns of the same rows are apart, other views whose ranges of memory meet count as shared.  Zero rows (or tokens) are allowed: gradients of weights are then zero.  Refusals: CCSM_ERR_INVALID_ARG (text in

@@ -12,20 +12,21 @@
  *
  * Conventions: every pointer is device memory of `device`; all matrices of a call share one type; `ld*` are row strides in elements (at
  * least the row's width); rows, columns and strides may be odd and bases need the alignment of one element only (rows of whole, aligned
- * 16-byte pieces are fastest).  At most 0x7fffff00 rows and 0x00ffff00 columns; a contraction along rows (linear_forward over `inner` with more than
- * 64 rows, dx over `outer`) has at most 8421504 columns in 16 bits and 4210752 in fp32; linear_backward takes up to 534773728 rows for each 256
- * columns of `outer`.  Work is enqueued on `stream` (NULL = the default stream) and never waits for the GPU, so every call can be
- * captured into a graph; nothing is kept from one call for the next.  `workspace` is scratch of at least *_workspace() bytes, 256-byte
- * aligned, used until the enqueued work is done: calls that may run at the same time, two captured graphs among them, need one each.
- * The current device is the caller's again when a call returns.  Sums, activations and their slopes are computed in 32 bits or more and
- * rounded once, with one exception: linear_backward in 16 bits takes d = dy act'(z) rounded to its type into dx and dw (not into dbias) where an
- * activation meets products in tiles (ccsm_train_linear_backward_way), so that those gradients carry two roundings, sqrt 2 times the error of
- * one.  fp16's d is brought into the type's range by a power of two first (a d below 2^-28 of dy's largest finite magnitude A is off by up to
- * 2^-39 A).  Smaller products keep d to 2^-16.  fp32 products are made of bf16
- * pieces; what is left out is below 2^-22 of each product, 2^-25 in the mean.  Infinities and NaN of operands give what they give in the
- * formulas above.  Results do not depend on timing (no floating-point atomics).  Outputs share no memory with inputs or each other, except y the residual
- * (same base and stride); columns of the same rows are apart, other views whose ranges of memory meet count as shared.  Zero rows (or tokens) are allowed: gradients of weights are then zero.  Refusals: CCSM_ERR_INVALID_ARG (text in
- * ccsm_train_ops_last_error), CCSM_ERR_CAPACITY for a workspace that is too small.
+ * 16-byte pieces are fastest).  At most 0x7fffff00 rows and 0x00ffff00 columns; a contraction along rows (linear_forward over `inner` with
+ * more than 64 rows, dx over `outer`) has at most 8421504 columns in 16 bits and 4210752 in fp32; linear_backward takes up to 534773728
+ * rows for each 256 columns of `outer`.  Work is enqueued on `stream` (NULL = the default stream) and never waits for the GPU, so every
+ * call can be captured into a graph; nothing is kept from one call for the next.  `workspace` is scratch of at least *_workspace() bytes,
+ * 256-byte aligned, used until the enqueued work is done: calls that may run at the same time, two captured graphs among them, need one
+ * each. The current device is the caller's again when a call returns.  Sums, activations and their slopes are computed in 32 bits or more
+ * and rounded once, with one exception: linear_backward in 16 bits takes d = dy act'(z) rounded to its type into dx and dw (not into dbias)
+ * where an activation meets products in tiles (ccsm_train_linear_backward_way), so that those gradients carry two roundings, sqrt 2 times
+ * the error of one.  fp16's d is brought into the type's range by a power of two first (a d below 2^-28 of dy's largest finite magnitude A
+ * is off by up to 2^-39 A).  Smaller products keep d to 2^-16.  fp32 products are made of bf16 pieces; what is left out is below 2^-22 of
+ * each product, 2^-25 in the mean.  Infinities and NaN of operands give what they give in the formulas above.  Results do not depend on
+ * timing (no floating-point atomics).  Outputs share no memory with inputs or each other, except y the residual (same base and stride);
+ * columns of the same rows are apart, other views whose ranges of memory meet count as shared.  Zero rows (or tokens) are allowed:
+ * gradients of weights are then zero.  Refusals: CCSM_ERR_INVALID_ARG (text in ccsm_train_ops_last_error), CCSM_ERR_CAPACITY for a
+ * workspace that is too small.
  */
 #ifndef CCSM_TRAIN_OPS_H_
 #define CCSM_TRAIN_OPS_H_
